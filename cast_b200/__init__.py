@@ -7,6 +7,8 @@ Public API:
 * :class:`cast_b200.par.FCPASMCorrector`
 * :class:`cast_b200.select.TABASelector`
 * :func:`cast_b200.components.make_cast_components` (reference-package drop-in)
+* :func:`cast_b200.rotary.rope`, :func:`cast_b200.rotary.qk_norm_rope`
+* :func:`cast_b200.window.window_attention`, :func:`cast_b200.window.paged_window_attention`
 * :mod:`cast_b200.distributed` (head / rollout sharding over NCCL)
 
 Kernels live in ``libcast_b200.so`` (built by ``python -m cast_b200.build``).
@@ -21,6 +23,8 @@ from .rcsa import (  # noqa: F401
     rcsa_attention,
     select_quant,
 )
+from .rotary import qk_norm_rope, rope, rope_frequencies, rope_table  # noqa: F401
+from .window import paged_window_attention, window_attention  # noqa: F401
 from .par import FCPASMCorrector  # noqa: F401
 from .select import TABASelector  # noqa: F401
 

@@ -103,6 +103,29 @@ SIGNATURES = {
          c_void_p, c_void_p, c_void_p],
     ),
     "cast_swap_route_workspace_bytes": (c_size_t, [c_int] * 10),
+    "cast_rope": (
+        c_int,
+        [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_longlong, c_longlong, c_void_p]
+        + [c_int] * 6 + [c_void_p, c_void_p, c_void_p],
+    ),
+    "cast_qk_norm_rope": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_float,
+         c_void_p, c_int, c_void_p, c_int, c_longlong, c_longlong, c_void_p] + [c_int] * 7
+        + [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
+    ),
+    "cast_window_attention": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_int, c_void_p] + [c_int] * 6
+        + [c_void_p, c_longlong, c_longlong, c_int, c_float, c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
+    "cast_window_attention_workspace_bytes": (c_size_t, [c_int] * 6 + [c_longlong, c_longlong, c_int]),
+    "cast_paged_window_attention": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_void_p] + [c_int] * 5
+        + [c_void_p, c_longlong, c_longlong, c_int, c_float, c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
+    "cast_paged_window_attention_workspace_bytes": (c_size_t, [c_int] * 7 + [c_longlong, c_longlong, c_int]),
     "cast_par_fcpasm": (
         c_int,
         [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float,

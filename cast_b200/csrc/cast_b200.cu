@@ -17,6 +17,8 @@
 #include "compact.cuh"
 #include "barycentric.cuh"
 #include "swap_router.cuh"
+#include "rotary.cuh"
+#include "window.cuh"
 
 namespace cast {
 
@@ -1121,6 +1123,373 @@ extern "C" int cast_compact_unpack(const void *packed, const int32_t *token_to_p
       static_cast<__nv_bfloat16 *>(out));
   CAST_CUDA_TRY(cudaGetLastError());
   return CAST_OK;
+}
+
+// ===========================================================================
+// rotary positions, and the norm of query / key heads with the rotation
+// ===========================================================================
+enum { kBf16 = 0, kFp32 = 1, kFp16 = 2 };
+
+static bool dtype_ok(int t) { return t == kBf16 || t == kFp32 || t == kFp16; }
+
+// 16-byte pieces: strides of a 2-byte type are multiples of 8 elements, of
+// float32 multiples of 4.
+static bool strides_ok(const long long *s, int n, int dtype) {
+  for (int i = 0; i < n; ++i)
+    if (s[i] % (dtype == kFp32 ? 4 : 8)) return false;
+  return true;
+}
+
+struct RotaryPositions {
+  const float *table;
+  int table_rows;
+  const void *positions;
+  int positions_64;
+  long long pos_batch_stride, first_position;
+  const int *axes;
+};
+
+// Checks shared by both entry points and the parameters they share.
+static int rotary_params(castk::RotaryParams &p, const RotaryPositions &at, int B, int L, int heads,
+                         int D, int R, int flags) {
+  if (B <= 0 || L <= 0 || heads <= 0) return fail(CAST_ERR_INVALID_ARGUMENT, "non-positive size");
+  if (D <= 0 || D % 8 || D > 256)
+    return fail(CAST_ERR_UNSUPPORTED, "head_dim %d (supported: multiples of 8 up to 256)", D);
+  if (flags & ~3) return fail(CAST_ERR_INVALID_ARGUMENT, "flags %d", flags);
+  const bool half = !(flags & 1);
+  if (R < 0 || R > D) return fail(CAST_ERR_INVALID_ARGUMENT, "rotated part %d of head_dim %d", R, D);
+  if (R % (half ? 16 : 8))
+    return fail(CAST_ERR_UNSUPPORTED, "rotated part %d (multiples of %d in this layout)", R, half ? 16 : 8);
+  if (R > 0) {
+    if (!at.table || at.table_rows <= 0) return fail(CAST_ERR_INVALID_ARGUMENT, "a rotation needs a table");
+    if (!aligned16(at.table)) return fail(CAST_ERR_ALIGNMENT, "the table must be 16-byte aligned");
+  }
+  memset(&p, 0, sizeof(p));
+  p.n_axes = 1;
+  p.axis_end0 = p.axis_end1 = R / 2;
+  if (at.axes && R > 0) {
+    if (at.axes[0] < 0 || at.axes[1] < 0 || at.axes[2] < 0 ||
+        (long long)at.axes[0] + at.axes[1] + at.axes[2] != R / 2)
+      return fail(CAST_ERR_INVALID_ARGUMENT, "axes %d + %d + %d pairs of %d", at.axes[0], at.axes[1], at.axes[2], R / 2);
+    if (!at.positions) return fail(CAST_ERR_INVALID_ARGUMENT, "positions on three axes must be given");
+    p.n_axes = 3;
+    p.axis_end0 = at.axes[0];
+    p.axis_end1 = at.axes[0] + at.axes[1];
+  }
+  p.table = at.table;
+  p.table_rows = at.table_rows;
+  p.positions = at.positions;
+  p.pos64 = at.positions_64;
+  p.pos_batch_stride = at.pos_batch_stride;
+  p.first_position = at.first_position;
+  p.tokens = (long long)B * L;
+  p.L = L;
+  p.D = D;
+  p.R = R;
+  p.heads = heads;
+  p.inverse = (flags >> 1) & 1;
+  p.lanes = 8;
+  while (p.lanes < D / 8) p.lanes *= 2;
+  const int slots = castk::kRotaryThreads / p.lanes;
+  p.slots_per_token = 1;
+  while (p.slots_per_token < slots && p.slots_per_token < heads) p.slots_per_token *= 2;
+  p.tokens_per_cta = slots / p.slots_per_token;
+  if ((p.tokens + p.tokens_per_cta - 1) / p.tokens_per_cta >= (1ll << 31))
+    return fail(CAST_ERR_UNSUPPORTED, "%lld tokens in one call", p.tokens);
+  return CAST_OK;
+}
+
+template <typename InT, typename OutT>
+static int launch_rotary(const castk::RotaryParams &p, bool norm, bool half, cudaStream_t s) {
+  const unsigned grid = (unsigned)((p.tokens + p.tokens_per_cta - 1) / p.tokens_per_cta);
+  if (norm && half)
+    castk::rotary_kernel<InT, OutT, true, true><<<grid, castk::kRotaryThreads, 0, s>>>(p);
+  else if (norm)
+    castk::rotary_kernel<InT, OutT, true, false><<<grid, castk::kRotaryThreads, 0, s>>>(p);
+  else if (half)
+    castk::rotary_kernel<InT, OutT, false, true><<<grid, castk::kRotaryThreads, 0, s>>>(p);
+  else
+    castk::rotary_kernel<InT, OutT, false, false><<<grid, castk::kRotaryThreads, 0, s>>>(p);
+  CAST_CUDA_TRY(cudaGetLastError());
+  return CAST_OK;
+}
+
+static int launch_rotary(const castk::RotaryParams &p, int dtype, int out_dtype, bool norm, bool half,
+                         cudaStream_t s) {
+  if (dtype == kBf16) return launch_rotary<__nv_bfloat16, __nv_bfloat16>(p, norm, half, s);
+  if (dtype == kFp16) return launch_rotary<__half, __half>(p, norm, half, s);
+  if (out_dtype == kFp32) return launch_rotary<float, float>(p, norm, half, s);
+  return launch_rotary<float, __nv_bfloat16>(p, norm, half, s);
+}
+
+static void rotary_tensor(castk::RotaryTensor &t, const void *src, void *dst, const void *weight, int heads,
+                          const long long *ss, const long long *ds) {
+  t.src = src;
+  t.dst = dst;
+  t.weight = weight;
+  t.heads = heads;
+  for (int i = 0; i < 3; ++i) {
+    t.ss[i] = ss[i];
+    t.ds[i] = ds ? ds[i] : 0;
+  }
+}
+
+extern "C" int cast_rope(const void *x, int dtype, const float *table, int table_rows, const void *positions,
+                         int positions_64, long long pos_batch_stride, long long first_position,
+                         const int *axes, int B, int L, int H, int D, int R, int flags,
+                         const long long *strides, void *out, cast_stream_t stream) {
+  if (!x || !out || !strides) return fail(CAST_ERR_INVALID_ARGUMENT, "x, strides and out are required");
+  if (!dtype_ok(dtype)) return fail(CAST_ERR_INVALID_ARGUMENT, "dtype %d (0 = bf16, 1 = fp32, 2 = fp16)", dtype);
+  castk::RotaryParams p;
+  int st = rotary_params(p, {table, table_rows, positions, positions_64, pos_batch_stride, first_position, axes},
+                         B, L, H, D, R, flags);
+  if (st) return st;
+  if (!aligned16(x) || !aligned16(out) || !strides_ok(strides, 6, dtype))
+    return fail(CAST_ERR_ALIGNMENT, "x and out must start, and their strides step, on 16-byte boundaries");
+  if ((st = current_device_sm100(nullptr))) return st;
+  rotary_tensor(p.t[0], x, out, nullptr, H, strides, strides + 3);
+  return launch_rotary(p, dtype, dtype, false, !(flags & 1), reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int cast_qk_norm_rope(const void *q, const void *k, const void *v, int dtype, int out_dtype,
+                                 const void *q_weight, const void *k_weight, int weight_fp32,
+                                 int weight_per_head, float eps, const float *table, int table_rows,
+                                 const void *positions, int positions_64, long long pos_batch_stride,
+                                 long long first_position, const int *axes, int B, int L, int Hq, int Hk,
+                                 int D, int R, int flags, const long long *strides, void *q_out,
+                                 void *k_out, void *v_out, const void *slots, int slots_64, int n_pages,
+                                 int page, cast_stream_t stream) {
+  if (!q || !k || !strides || !q_out || !k_out)
+    return fail(CAST_ERR_INVALID_ARGUMENT, "q, k, strides, q_out and k_out are required");
+  if (!dtype_ok(dtype) || !dtype_ok(out_dtype))
+    return fail(CAST_ERR_INVALID_ARGUMENT, "dtype %d, out_dtype %d (0 = bf16, 1 = fp32, 2 = fp16)", dtype, out_dtype);
+  if (out_dtype != dtype && !(dtype == kFp32 && out_dtype == kBf16))
+    return fail(CAST_ERR_UNSUPPORTED, "out_dtype %d of dtype %d (the same, or bf16 of fp32)", out_dtype, dtype);
+  if ((v != nullptr) != (v_out != nullptr) || (slots != nullptr) != (v != nullptr))
+    return fail(CAST_ERR_INVALID_ARGUMENT, "v, v_out and slots come together");
+  if (Hq <= 0 || Hk <= 0 || Hq > 65536 || Hk > 65536)
+    return fail(CAST_ERR_INVALID_ARGUMENT, "%d query and %d key heads", Hq, Hk);
+  if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(CAST_ERR_INVALID_ARGUMENT, "eps must be finite, 0 or more");
+  if (slots && (n_pages <= 0 || page <= 0)) return fail(CAST_ERR_INVALID_ARGUMENT, "non-positive cache size");
+  castk::RotaryParams p;
+  int st = rotary_params(p, {table, table_rows, positions, positions_64, pos_batch_stride, first_position, axes},
+                         B, L, Hq + (v ? 2 : 1) * Hk, D, R, flags);
+  if (st) return st;
+  if (!aligned16(q) || !aligned16(k) || (v && !aligned16(v)) || !aligned16(q_out) || !aligned16(k_out) ||
+      (v_out && !aligned16(v_out)) || (q_weight && !aligned16(q_weight)) || (k_weight && !aligned16(k_weight)) ||
+      !strides_ok(strides, v ? 9 : 6, dtype) || !strides_ok(strides + 9, 6, out_dtype))
+    return fail(CAST_ERR_ALIGNMENT, "tensors must start, and their strides step, on 16-byte boundaries");
+  if ((st = current_device_sm100(nullptr))) return st;
+  rotary_tensor(p.t[0], q, q_out, q_weight, Hq, strides, strides + 9);
+  rotary_tensor(p.t[1], k, k_out, k_weight, Hk, strides + 3, strides + 12);
+  if (v) rotary_tensor(p.t[2], v, v_out, nullptr, Hk, strides + 6, nullptr);
+  p.weight_f32 = weight_fp32;
+  p.weight_per_head = weight_per_head;
+  p.eps = eps;
+  p.slots = slots;
+  p.slots64 = slots_64;
+  p.n_slots = (long long)n_pages * page;
+  p.page = page;
+  return launch_rotary(p, dtype, out_dtype, q_weight || k_weight, !(flags & 1), reinterpret_cast<cudaStream_t>(stream));
+}
+
+// ===========================================================================
+// sliding-window attention with sinks
+// ===========================================================================
+struct RowsPlan {
+  int mt = 1, row_tiles = 1, n_split = 1;
+  bool cluster = false;  // joined in a cluster (else through the workspace, or nothing to join)
+  size_t ws_bytes = 0;
+};
+
+// How the few-row kernel cuts a call.  Two of its CTAs fit on an SM and a CTA
+// keeps 48 KB of copies in flight, so the keys of a tile of rows are split
+// until there are two CTAs for each SM, or until a part has 128 keys (two
+// groups of 16 for each of its warps).  Up to eight parts are joined in a
+// cluster; more go through the workspace.
+static RowsPlan rows_plan(long long B, int Hk, int group, int Lq, int capacity, long long window,
+                          long long sinks, int frame, int D, int n_sms) {
+  RowsPlan r;
+  const long long rows = (long long)group * Lq;
+  r.mt = rows <= 16 ? 1 : 2;
+  r.row_tiles = (int)((rows + 16 * r.mt - 1) / (16 * r.mt));
+  const long long items = B * Hk * r.row_tiles;
+  const long long tokens = std::min<long long>(Lq, 16 * r.mt / group + 2);
+  const double span = std::min<double>(capacity, (double)(window + sinks + 1) * frame + (double)tokens);
+  const long long most = std::max<long long>(1, (long long)(span / 128));
+  const long long want = std::max<long long>(1, 2ll * n_sms / items);
+  long long n = std::min(most, want);
+  if (n <= castk::kRowsMaxCluster) {
+    long long c = 1;
+    while (2 * c <= n) c *= 2;
+    r.n_split = (int)c;
+    r.cluster = c > 1;
+  } else {
+    r.n_split = (int)n;
+    r.ws_bytes = (size_t)items * n * (16 * r.mt) * (D + 4) * sizeof(float);
+  }
+  return r;
+}
+
+template <typename T, int D, int MT, bool kPaged>
+static int launch_rows(const castk::RowsParams &p, const RowsPlan &plan, cudaStream_t s) {
+  using S = castk::RowsSmem<T, D, MT, kPaged>;
+  auto kernel = castk::window_rows_kernel<T, D, MT, kPaged>;
+  static std::once_flag once;
+  static cudaError_t err = cudaSuccess;
+  std::call_once(once, [&] {
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes);
+  });
+  CAST_CUDA_TRY(err);
+  const long long items = (long long)p.B * p.Hk * p.row_tiles;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(items * p.n_split));
+  cfg.blockDim = dim3(castk::kRowsWarps * 32);
+  cfg.dynamicSmemBytes = S::bytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  if (plan.cluster) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = p.n_split;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+  CAST_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p));
+  if (p.part) {
+    castk::window_rows_join_kernel<T, D, MT, kPaged><<<(unsigned)(items * castk::kJoinShare), 128, 0, s>>>(p);
+    CAST_CUDA_TRY(cudaGetLastError());
+  }
+  return CAST_OK;
+}
+
+template <bool kPaged>
+static int launch_rows(const castk::RowsParams &p, const RowsPlan &plan, int dtype, int D, cudaStream_t s) {
+  using bf16 = __nv_bfloat16;
+  if (dtype == kBf16 && D == 128)
+    return plan.mt == 1 ? launch_rows<bf16, 128, 1, kPaged>(p, plan, s) : launch_rows<bf16, 128, 2, kPaged>(p, plan, s);
+  if (dtype == kBf16)
+    return plan.mt == 1 ? launch_rows<bf16, 64, 1, kPaged>(p, plan, s) : launch_rows<bf16, 64, 2, kPaged>(p, plan, s);
+  if (D == 128)
+    return plan.mt == 1 ? launch_rows<__half, 128, 1, kPaged>(p, plan, s) : launch_rows<__half, 128, 2, kPaged>(p, plan, s);
+  return plan.mt == 1 ? launch_rows<__half, 64, 1, kPaged>(p, plan, s) : launch_rows<__half, 64, 2, kPaged>(p, plan, s);
+}
+
+static int window_dims_ok(int B, int Hq, int Hk, int Lq, int Lk, int D, long long window, long long sinks,
+                          int frame) {
+  if (B <= 0 || Hq <= 0 || Hk <= 0 || Lq <= 0 || Lk <= 0) return fail(CAST_ERR_INVALID_ARGUMENT, "non-positive size");
+  if (Hq % Hk) return fail(CAST_ERR_INVALID_ARGUMENT, "%d query heads do not share %d key heads evenly", Hq, Hk);
+  if (D != 64 && D != 128) return fail(CAST_ERR_UNSUPPORTED, "window attention head_dim %d (supported: 64, 128)", D);
+  if (window <= 0 || sinks < 0 || frame <= 0)
+    return fail(CAST_ERR_INVALID_ARGUMENT, "window %lld (at least 1), sinks %lld (at least 0), frame_tokens %d (at least 1)",
+                window, sinks, frame);
+  if ((long long)Hq / Hk * Lq >= (1ll << 30) || (long long)B * Hq >= (1ll << 24) || Lk >= (1 << 30))
+    return fail(CAST_ERR_UNSUPPORTED, "size outside the kernels' index range");
+  return CAST_OK;
+}
+
+static int rows_call(castk::RowsParams &p, const RowsPlan &plan, bool paged, int dtype, int D, void *workspace,
+                     size_t workspace_bytes, cudaStream_t s) {
+  if ((long long)p.B * p.Hk * plan.row_tiles * std::max(plan.n_split, castk::kJoinShare) >= (1ll << 31))
+    return fail(CAST_ERR_UNSUPPORTED, "size outside the kernels' grid");
+  p.row_tiles = plan.row_tiles;
+  p.n_split = plan.n_split;
+  p.part = nullptr;
+  if (plan.ws_bytes) {
+    if (!workspace || workspace_bytes < plan.ws_bytes)
+      return fail(CAST_ERR_WORKSPACE, "workspace of %zu bytes < %zu required", workspace ? workspace_bytes : 0, plan.ws_bytes);
+    if (!aligned16(workspace)) return fail(CAST_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+    p.part = static_cast<float *>(workspace);
+  }
+  return paged ? launch_rows<true>(p, plan, dtype, D, s) : launch_rows<false>(p, plan, dtype, D, s);
+}
+
+static int rows_params(castk::RowsParams &p, const void *q, const void *k, const void *v, int dtype,
+                       const int32_t *kv_lens, int B, int Hq, int Hk, int Lq, int Lk, const long long *strides,
+                       long long window, long long sinks, int frame, float sm_scale, void *out) {
+  if (!q || !k || !v || !out || !strides) return fail(CAST_ERR_INVALID_ARGUMENT, "q, k, v, strides and out are required");
+  if (dtype != kBf16 && dtype != kFp16)
+    return fail(CAST_ERR_UNSUPPORTED, "dtype %d (0 = bf16, 2 = fp16)", dtype);
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !strides_ok(strides, 12, dtype))
+    return fail(CAST_ERR_ALIGNMENT, "tensors must start, and their strides step, on 16-byte boundaries");
+  if (!(sm_scale > 0.0f) || !std::isfinite(sm_scale))
+    return fail(CAST_ERR_INVALID_ARGUMENT, "sm_scale must be positive and finite");
+  memset(&p, 0, sizeof(p));
+  p.q = q, p.k = k, p.v = v, p.out = out;
+  for (int i = 0; i < 3; ++i) {
+    p.qs[i] = strides[i];
+    p.ks[i] = strides[3 + i];
+    p.vs[i] = strides[6 + i];
+    p.os[i] = strides[9 + i];
+  }
+  p.kv_lens = kv_lens;
+  // (no key lies 2^31 frames back, so larger windows and sinks are the same)
+  p.rule.window = std::min(window, 1ll << 31);
+  p.rule.sinks = std::min(sinks, 1ll << 31);
+  p.rule.frame = frame;
+  p.B = B, p.Hq = Hq, p.Hk = Hk, p.Lq = Lq, p.lk = Lk;
+  p.group = Hq / Hk;
+  p.rows = p.group * Lq;
+  p.scale_log2 = sm_scale * 1.4426950408889634f;
+  return CAST_OK;
+}
+
+extern "C" size_t cast_window_attention_workspace_bytes(int B, int Hq, int Hk, int Lq, int Lk, int D,
+                                                        long long window, long long sinks, int frame_tokens) {
+  int n_sms = 0;
+  if (window_dims_ok(B, Hq, Hk, Lq, Lk, D, window, sinks, frame_tokens) || current_device_sm100(&n_sms)) return 0;
+  return rows_plan(B, Hk, Hq / Hk, Lq, Lk, window, sinks, frame_tokens, D, n_sms).ws_bytes;
+}
+
+extern "C" int cast_window_attention(const void *q, const void *k, const void *v, int dtype,
+                                     const int32_t *kv_lens, int B, int Hq, int Hk, int Lq, int Lk, int D,
+                                     const long long *strides, long long window, long long sinks,
+                                     int frame_tokens, float sm_scale, void *out, void *workspace,
+                                     size_t workspace_bytes, cast_stream_t stream) {
+  int st = window_dims_ok(B, Hq, Hk, Lq, Lk, D, window, sinks, frame_tokens);
+  if (st) return st;
+  castk::RowsParams p;
+  st = rows_params(p, q, k, v, dtype, kv_lens, B, Hq, Hk, Lq, Lk, strides, window, sinks, frame_tokens, sm_scale, out);
+  if (st) return st;
+  int n_sms = 0;
+  if ((st = current_device_sm100(&n_sms))) return st;
+  const RowsPlan plan = rows_plan(B, Hk, p.group, Lq, Lk, window, sinks, frame_tokens, D, n_sms);
+  return rows_call(p, plan, false, dtype, D, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t cast_paged_window_attention_workspace_bytes(int B, int Hq, int Hk, int Lq, int D, int page,
+                                                              int max_pages, long long window,
+                                                              long long sinks, int frame_tokens) {
+  int n_sms = 0;
+  const long long cap = (long long)page * max_pages;
+  if (page <= 0 || max_pages <= 0 || cap >= (1 << 30) ||
+      window_dims_ok(B, Hq, Hk, Lq, (int)cap, D, window, sinks, frame_tokens) || current_device_sm100(&n_sms))
+    return 0;
+  return rows_plan(B, Hk, Hq / Hk, Lq, (int)cap, window, sinks, frame_tokens, D, n_sms).ws_bytes;
+}
+
+extern "C" int cast_paged_window_attention(const void *q, const void *k_pages, const void *v_pages, int dtype,
+                                           const int32_t *block_table, int max_pages, int n_pages, int page,
+                                           const int32_t *kv_lens, int B, int Hq, int Hk, int Lq, int D,
+                                           const long long *strides, long long window, long long sinks,
+                                           int frame_tokens, float sm_scale, void *out, void *workspace,
+                                           size_t workspace_bytes, cast_stream_t stream) {
+  if (!block_table || !kv_lens) return fail(CAST_ERR_INVALID_ARGUMENT, "block_table and kv_lens are required");
+  if (page <= 0 || max_pages <= 0 || n_pages <= 0) return fail(CAST_ERR_INVALID_ARGUMENT, "non-positive cache size");
+  const long long cap = (long long)page * max_pages;
+  if (cap >= (1 << 30)) return fail(CAST_ERR_UNSUPPORTED, "%lld keys in one session", cap);
+  int st = window_dims_ok(B, Hq, Hk, Lq, (int)cap, D, window, sinks, frame_tokens);
+  if (st) return st;
+  castk::RowsParams p;
+  st = rows_params(p, q, k_pages, v_pages, dtype, kv_lens, B, Hq, Hk, Lq, (int)cap, strides, window, sinks,
+                   frame_tokens, sm_scale, out);
+  if (st) return st;
+  int n_sms = 0;
+  if ((st = current_device_sm100(&n_sms))) return st;
+  p.block_table = block_table;
+  p.page = page, p.max_pages = max_pages, p.n_pages = n_pages;
+  const RowsPlan plan = rows_plan(B, Hk, p.group, Lq, (int)cap, window, sinks, frame_tokens, D, n_sms);
+  return rows_call(p, plan, true, dtype, D, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
 }
 
 // ===========================================================================

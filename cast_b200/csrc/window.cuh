@@ -1,0 +1,593 @@
+// Sliding-window attention with visible first tokens (sinks), for few query
+// rows: a split over the keys, dense or paged.
+//
+// Query i of Lq (position p = len - Lq + i of a session of len keys) sees key
+// j < len with f(j) <= f(p) and (f(j) > f(p) - window or f(j) < sinks), where
+// f(x) = x / frame: the keys [lo(p), hi(p)) and the sinks [0, S),
+//   hi(p) = min(len, (f(p) + 1) frame), lo(p) = max(0, (f(p) - window + 1) frame),
+//   S = sinks * frame.
+// Both bounds grow with p, so the rows of a tile together see one list of
+// keys: the S sinks followed by [lo(first row), hi(last row)), or [0, hi)
+// where the two meet.  A place in that list is a "virtual" key.
+//
+// out = sum_j 2^(s_j - m) v_j / sum_j 2^(s_j - m), s_j = q.k_j scale log2(e),
+// in one pass over the keys with a running m.
+#pragma once
+
+#include <cooperative_groups.h>
+#include <cuda_fp16.h>
+
+#include "attention.cuh"
+#include "common.cuh"
+
+namespace castk {
+
+// ------------------------------------------------------------------ masks
+struct WindowRule {
+  long long window, sinks;  // in frames
+  int frame;
+};
+
+// What the rows of one tile see of a session of `len` keys.
+struct WindowSpan {
+  int len, lq;
+  int sinks;      // S, clipped to len
+  int s_n;        // virtual keys that are sinks (0 where the list is contiguous)
+  int base;       // key of virtual key s_n
+  int n;          // virtual keys
+  int lo0, hi0;   // lo, hi of the first row that has a position
+  int lo1, hi1;   // of the last row
+  bool unplaced;  // some row has no position (it sees nothing)
+  __device__ __forceinline__ int key(int v) const { return v < s_n ? v : base + (v - s_n); }
+  // whether a key of the list is hidden from some row of the tile
+  __device__ __forceinline__ bool some(int key) const {
+    return unplaced || (key >= sinks && (key < lo1 || key >= hi0));
+  }
+};
+
+__device__ __forceinline__ void window_bounds(const WindowRule &r, int len, int p, int &lo, int &hi) {
+  const long long f = p / r.frame;
+  const long long h = (f + 1) * r.frame;
+  hi = h < len ? (int)h : len;
+  const long long l = f + 1 - r.window;  // first visible frame
+  lo = l <= 0 ? 0 : (int)min(l * r.frame, (long long)len);
+}
+
+// Rows i0 .. i1 (inclusive) of lq queries.
+__device__ __forceinline__ WindowSpan window_span(const WindowRule &r, int len, int lq, int i0, int i1) {
+  WindowSpan s;
+  s.len = len;
+  s.lq = lq;
+  s.sinks = (int)min(r.sinks * r.frame, (long long)len);
+  s.s_n = s.base = s.n = s.lo0 = s.hi0 = s.lo1 = s.hi1 = 0;
+  s.unplaced = len - lq + i0 < 0;
+  const int p1 = len - lq + i1;
+  if (p1 < 0) return s;  // no row of the tile has a position
+  const int p0 = max(0, len - lq + i0);
+  window_bounds(r, len, p0, s.lo0, s.hi0);
+  window_bounds(r, len, p1, s.lo1, s.hi1);
+  if (s.sinks < s.lo0) {
+    s.s_n = s.sinks;
+    s.base = s.lo0;
+  }
+  s.n = s.s_n + s.hi1 - s.base;
+  return s;
+}
+
+__device__ __forceinline__ bool window_sees(int key, int lo, int hi, int sinks) {
+  return key < hi && (key >= lo || key < sinks);
+}
+
+// ------------------------------------------------------------- type traits
+template <typename T>
+struct Half2;
+template <>
+struct Half2<__nv_bfloat16> {
+  // P = 2^(s - m + kShift).  The running maximum m moves only where a score is
+  // above it by more than kSlack, so P <= 2^(kSlack + kShift): bf16 has
+  // float32's range.
+  static constexpr float kShift = 0.0f, kSlack = 8.0f;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+  static __device__ __forceinline__ float2 unpack(uint32_t u) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+  }
+  static __device__ __forceinline__ __nv_bfloat16 round(float x) { return __float2bfloat16_rn(x); }
+  // whether either half is an infinity or NaN
+  static __device__ __forceinline__ uint32_t bad(uint32_t u) {
+    return ((u & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) | ((u & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u);
+  }
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+template <>
+struct Half2<__half> {
+  // P <= 2^12; the shift keeps weights down to 2^-32 of the largest (2^-24
+  // without it), which thousands of small ones can add up to.
+  static constexpr float kShift = 8.0f, kSlack = 4.0f;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t u) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&u));
+  }
+  static __device__ __forceinline__ __half round(float x) { return __float2half_rn(x); }
+  static __device__ __forceinline__ uint32_t bad(uint32_t u) {
+    return ((u & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u) | ((u & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u);
+  }
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// 16 bytes global -> shared, zeros where !live (nothing is read then).
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool live) {
+  const int bytes = live ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// --------------------------------------------------------------- few rows
+constexpr int kRowsWarps = 4;
+constexpr int kRowsStages = 3;
+constexpr int kRowsMaxCluster = 8;
+
+struct RowsParams {
+  const void *q, *k, *v;
+  void *out;
+  long long qs[3], ks[3], vs[3], os[3];  // strides of batch, head, token (pages: page, head, token)
+  const int32_t *kv_lens;                // nullptr: every session has lk keys
+  const int32_t *block_table;            // [B, max_pages] (paged)
+  float *part;                           // partial results (n_split > kRowsMaxCluster), else nullptr
+  WindowRule rule;
+  int B, Hq, Hk, Lq, lk;                 // lk: keys a session can have
+  int page, max_pages, n_pages;
+  int group, rows, row_tiles;            // rows = group * Lq of one key head
+  int n_split;
+  float scale_log2;
+};
+
+// One CTA: rows 16 MT of one (session, key head), part `split` of their
+// virtual keys.  Each of its warps takes every kRowsWarps-th group of 16 keys
+// through a ring of its own in shared memory (cp.async, no CTA barrier in the
+// loop): S = Q K^T and O += P V are m16n8k16 products whose rows are the query
+// heads that share the key head, so a key is read once for all of them.  The
+// warps' results are joined in shared memory, the CTAs' through distributed
+// shared memory of a cluster, or, for more parts than a cluster has, from
+// `part` by window_rows_join_kernel.  The order of every sum is fixed.
+template <typename T, int D, int MT, bool kPaged>
+struct RowsSmem {
+  static constexpr int row_bytes = D * 2;
+  static constexpr int group_bytes = 16 * row_bytes;               // 16 keys of K or V
+  static constexpr int warp_bytes = kRowsStages * 2 * group_bytes;
+  static constexpr int ring = kRowsWarps * warp_bytes;
+  static constexpr int join = kRowsWarps * 16 * MT * (D + 4) * 4;  // O, m, l of each warp
+  static constexpr int bytes = (ring > join ? ring : join) + 16 * MT * (D + 4) * 4;  // + the CTA's own
+};
+
+// Where a value of a virtual key lies (nullptr: its page is not one).
+template <typename T, bool kPaged>
+__device__ __forceinline__ const T *rows_value(const RowsParams &p, int b, int hk, int key) {
+  const T *v = static_cast<const T *>(p.v) + hk * p.vs[1];
+  if (!kPaged) return v + b * p.vs[0] + key * p.vs[2];
+  const int pg = __ldg(p.block_table + (long long)b * p.max_pages + key / p.page);
+  return pg < 0 || pg >= p.n_pages ? nullptr : v + pg * p.vs[0] + (key % p.page) * p.vs[2];
+}
+
+// Joins the parts' (O, m, l) of rows r0 .. r_end - 1, normalises and writes
+// share `rank` of `ranks` of them; part(j) is the j-th part's buffer, rows of
+// D + 4 floats: O, m, l and whether the part took an infinity or NaN out of a
+// value that only some rows see.
+template <typename T, int D, int MT, bool kPaged, typename Part>
+__device__ __forceinline__ void window_write(const RowsParams &p, const WindowSpan &span, int b, int hk, int r0,
+                                             int r_end, int rank, int ranks, const Part &part, int thread,
+                                             int threads) {
+  constexpr int kRow = D + 4;
+  for (int x = rank * threads + thread; x < (r_end - r0) * (D / 4); x += ranks * threads) {
+    const int r = x / (D / 4), c = (x % (D / 4)) * 4;
+    float m = -INFINITY, bad = 0.0f;
+    for (int j = 0; j < p.n_split; ++j) m = fmaxf(m, part(j)[r * kRow + D]);
+    float l = 0.0f, a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < p.n_split; ++j) {
+      const float *row = part(j) + r * kRow;
+      const float4 tail = *reinterpret_cast<const float4 *>(row + D);
+      const float f = tail.x == -INFINITY ? 0.0f : fast_exp2(tail.x - m);
+      const float4 v = *reinterpret_cast<const float4 *>(row + c);
+      l = fmaf(tail.y, f, l);
+      a[0] = fmaf(v.x, f, a[0]), a[1] = fmaf(v.y, f, a[1]), a[2] = fmaf(v.z, f, a[2]), a[3] = fmaf(v.w, f, a[3]);
+      if (__float_as_int(tail.z)) bad = 1.0f;
+    }
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // (a NaN sum stays one)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] *= inv;
+    const int token = (r0 + r) / p.group, head = hk * p.group + (r0 + r) % p.group;
+    if (bad != 0.0f) {
+      int lo = 0, hi = 0;
+      const int pos = span.len - p.Lq + token;
+      if (pos >= 0) window_bounds(p.rule, span.len, pos, lo, hi);
+      for (int v = 0; v < span.n; ++v) {
+        const int key = span.key(v);
+        if (!span.some(key) || hi == 0 || !window_sees(key, lo, hi, span.sinks)) continue;
+        const T *src = rows_value<T, kPaged>(p, b, hk, key);
+        if (!src) continue;
+        for (int i = 0; i < 4; ++i) {
+          const float y = (float)src[c + i];
+          if (!isfinite(y)) a[i] += y;
+        }
+      }
+    }
+    T *dst = static_cast<T *>(p.out) + b * p.os[0] + (long long)head * p.os[1] + (long long)token * p.os[2] + c;
+    *reinterpret_cast<uint2 *>(dst) = make_uint2(Half2<T>::pack(a[0], a[1]), Half2<T>::pack(a[2], a[3]));
+  }
+}
+
+template <typename T, int D, int MT, bool kPaged>
+__global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __grid_constant__ RowsParams p) {
+  using S = RowsSmem<T, D, MT, kPaged>;
+  using H2 = Half2<T>;
+  constexpr int kChunks = D / 8;  // 16-byte pieces of a row
+  constexpr int R = 16 * MT;
+  extern __shared__ __align__(1024) uint8_t smem_rows[];
+  __shared__ int flag_bad;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = blockIdx.x % p.n_split;
+  const int item = blockIdx.x / p.n_split;
+  const int rt = item % p.row_tiles;
+  const int bh = item / p.row_tiles;
+  const int b = bh / p.Hk, hk = bh - b * p.Hk;
+  const int r0 = rt * R;  // first row: token r / group, head r % group
+  const int r_end = min(p.rows, r0 + R);
+  int len = p.kv_lens ? p.kv_lens[b] : p.lk;
+  if (len < 0 || len > p.lk) {  // a session longer than its cache: nothing past the cache is read
+    if (threadIdx.x == 0) atomicExch(&g_cast_device_error, (int)CAST_ERR_INVALID_ARGUMENT);
+    len = min(max(len, 0), p.lk);
+  }
+  const WindowSpan span = window_span(p.rule, len, p.Lq, r0 / p.group, (r_end - 1) / p.group);
+  const int groups = (span.n + 15) / 16;
+  // this CTA's groups of 16 keys
+  const int g_lo = (int)((long long)groups * split / p.n_split);
+  const int g_hi = (int)((long long)groups * (split + 1) / p.n_split);
+  const bool partial = span.lo0 != span.lo1 || span.hi0 != span.hi1 || span.unplaced;
+  if (threadIdx.x == 0) flag_bad = 0;
+  __syncthreads();
+
+  // ---- Q fragments: row r = lane / 4 (+ 8), columns 2 (lane % 4) (+ 8) of each 16
+  uint32_t qf[MT][D / 16][4];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const int r = r0 + 16 * mt + lane / 4 + 8 * hh;
+      const bool on = r < r_end;
+      const int i = r / p.group, g = r - i * p.group;
+      const T *src = static_cast<const T *>(p.q) + b * p.qs[0] + (long long)(hk * p.group + g) * p.qs[1] + (long long)i * p.qs[2];
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {
+        qf[mt][s][hh] = on ? *reinterpret_cast<const uint32_t *>(src + 16 * s + 2 * (lane % 4)) : 0u;
+        qf[mt][s][2 + hh] = on ? *reinterpret_cast<const uint32_t *>(src + 16 * s + 8 + 2 * (lane % 4)) : 0u;
+      }
+    }
+  }
+  // what each of this lane's rows sees
+  int lo[MT][2], hi[MT][2];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const int r = r0 + 16 * mt + lane / 4 + 8 * hh;
+      const int pos = len - p.Lq + r / p.group;
+      lo[mt][hh] = hi[mt][hh] = 0;
+      if (r < r_end && pos >= 0) window_bounds(p.rule, len, pos, lo[mt][hh], hi[mt][hh]);
+    }
+
+  float o[MT][D / 8][4];
+  float m_run[MT][2], l_run[MT][2];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[mt][j][c] = 0.0f;
+    m_run[mt][0] = m_run[mt][1] = -INFINITY;
+    l_run[mt][0] = l_run[mt][1] = 0.0f;
+  }
+
+  const uint32_t ring = castdev::smem_u32(smem_rows) + warp * S::warp_bytes;
+  const T *kbase = static_cast<const T *>(p.k) + (kPaged ? 0 : b * p.ks[0]) + hk * p.ks[1];
+  const T *vbase = static_cast<const T *>(p.v) + (kPaged ? 0 : b * p.vs[0]) + hk * p.vs[1];
+
+  // Page of this lane's key (lane % 16) of group g; -1: no key there.
+  auto page_of = [&](int g) -> int {
+    const int v = 16 * g + (lane & 15);
+    if (g >= g_hi || v >= span.n) return -1;
+    if (!kPaged) return 0;
+    const int pg = __ldg(p.block_table + (long long)b * p.max_pages + span.key(v) / p.page);
+    if (pg < 0 || pg >= p.n_pages) {
+      atomicExch(&g_cast_device_error, (int)CAST_ERR_INVALID_ARGUMENT);
+      return -1;
+    }
+    return pg;
+  };
+  // Starts the copies of group g into stage st; returns a bit for each of the
+  // 16 keys that are there.
+  auto start = [&](int g, int st, int pg) -> uint32_t {
+    const int v = 16 * g + (lane & 15);
+    long long ko = 0, vo = 0;
+    if (pg >= 0) {
+      const int key = span.key(v);
+      if (kPaged) {
+        const int in = key % p.page;
+        ko = pg * p.ks[0] + in * p.ks[2];
+        vo = pg * p.vs[0] + in * p.vs[2];
+      } else {
+        ko = key * p.ks[2];
+        vo = key * p.vs[2];
+      }
+    }
+    const uint32_t there = __ballot_sync(0xffffffffu, pg >= 0) & 0xFFFFu;
+    const uint32_t dst = ring + st * 2 * S::group_bytes;
+    constexpr int kRowsPer = 32 / kChunks;  // rows a pass of the warp covers
+    const int c = lane % kChunks;
+#pragma unroll
+    for (int i = 0; i < 16 / kRowsPer; ++i) {
+      const int row = i * kRowsPer + lane / kChunks;
+      const long long kr = __shfl_sync(0xffffffffu, ko, row), vr = __shfl_sync(0xffffffffu, vo, row);
+      const bool live = (there >> row) & 1u;
+      const uint32_t off = row * S::row_bytes + ((c ^ (row & 7)) * 16);
+      cp_async16(dst + off, kbase + kr + 8 * c, live);
+      cp_async16(dst + S::group_bytes + off, vbase + vr + 8 * c, live);
+    }
+    return there;
+  };
+
+  // groups g_lo + warp + kRowsWarps * t of this warp
+  const int first = g_lo + warp;
+  uint32_t there[kRowsStages];
+  int next_page = page_of(first);
+#pragma unroll
+  for (int st = 0; st < kRowsStages - 1; ++st) {
+    const int g = first + kRowsWarps * st;
+    const int pg = next_page;
+    next_page = page_of(g + kRowsWarps);
+    there[st] = start(g, st, pg);
+    cp_async_commit();
+  }
+  there[kRowsStages - 1] = 0;
+  int saw_bad = 0;
+
+  for (int t = 0; first + kRowsWarps * t < g_hi; ++t) {
+    const int g = first + kRowsWarps * t;
+    const int st = t % kRowsStages;
+    cp_async_wait<kRowsStages - 2>();
+    __syncwarp();
+    {  // the stage read in the last step is free: start the group it takes
+      const int gn = g + kRowsWarps * (kRowsStages - 1), sn = (t + kRowsStages - 1) % kRowsStages;
+      const int pg = next_page;
+      next_page = page_of(gn + kRowsWarps);
+      const uint32_t bits = start(gn, sn, pg);
+      cp_async_commit();
+#pragma unroll
+      for (int x = 0; x < kRowsStages; ++x)
+        if (x == sn) there[x] = bits;
+    }
+    uint32_t mine = 0;
+#pragma unroll
+    for (int x = 0; x < kRowsStages; ++x)
+      if (x == st) mine = there[x];
+    const uint32_t ks = ring + st * 2 * S::group_bytes, vs = ks + S::group_bytes;
+
+    // S = Q K^T of 16 keys
+    float s[MT][2][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[mt][0][c] = s[mt][1][c] = 0.0f;
+    {
+      const int row = (lane & 7) + ((lane >> 4) << 3), cc = (lane >> 3) & 1;
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        uint32_t kf[4];
+        ldmatrix_x4(ks + row * S::row_bytes + (((2 * j + cc) ^ (row & 7)) * 16), kf);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          H2::mma(s[mt][0], qf[mt][j], kf[0], kf[1]);
+          H2::mma(s[mt][1], qf[mt][j], kf[2], kf[3]);
+        }
+      }
+    }
+    // keys of this lane's four columns: 2 (lane % 4) + {0, 1, 8, 9}
+    int key[4];
+    uint32_t col_there = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int col = 2 * (lane % 4) + (c & 1) + 8 * (c >> 1);
+      key[c] = span.key(16 * g + col);
+      if ((mine >> col) & 1u) col_there |= 1u << c;
+    }
+    uint32_t pf[MT][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      float mx[2];
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        float x = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float &v = s[mt][c >> 1][2 * hh + (c & 1)];
+          const bool on = ((col_there >> c) & 1u) && window_sees(key[c], lo[mt][hh], hi[mt][hh], span.sinks) && hi[mt][hh] > 0;
+          v = on ? v * p.scale_log2 : -INFINITY;
+          x = fmaxf(x, v);
+        }
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+        mx[hh] = x;
+      }
+      const bool move0 = mx[0] > m_run[mt][0] + H2::kSlack, move1 = mx[1] > m_run[mt][1] + H2::kSlack;
+      if (__any_sync(0xffffffffu, move0 || move1)) {
+        const float n0 = move0 ? mx[0] : m_run[mt][0], n1 = move1 ? mx[1] : m_run[mt][1];
+        const float f0 = move0 ? fast_exp2(m_run[mt][0] - n0) : 1.0f, f1 = move1 ? fast_exp2(m_run[mt][1] - n1) : 1.0f;
+        m_run[mt][0] = n0, m_run[mt][1] = n1;
+        l_run[mt][0] *= f0, l_run[mt][1] *= f1;
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) {
+          o[mt][j][0] *= f0, o[mt][j][1] *= f0;
+          o[mt][j][2] *= f1, o[mt][j][3] *= f1;
+        }
+      }
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const float base = m_run[mt][hh] == -INFINITY ? 0.0f : m_run[mt][hh] - H2::kShift;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          const uint32_t u = H2::pack(fast_exp2(s[mt][nt][2 * hh] - base), fast_exp2(s[mt][nt][2 * hh + 1] - base));
+          pf[mt][2 * nt + hh] = u;
+          // the weights that P V uses, so that they sum to one
+          const float2 w = H2::unpack(u);
+          l_run[mt][hh] += w.x + w.y;
+        }
+      }
+    }
+    if (partial) {
+      // A key that only some rows of the tile see: its value meets a zero
+      // weight in the others, so an infinity or NaN there is taken out here
+      // and given back to the rows that see it at the end.
+      const int col = lane & 15;
+      const int kk = span.key(16 * g + col);
+      const bool some = ((mine >> col) & 1u) && span.some(kk);
+      uint32_t todo = __ballot_sync(0xffffffffu, some) & 0xFFFFu;
+      while (todo) {
+        const int row = __ffs(todo) - 1;
+        todo &= todo - 1;
+        uint32_t *w = reinterpret_cast<uint32_t *>(smem_rows + (vs - castdev::smem_u32(smem_rows)) + row * S::row_bytes);
+#pragma unroll
+        for (int x = lane; x < D / 2; x += 32) {
+          const uint32_t u = w[x], bad = H2::bad(u);
+          if (bad) {
+            w[x] = u & ~bad;
+            saw_bad = 1;
+          }
+        }
+      }
+      __syncwarp();
+    }
+    // O += P V
+    {
+      const int row = (lane & 7) + (((lane >> 3) & 1) << 3), cc = lane >> 4;
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        uint32_t vf[4];
+        ldmatrix_x4_trans(vs + row * S::row_bytes + (((2 * j + cc) ^ (row & 7)) * 16), vf);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          H2::mma(o[mt][2 * j], pf[mt], vf[0], vf[1]);
+          H2::mma(o[mt][2 * j + 1], pf[mt], vf[2], vf[3]);
+        }
+      }
+    }
+    __syncwarp();
+  }
+  cp_async_wait<0>();
+  if (saw_bad) flag_bad = 1;
+  __syncthreads();
+
+  // ---- join the warps: (O, m, l) of each in shared memory, rows of D + 4 floats
+  constexpr int kRow = D + 4;
+  float *js = reinterpret_cast<float *>(smem_rows);
+  float *own = reinterpret_cast<float *>(smem_rows + (S::ring > S::join ? S::ring : S::join));
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      float l = l_run[mt][hh];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      float *row = js + (warp * R + 16 * mt + lane / 4 + 8 * hh) * kRow;
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j)
+        *reinterpret_cast<float2 *>(row + 8 * j + 2 * (lane % 4)) = make_float2(o[mt][j][2 * hh], o[mt][j][2 * hh + 1]);
+      if (lane % 4 == 0) {
+        row[D] = m_run[mt][hh];
+        row[D + 1] = l;
+      }
+    }
+  __syncthreads();
+  float *part = p.part ? p.part + (long long)blockIdx.x * (R * kRow) : own;
+  for (int x = threadIdx.x; x < R * (D / 4); x += blockDim.x) {
+    const int r = x / (D / 4), c = (x % (D / 4)) * 4;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kRowsWarps; ++w) m = fmaxf(m, js[(w * R + r) * kRow + D]);
+    float l = 0.0f;
+    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < kRowsWarps; ++w) {
+      const float *row = js + (w * R + r) * kRow;
+      const float f = row[D] == -INFINITY ? 0.0f : fast_exp2(row[D] - m);
+      const float4 v = *reinterpret_cast<const float4 *>(row + c);
+      l = fmaf(row[D + 1], f, l);
+      a.x = fmaf(v.x, f, a.x), a.y = fmaf(v.y, f, a.y), a.z = fmaf(v.z, f, a.z), a.w = fmaf(v.w, f, a.w);
+    }
+    *reinterpret_cast<float4 *>(part + r * kRow + c) = a;
+    if (c == 0) {
+      part[r * kRow + D] = m;
+      part[r * kRow + D + 1] = l;
+      part[r * kRow + D + 2] = __int_as_float(flag_bad);
+    }
+  }
+  if (p.part) return;  // window_rows_join_kernel joins the CTAs
+
+  // ---- join the cluster's CTAs and write
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  if (p.n_split > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  window_write<T, D, MT, kPaged>(p, span, b, hk, r0, r_end, split, p.n_split,
+                                 [&](int j) { return p.n_split > 1 ? cluster.map_shared_rank(own, j) : own; },
+                                 (int)threadIdx.x, (int)blockDim.x);
+  if (p.n_split > 1) cluster.sync();  // no CTA leaves while its memory is read
+}
+
+// Joins the parts that window_rows_kernel left in p.part: kJoinShare CTAs for
+// each tile of rows.
+constexpr int kJoinShare = 4;
+template <typename T, int D, int MT, bool kPaged>
+__global__ void __launch_bounds__(128) window_rows_join_kernel(const __grid_constant__ RowsParams p) {
+  constexpr int R = 16 * MT;
+  const int item = blockIdx.x / kJoinShare;
+  const int rt = item % p.row_tiles, bh = item / p.row_tiles;
+  const int b = bh / p.Hk, hk = bh - b * p.Hk;
+  const int r0 = rt * R, r_end = min(p.rows, r0 + R);
+  const int len = min(max(p.kv_lens ? p.kv_lens[b] : p.lk, 0), p.lk);
+  const WindowSpan span = window_span(p.rule, len, p.Lq, r0 / p.group, (r_end - 1) / p.group);
+  const float *base = p.part + (long long)item * p.n_split * (R * (D + 4));
+  window_write<T, D, MT, kPaged>(p, span, b, hk, r0, r_end, blockIdx.x % kJoinShare, kJoinShare,
+                                 [&](int j) { return base + (long long)j * (R * (D + 4)); }, (int)threadIdx.x,
+                                 (int)blockDim.x);
+}
+
+}  // namespace castk

@@ -367,6 +367,94 @@ CAST_API int cast_compact_unpack(const void *packed, const int32_t *token_to_pac
                         int H, int D, int P, void *out, cast_stream_t stream);
 
 /*
+ * Rotary positions.  Element type `dtype`: 0 = bf16, 1 = fp32, 2 = fp16.
+ *   x          [B,L,H,D], head vectors contiguous, other strides free
+ *   table      float [table_rows, R/2] (cos, sin) pairs; pair j of a token at
+ *              position p turns by entry (p, j)
+ *   positions  int32 (positions_64 0) or int64 [L] or [B,L], [.., 3] with
+ *              axes; pos_batch_stride 0 or the elements of one batch;
+ *              NULL: first_position + token
+ *   axes       NULL, or the pairs (n0, n1, n2) whose sum is R/2 that turn
+ *              with the first, second and third position
+ *   flags      1: pairs are (2j, 2j+1), else (j, j + R/2); 2: turn back (-angle)
+ *   strides    (batch, token, head) of x, then of out, in elements
+ *   out        as x; may be x itself
+ * out = x with the pairs of the first R values turned, in float32, rounded
+ * once.  Supported: D a multiple of 8 up to 256; R a multiple of 8 (pairs
+ * side by side) or 16; strides on 16-byte boundaries.  A token whose position
+ * is no row of the table is written as zeros and reported by
+ * cast_device_error().
+ */
+CAST_API int cast_rope(const void *x, int dtype, const float *table, int table_rows, const void *positions,
+                       int positions_64, long long pos_batch_stride, long long first_position,
+                       const int *axes, int B, int L, int H, int D, int R, int flags,
+                       const long long *strides, void *out, cast_stream_t stream);
+
+/*
+ * RMS norm of query and key heads, x / sqrt(mean(x^2) + eps) * weight, with
+ * the rotation of cast_rope in the same pass (R 0: no rotation).
+ *   q, k       [B,L,Hq,D], [B,L,Hk,D]; v [B,L,Hk,D] or NULL
+ *   out_dtype  dtype, or bf16 of fp32
+ *   weights    [D], or [H,D] (weight_per_head), of dtype or fp32
+ *              (weight_fp32); NULL: that tensor is not normalised
+ *   strides    (batch, token, head) of q, k, v, q_out, k_out
+ * With v: k_out and v_out are caches [n_pages,Hk,page,D], contiguous, and
+ * token (b, l)'s key and value (copied) go to place slots[b,l] of the
+ * n_pages * page ones (int32, or int64 with slots_64): below zero it is not
+ * written, past the end it is not written and reported.  Slots differ from
+ * one another; of two tokens with one slot either may be kept, piece by piece.
+ */
+CAST_API int cast_qk_norm_rope(const void *q, const void *k, const void *v, int dtype, int out_dtype,
+                               const void *q_weight, const void *k_weight, int weight_fp32,
+                               int weight_per_head, float eps, const float *table, int table_rows,
+                               const void *positions, int positions_64, long long pos_batch_stride,
+                               long long first_position, const int *axes, int B, int L, int Hq, int Hk,
+                               int D, int R, int flags, const long long *strides, void *q_out,
+                               void *k_out, void *v_out, const void *slots, int slots_64, int n_pages,
+                               int page, cast_stream_t stream);
+
+/*
+ * Sliding-window attention with sinks.  Query i of batch b is at position
+ * p = kv_lens[b] - Lq + i and sees key j < kv_lens[b] iff f(j) <= f(p) and
+ * (f(j) > f(p) - window or f(j) < sinks), f(x) = x / frame_tokens (window and
+ * sinks count tokens with frame_tokens 1).  A query that sees nothing
+ * gives zeros; what it does not see never reaches it, NaN included.
+ *   q [B,Hq,Lq,D], k, v [B,Hk,Lk,D], out [B,Hq,Lq,D]: bf16 (dtype 0) or
+ *       fp16 (2), Hq a multiple of Hk, D 64 or 128; head vectors contiguous,
+ *       other strides free on 16-byte boundaries
+ *   strides  (batch, head, token) of q, k, v, out, in elements
+ *   kv_lens  int32 [B], or NULL (Lk); one outside [0, Lk] is clipped and
+ *            reported by cast_device_error()
+ *   workspace  at least the size that cast_window_attention_workspace_bytes
+ *            gives (often 0: NULL then), any contents; calls that may overlap
+ *            on the GPU use their own
+ */
+CAST_API size_t cast_window_attention_workspace_bytes(int B, int Hq, int Hk, int Lq, int Lk, int D,
+                                                      long long window, long long sinks, int frame_tokens);
+CAST_API int cast_window_attention(const void *q, const void *k, const void *v, int dtype,
+                                   const int32_t *kv_lens, int B, int Hq, int Hk, int Lq, int Lk, int D,
+                                   const long long *strides, long long window, long long sinks,
+                                   int frame_tokens, float sm_scale, void *out, void *workspace,
+                                   size_t workspace_bytes, cast_stream_t stream);
+
+/*
+ * The same over a paged cache: key j of batch b is row j % page of page
+ * block_table[b, j / page] of k_pages, v_pages [n_pages,Hk,page,D] (strides:
+ * page, head, token).  Entries of pages that no query sees are not read; one
+ * outside [0, n_pages) that is seen hides its keys and is reported by
+ * cast_device_error().
+ */
+CAST_API size_t cast_paged_window_attention_workspace_bytes(int B, int Hq, int Hk, int Lq, int D, int page,
+                                                            int max_pages, long long window, long long sinks,
+                                                            int frame_tokens);
+CAST_API int cast_paged_window_attention(const void *q, const void *k_pages, const void *v_pages, int dtype,
+                                         const int32_t *block_table, int max_pages, int n_pages, int page,
+                                         const int32_t *kv_lens, int B, int Hq, int Hk, int Lq, int D,
+                                         const long long *strides, long long window, long long sinks,
+                                         int frame_tokens, float sm_scale, void *out, void *workspace,
+                                         size_t workspace_bytes, cast_stream_t stream);
+
+/*
  * Two-anchor residual writer of the control-barycentric reconstruction.
  * Replaces direct_control_barycentric_pair_write (proposed/matrix_control_
  * barycentric_pair_kernel.py:22-204), which the frame weave's control-

@@ -1,0 +1,144 @@
+"""CPU: the rotary tables, and what the rotary entry points refuse."""
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from cast_b200 import _lib, rotary
+from oracle import rotary as ora
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from cast_b200 import build
+
+    build.build()
+    return _lib.load()
+
+
+def test_frequencies_of_one_axis_and_three():
+    f = rotary.rope_frequencies(128)
+    assert f.dtype == torch.float64 and f.shape == (64,)
+    for j in (0, 1, 17, 63):
+        assert f[j].item() == pytest.approx(10000.0 ** (-2 * j / 128), rel=1e-14)
+    g = rotary.rope_frequencies(128, axes=(22, 21, 21))
+    assert g[22].item() == 1.0 and g[43].item() == 1.0
+    assert g[23].item() == pytest.approx(10000.0 ** (-1 / 21), rel=1e-14)
+
+
+def test_frequencies_scaled_for_long_contexts():
+    f = rotary.rope_frequencies(64, base=500.0)
+    assert torch.equal(rotary.rope_frequencies(64, base=500.0, scaling=("linear", 4.0)), f / 4)
+    n = rotary.rope_frequencies(64, base=500.0, scaling=("ntk", 4.0))
+    assert n[0] == f[0] and n[-1].item() == pytest.approx(f[-1].item() / 4, rel=1e-12)
+    assert (n[1:] < f[1:]).all()
+    y = rotary.rope_frequencies(64, scaling=("yarn", 8.0, 4096))
+    f = rotary.rope_frequencies(64)
+    turns = f * 4096 / (2 * math.pi)
+    assert torch.equal(y[turns > 40], f[turns > 40])
+    assert torch.allclose(y[turns < 0.7], f[turns < 0.7] / 8, rtol=1e-12)
+    assert ((y <= f) & (y >= f / 8 * (1 - 1e-12))).all()
+
+
+@pytest.mark.parametrize("kwargs", [dict(rotary_dim=7), dict(rotary_dim=0), dict(rotary_dim=8, base=1.0),
+                                    dict(rotary_dim=8, axes=(1, 1, 1)), dict(rotary_dim=8, scaling=("other", 2.0)),
+                                    dict(rotary_dim=8, scaling=("linear", 0.0))])
+def test_frequencies_refused(kwargs):
+    with pytest.raises(ValueError):
+        rotary.rope_frequencies(**kwargs)
+
+
+def test_table_holds_far_positions():
+    f = rotary.rope_frequencies(16)
+    t = rotary.rope_table(f, 200001, amplitude=0.5, device="cpu")
+    assert t.shape == (200001, 8, 2) and t.dtype == torch.float32
+    theta = ora.angles(torch.tensor([[200000]]), f)[0, 0]
+    # float32 rounding of a value up to 1/2; float64 angles are off by 200000 * 2^-53
+    assert torch.allclose(t[200000, :, 0].double(), 0.5 * theta.cos(), rtol=0, atol=2.0 ** -25 * 1.01)
+    assert torch.allclose(t[200000, :, 1].double(), 0.5 * theta.sin(), rtol=0, atol=2.0 ** -25 * 1.01)
+    with pytest.raises(ValueError):
+        rotary.rope_table(f, 0, device="cpu")
+
+
+def test_a_turn_by_an_inverse_turn_is_the_identity():
+    x = torch.randn(1, 3, 2, 16, dtype=torch.float64)
+    theta = torch.randn(1, 3, 6, dtype=torch.float64)
+    for inter in (False, True):
+        back = ora.turn(ora.turn(x, theta, inter), -theta, inter)
+        assert torch.allclose(back, x, atol=1e-14)
+        # scores depend on the distance of positions alone
+        y = torch.randn(1, 3, 2, 16, dtype=torch.float64)
+        a = (ora.turn(x, theta, inter) * ora.turn(y, theta + 0.3, inter)).sum(-1)
+        b = (ora.turn(x, theta + 5, inter) * ora.turn(y, theta + 5.3, inter)).sum(-1)
+        assert torch.allclose(a, b, atol=1e-12)
+
+
+def test_python_refuses_host_tensors():
+    x = torch.zeros(1, 2, 2, 16)
+    with pytest.raises(ValueError, match="CUDA"):
+        rotary.rope(x, torch.zeros(2, 8, 2))
+    with pytest.raises(ValueError, match="CUDA"):
+        rotary.qk_norm_rope(x, x, None, None)
+
+
+def _rope(lib, **kw):
+    a = dict(x=4096, dtype=0, table=4096, rows=4, positions=None, p64=0, batch=0, first=0, axes=None, B=1, L=2, H=2,
+             D=128, R=128, flags=1, strides=[512, 256, 128] * 2, out=8192)
+    a.update(kw)
+    st = (ctypes.c_longlong * 6)(*a["strides"])
+    ax = None if a["axes"] is None else (ctypes.c_int * 3)(*a["axes"])
+    return lib.cast_rope(a["x"], a["dtype"], a["table"], a["rows"], a["positions"], a["p64"], a["batch"], a["first"], ax,
+                         a["B"], a["L"], a["H"], a["D"], a["R"], a["flags"], st, a["out"], None)
+
+
+@pytest.mark.parametrize("kw,status,text", [
+    (dict(x=None), 1, b"required"),
+    (dict(dtype=3), 1, b"dtype"),
+    (dict(L=0), 1, b"non-positive"),
+    (dict(D=260), 2, b"head_dim"),
+    (dict(D=20, R=16), 2, b"head_dim"),
+    (dict(R=130), 1, b"rotated part"),
+    (dict(R=12), 2, b"rotated part"),
+    (dict(R=24, flags=0), 2, b"rotated part"),
+    (dict(flags=4), 1, b"flags"),
+    (dict(table=None), 1, b"table"),
+    (dict(rows=0), 1, b"table"),
+    (dict(table=4100), 3, b"table"),
+    (dict(axes=(22, 21, 20), positions=4096), 1, b"axes"),
+    (dict(axes=(22, 21, 21)), 1, b"positions"),
+    (dict(x=4098), 3, b"16-byte"),
+    (dict(strides=[512, 252, 128] * 2), 3, b"16-byte"),
+])
+def test_rope_refused(lib, kw, status, text):
+    assert _rope(lib, **kw) == status
+    assert text in lib.cast_last_error_message()
+
+
+def _norm(lib, **kw):
+    a = dict(q=4096, k=4096, v=None, dtype=0, out_dtype=0, eps=1e-6, Hq=4, Hk=2, D=128, qo=4096, ko=4096, vo=None,
+             slots=None, pages=0, page=0, qw=4096, strides=[1024, 512, 128] * 5)
+    a.update(kw)
+    st = (ctypes.c_longlong * 15)(*a["strides"])
+    return lib.cast_qk_norm_rope(a["q"], a["k"], a["v"], a["dtype"], a["out_dtype"], a["qw"], 4096, 0, 0, a["eps"], 4096,
+                                 4, None, 0, 0, 0, None, 1, 2, a["Hq"], a["Hk"], a["D"], 64, 1, st, a["qo"], a["ko"],
+                                 a["vo"], a["slots"], 0, a["pages"], a["page"], None)
+
+
+@pytest.mark.parametrize("kw,status,text", [
+    (dict(k=None), 1, b"required"),
+    (dict(out_dtype=2), 2, b"out_dtype"),
+    (dict(dtype=2, out_dtype=0), 2, b"out_dtype"),
+    (dict(v=4096), 1, b"together"),
+    (dict(v=4096, vo=4096), 1, b"together"),
+    (dict(v=4096, vo=4096, slots=4096), 1, b"cache"),
+    (dict(eps=-1.0), 1, b"eps"),
+    (dict(eps=float("nan")), 1, b"eps"),
+    (dict(Hk=0), 1, b"heads"),
+    (dict(qw=4100), 3, b"16-byte"),
+    (dict(strides=[1024, 512, 128] * 4 + [1024, 512, 4]), 3, b"16-byte"),
+])
+def test_qk_norm_rope_refused(lib, kw, status, text):
+    assert _norm(lib, **kw) == status
+    assert text in lib.cast_last_error_message()

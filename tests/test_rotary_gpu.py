@@ -1,0 +1,263 @@
+"""Rotary positions and the norm of query / key heads on the GPU, against the
+formulas in 64 bits.
+
+Tolerances (u = half a step of the output type, eps / 2): the output is
+rounded once, u |y|.  Before that, in float32 (2^-24 a rounding): a turn takes
+the table's rounded cos and sin, two products and a sum, 4 * 2^-24 (|a| + |b|)
+of its pair; the norm takes a sum of D squares, eight by eight in a lane and
+then over at most 32 lanes (16 roundings), halved by the root, a reciprocal
+root off by 2 * 2^-24 * 2, a division, and two products: 16 * 2^-24 more.
+float16 results below its normal range are off by 2^-25.
+"""
+
+import pytest
+import torch
+
+from cast_b200 import _lib, rotary
+from cast_b200._lib import CastError
+from oracle import rotary as ora
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _close(got, want, size, units, dtype=None):
+    dtype = dtype or got.dtype
+    tol = torch.finfo(dtype).eps / 2 * want.abs() + units * 2.0 ** -24 * size
+    if dtype == torch.float16:
+        tol = tol + 2.0 ** -25
+    off = (got.double() - want).abs()
+    assert (off <= tol * 1.01).all(), f"off by {(off / tol.clamp_min(1e-300)).max().item():.3f} of the tolerance"
+
+
+def _x(*shape, dtype, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * 2).to(dtype)
+
+
+def _quiet():
+    """No device error is pending."""
+    _lib.check_device(torch.cuda.current_stream().cuda_stream, "test")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("b,l,h,d,r", [(1, 1, 1, 8, 0), (1, 1, 24, 128, 128), (2, 5, 3, 64, 32), (3, 7, 1, 80, 80),
+                                       (1, 33, 5, 96, 48), (2, 130, 9, 256, 256), (1, 4, 40, 256, 16)])
+def test_rope(cuda, dtype, interleaved, b, l, h, d, r):
+    if r == 0:
+        r = 8 if interleaved else 0
+        if not r:
+            d, r = 16, 16
+    f = rotary.rope_frequencies(r)
+    table = rotary.rope_table(f, 700)
+    x = _x(b, l, h, d, dtype=dtype)
+    pos = torch.randint(0, 700, (b, l), device="cuda", dtype=torch.int32)
+    want = ora.turn(x.double(), ora.angles(pos, f), interleaved)
+    size = ora.pair_size(x.double(), r, interleaved)
+    _close(rotary.rope(x, table, pos, interleaved=interleaved), want, size, 4)
+    # positions of 64 bits, shared by the batch
+    want = ora.turn(x.double(), ora.angles(pos[:1].expand(b, l), f), interleaved)
+    _close(rotary.rope(x, table, pos[0].long(), interleaved=interleaved), want, size, 4)
+    # none: one after the other
+    want = ora.turn(x.double(), ora.angles(torch.arange(3, 3 + l, device="cuda").expand(b, l), f), interleaved)
+    _close(rotary.rope(x, table, interleaved=interleaved, start=3), want, size, 4)
+    _quiet()
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_rope_axes_far_and_scaled(cuda, interleaved):
+    axes = (22, 21, 21)
+    f = rotary.rope_frequencies(128, axes=axes, scaling=("ntk", 4.0))
+    table = rotary.rope_table(f, 64)
+    x = _x(2, 50, 3, 128, dtype=torch.bfloat16)
+    pos = torch.randint(0, 64, (2, 50, 3), device="cuda")
+    want = ora.turn(x.double(), ora.angles(pos, f, axes), interleaved)
+    got = rotary.rope(x, table, pos, interleaved=interleaved, axes=axes)
+    _close(got, want, ora.pair_size(x.double(), 128, interleaved), 4)
+    f = rotary.rope_frequencies(64, scaling=("yarn", 8.0, 4096))
+    table = rotary.rope_table(f, 1_000_001)
+    x = _x(1, 4, 2, 64, dtype=torch.float32)
+    pos = torch.tensor([[0, 131071, 999999, 1000000]], device="cuda")
+    want = ora.turn(x.double(), ora.angles(pos, f), interleaved)
+    _close(rotary.rope(x, table, pos, interleaved=interleaved), want, ora.pair_size(x.double(), 64, interleaved), 4)
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_rope_strides_in_place_and_back(cuda, interleaved):
+    f = rotary.rope_frequencies(64)
+    table = rotary.rope_table(f, 100)
+    qkv = _x(2, 9, 12, 128, dtype=torch.bfloat16)
+    before = qkv.clone()
+    part = qkv[:, :, 4:8]  # a slice of a projection
+    pos = torch.arange(9, device="cuda").flip(0)
+    theta = ora.angles(pos.expand(2, 9), f)
+    want, size = ora.turn(part.double(), theta, interleaved), ora.pair_size(part.double(), 64, interleaved)
+    out = torch.empty(2, 4, 9, 128, dtype=torch.bfloat16, device="cuda").transpose(1, 2)
+    assert rotary.rope(part, table, pos, interleaved=interleaved, out=out) is out
+    _close(out, want, size, 4)
+    rotary.rope(part, table, pos, interleaved=interleaved, out=part)  # in place
+    assert torch.equal(part, out)
+    assert torch.equal(qkv[:, :, :4], before[:, :, :4]) and torch.equal(qkv[:, :, 8:], before[:, :, 8:])
+    back = rotary.rope(part, table, pos, interleaved=interleaved, inverse=True)
+    _close(back, ora.turn(part.double(), -theta, interleaved), ora.pair_size(part.double(), 64, interleaved), 4)
+    # a head that all heads share (stride 0), and head-major tensors
+    one = _x(2, 9, 1, 128, dtype=torch.bfloat16).expand(2, 9, 5, 128)
+    want = ora.turn(one.double(), theta, interleaved)
+    _close(rotary.rope(one, table, pos, interleaved=interleaved), want, ora.pair_size(one.double(), 64, interleaved), 4)
+
+
+def test_rope_special_values(cuda):
+    f = rotary.rope_frequencies(16)
+    table = rotary.rope_table(f, 8)
+    x = _x(1, 3, 2, 32, dtype=torch.float16)
+    x[0, 1, 0, 0] = float("inf")
+    x[0, 1, 1, 31] = float("nan")  # not turned: stays alone
+    x[0, 2, 0, 3] = 6e-8
+    y = rotary.rope(x, table)
+    bad = ~torch.isfinite(y)
+    assert bad[0, 1, 0, :2].any() and bad[0, 1, 1, 31] and int(bad.sum()) <= 3
+    assert not bad[0, 0].any() and not bad[0, 2].any()
+
+
+def test_unknown_positions_are_zeros_and_reported(cuda):
+    table = rotary.rope_table(rotary.rope_frequencies(64), 10)
+    x = _x(1, 4, 3, 64, dtype=torch.bfloat16)
+    pos = torch.tensor([3, 10, -1, 9], device="cuda")
+    y = rotary.rope(x, table, pos)
+    with pytest.raises(CastError):
+        _quiet()
+    assert (y[0, 1:3] == 0).all() and (y[0, 0] != 0).any() and (y[0, 3] != 0).any()
+    _quiet()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("b,l,hq,hk,d,r,f32,per_head", [
+    (1, 1, 1, 1, 64, 64, False, False), (3, 1, 32, 8, 128, 128, True, False), (2, 37, 6, 2, 128, 64, False, True),
+    (1, 130, 5, 5, 80, 48, True, True), (2, 9, 3, 1, 256, 256, False, False), (1, 17, 24, 24, 96, 0, False, False)])
+def test_qk_norm_rope(cuda, dtype, interleaved, b, l, hq, hk, d, r, f32, per_head):
+    qkv = _x(b, l, hq + 2 * hk, d, dtype=dtype)
+    q, k = qkv[:, :, :hq], qkv[:, :, hq:hq + hk]
+    wt = torch.float32 if f32 else dtype
+    qw, kw = (1 + _x(*((h, d) if per_head else (d,)), dtype=torch.float32, seed=h) / 8 for h in (hq, hk))
+    qw, kw = qw.to(wt), kw.to(wt)
+    f = rotary.rope_frequencies(r) if r else None
+    table = rotary.rope_table(f, 300) if r else None
+    pos = torch.randint(0, 300, (b, l), device="cuda") if r else None
+    got = rotary.qk_norm_rope(q, k, qw, kw, table, pos, eps=1e-5, interleaved=interleaved)
+    for y, x, w in zip(got, (q, k), (qw, kw)):
+        assert y.shape == (b, x.shape[2], l, d) and y.is_contiguous()
+        z = ora.norm(x, w, 1e-5)
+        want = ora.turn(z, ora.angles(pos, f), interleaved) if r else z
+        size = ora.pair_size(z, r, interleaved) if r else z.abs()
+        _close(y.transpose(1, 2), want, size, 20)
+    _quiet()
+
+
+def test_qk_norm_rope_one_side_types_and_out(cuda):
+    f = rotary.rope_frequencies(128)
+    table = rotary.rope_table(f, 64)
+    q, k = _x(2, 11, 4, 128, dtype=torch.float32), _x(2, 11, 2, 128, dtype=torch.float32, seed=1)
+    qw = 1 + _x(128, dtype=torch.float32, seed=2) / 8
+    qo = torch.empty(2, 11, 4, 128, dtype=torch.bfloat16, device="cuda")
+    got = rotary.qk_norm_rope(q, k, qw, None, table, out_dtype=torch.bfloat16, out=(qo.transpose(1, 2), None))
+    assert got[0].data_ptr() == qo.data_ptr() and got[1].dtype == torch.bfloat16
+    theta = ora.angles(torch.arange(11, device="cuda").expand(2, 11), f)
+    for y, z in ((qo, ora.norm(q, qw, 1e-6)), (got[1].transpose(1, 2), k.double())):
+        _close(y, ora.turn(z, theta, True), ora.pair_size(z, 128, True), 20)
+    # a head of zeros: the norm of nothing is nothing
+    q[0, 0, 0] = 0
+    assert (rotary.qk_norm_rope(q, k, qw, None, table)[0][0, 0, 0] == 0).all()
+
+
+@pytest.mark.parametrize("slot_type", [torch.int32, torch.int64])
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_qk_norm_rope_into_pages(cuda, slot_type, interleaved):
+    b, l, hq, hk, d, page = 2, 21, 4, 2, 64, 16
+    f = rotary.rope_frequencies(d)
+    table = rotary.rope_table(f, 64)
+    qkv = _x(b, l, hq + 2 * hk, d, dtype=torch.bfloat16)
+    q, k, v = qkv[:, :, :hq], qkv[:, :, hq:hq + hk], qkv[:, :, hq + hk:]
+    w = 1 + _x(d, dtype=torch.bfloat16, seed=3) / 8
+    kp, vp = _x(6, hk, page, d, dtype=torch.bfloat16, seed=4), _x(6, hk, page, d, dtype=torch.bfloat16, seed=5)
+    k0, v0 = kp.clone(), vp.clone()
+    slots = torch.randperm(6 * page, device="cuda")[:b * l].view(b, l).to(slot_type)
+    slots[0, 3], slots[1, 20] = -1, 6 * page  # not written; past the end
+    got, pages = rotary.qk_norm_rope(q, k, w, w, table, interleaved=interleaved, v=v, cache=(kp, vp), slots=slots)
+    assert pages[0] is kp and pages[1] is vp
+    with pytest.raises(CastError):
+        _quiet()
+    theta = ora.angles(torch.arange(l, device="cuda").expand(b, l), f)
+    z = ora.norm(q, w, 1e-6)
+    _close(got.transpose(1, 2), ora.turn(z, theta, interleaved), ora.pair_size(z, d, interleaved), 20)
+    plain_k = rotary.qk_norm_rope(q, k, w, w, table, interleaved=interleaved)[1]
+    touched = torch.zeros(6, page, dtype=torch.bool, device="cuda")
+    for bb in range(b):
+        for t in range(l):
+            s = int(slots[bb, t])
+            if 0 <= s < 6 * page:
+                assert torch.equal(kp[s // page, :, s % page], plain_k[bb, :, t])
+                assert torch.equal(vp[s // page, :, s % page], v[bb, t])
+                touched[s // page, s % page] = True
+    left = ~touched[:, None, :, None].expand_as(kp)
+    assert torch.equal(kp[left], k0[left]) and torch.equal(vp[left], v0[left])
+    _quiet()
+
+
+def test_rotary_refusals(cuda):
+    table = rotary.rope_table(rotary.rope_frequencies(64), 10)
+    x = _x(1, 4, 3, 64, dtype=torch.bfloat16)
+    for bad in (dict(x=x.double()), dict(x=x[0]), dict(x=x.transpose(2, 3)), dict(x=x[..., :32]),
+                dict(table=table.double()), dict(table=table.cpu()), dict(start=7),
+                dict(positions=torch.zeros(5, device="cuda", dtype=torch.int32)),
+                dict(positions=torch.zeros(4, device="cuda")), dict(positions=torch.zeros(4, dtype=torch.int32)),
+                dict(axes=(16, 16)), dict(out=torch.empty_like(x[:, :2])), dict(out=x[:, :, :1].expand(1, 4, 3, 64)),
+                dict(x=x.clone().requires_grad_())):
+        args = dict(x=x, table=table)
+        args.update(bad)
+        with pytest.raises(ValueError):
+            rotary.rope(args.pop("x"), args.pop("table"), args.pop("positions", None), **args)
+    with pytest.raises(CastError, match="16-byte"):
+        rotary.rope(torch.zeros(1, 2, 2, 65, dtype=torch.bfloat16, device="cuda")[..., 1:], table)
+    y = x.clone().requires_grad_()
+    with torch.no_grad():
+        assert torch.equal(rotary.rope(y, table), rotary.rope(x, table))
+    w = torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    kp = torch.zeros(2, 3, 8, 64, dtype=torch.bfloat16, device="cuda")
+    slots = torch.zeros(1, 4, dtype=torch.int32, device="cuda")
+    for bad in (dict(k=x[:, :2]), dict(kw=w.float()), dict(kw=w[:32]), dict(qw=w.double()), dict(v=x), dict(cache=(kp, kp)),
+                dict(v=x, slots=slots, cache=(kp, kp[:1])), dict(v=x, slots=slots[:, :3], cache=(kp, kp)),
+                dict(v=x, slots=slots, cache=(kp.half(), kp.half())), dict(out_dtype=torch.float16)):
+        args = dict(k=x, qw=w, kw=w)
+        args.update(bad)
+        with pytest.raises(ValueError):
+            rotary.qk_norm_rope(x, args.pop("k"), args.pop("qw"), args.pop("kw"), table, **args)
+    assert rotary.rope(x[:, :0], table).shape == (1, 0, 3, 64)
+    assert rotary.qk_norm_rope(x[:0], x[:0], w, w, table)[0].shape == (0, 3, 4, 64)
+
+
+def test_rotary_on_another_stream_and_in_a_graph(cuda):
+    f = rotary.rope_frequencies(128)
+    table = rotary.rope_table(f, 256)
+    x = _x(2, 64, 8, 128, dtype=torch.bfloat16)
+    w = torch.ones(128, dtype=torch.bfloat16, device="cuda")
+    want = rotary.rope(x, table)
+    wq, wk = rotary.qk_norm_rope(x, x[:, :, :2], w, w, table)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = rotary.rope(x, table)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want)
+    still = x.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = rotary.rope(still, table)
+        gq, gk = rotary.qk_norm_rope(still, still[:, :, :2], w, w, table)
+    still.zero_()
+    g.replay()
+    assert (y == 0).all() and (gq == 0).all()
+    still.copy_(x)
+    g.replay()
+    assert torch.equal(y, want) and torch.equal(gq, wq) and torch.equal(gk, wk)
