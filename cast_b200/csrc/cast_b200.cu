@@ -1,6 +1,7 @@
 // Single translation unit of libcast_b200.so: the extern "C" entry points
 // declared in include/cast_b200.h and the host-side launch logic.
 #include <algorithm>
+#include <atomic>
 #include <cstdarg>
 #include <cstdlib>
 #include <cmath>
@@ -39,13 +40,20 @@ int fail(int status, const char *fmt, ...) {
 int current_device_sm100(int *num_sms) {
   int dev = 0;
   CAST_CUDA_TRY(cudaGetDevice(&dev));
-  int major = 0, minor = 0;
-  CAST_CUDA_TRY(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev));
-  CAST_CUDA_TRY(cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev));
-  if (major != 10 || minor != 0)
-    return fail(CAST_ERR_NO_DEVICE, "device %d is sm_%d%d; this library is built for sm_100a", dev,
-                major, minor);
-  if (num_sms) CAST_CUDA_TRY(cudaDeviceGetAttribute(num_sms, cudaDevAttrMultiProcessorCount, dev));
+  // what a device is never changes: asked once (its SM count)
+  static std::atomic<int> known[64];
+  int sms = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (sms <= 0) {
+    int major = 0, minor = 0;
+    CAST_CUDA_TRY(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev));
+    CAST_CUDA_TRY(cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev));
+    if (major != 10 || minor != 0)
+      return fail(CAST_ERR_NO_DEVICE, "device %d is sm_%d%d; this library is built for sm_100a", dev,
+                  major, minor);
+    CAST_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    if (dev < 64) known[dev].store(sms, std::memory_order_relaxed);
+  }
+  if (num_sms) *num_sms = sms;
   return CAST_OK;
 }
 
@@ -1153,6 +1161,7 @@ struct RotaryPositions {
 static int rotary_params(castk::RotaryParams &p, const RotaryPositions &at, int B, int L, int heads,
                          int D, int R, int flags) {
   if (B <= 0 || L <= 0 || heads <= 0) return fail(CAST_ERR_INVALID_ARGUMENT, "non-positive size");
+  if (L > (1 << 30) || B > (1 << 30)) return fail(CAST_ERR_UNSUPPORTED, "%d x %d tokens in one call", B, L);
   if (D <= 0 || D % 8 || D > 256)
     return fail(CAST_ERR_UNSUPPORTED, "head_dim %d (supported: multiples of 8 up to 256)", D);
   if (flags & ~3) return fail(CAST_ERR_INVALID_ARGUMENT, "flags %d", flags);
@@ -1163,6 +1172,10 @@ static int rotary_params(castk::RotaryParams &p, const RotaryPositions &at, int 
   if (R > 0) {
     if (!at.table || at.table_rows <= 0) return fail(CAST_ERR_INVALID_ARGUMENT, "a rotation needs a table");
     if (!aligned16(at.table)) return fail(CAST_ERR_ALIGNMENT, "the table must be 16-byte aligned");
+    if ((long long)at.table_rows * R >= (1ll << 31))
+      return fail(CAST_ERR_UNSUPPORTED, "a table of %d positions of %d pairs", at.table_rows, R / 2);
+    if (!at.positions && (at.first_position < 0 || at.first_position > (1 << 30)))
+      return fail(CAST_ERR_INVALID_ARGUMENT, "first position %lld", at.first_position);
   }
   memset(&p, 0, sizeof(p));
   p.n_axes = 1;
@@ -1182,36 +1195,44 @@ static int rotary_params(castk::RotaryParams &p, const RotaryPositions &at, int 
   p.pos64 = at.positions_64;
   p.pos_batch_stride = at.pos_batch_stride;
   p.first_position = at.first_position;
-  p.tokens = (long long)B * L;
+  p.B = B;
   p.L = L;
   p.D = D;
   p.R = R;
-  p.heads = heads;
+  p.inv_d = 1.0f / (float)D;
   p.inverse = (flags >> 1) & 1;
   p.lanes = 8;
   while (p.lanes < D / 8) p.lanes *= 2;
-  const int slots = castk::kRotaryThreads / p.lanes;
-  p.slots_per_token = 1;
-  while (p.slots_per_token < slots && p.slots_per_token < heads) p.slots_per_token *= 2;
-  p.tokens_per_cta = slots / p.slots_per_token;
-  if ((p.tokens + p.tokens_per_cta - 1) / p.tokens_per_cta >= (1ll << 31))
-    return fail(CAST_ERR_UNSUPPORTED, "%lld tokens in one call", p.tokens);
+  const int groups = castk::kRotaryThreads / p.lanes;
+  p.slots_per_token = 1, p.slots_log2 = 0;
+  while (p.slots_per_token < groups && p.slots_per_token < heads) p.slots_per_token *= 2, ++p.slots_log2;
+  // A CTA takes the tokens its lanes have room for, and up to kRotaryRun times
+  // as many one after the other while the grid still fills the device.
+  const int at_once = groups >> p.slots_log2;
+  int run = 1;
+  while (run < castk::kRotaryRun && (long long)B * (L / (at_once * run * 2)) >= 148 * 16) run *= 2;
+  p.tokens_per_cta = at_once * run;
+  return CAST_OK;
+}
+
+template <typename InT, typename OutT, bool kNorm, bool kHalf>
+static int launch_rotary(const castk::RotaryParams &p, cudaStream_t s) {
+  const int by = std::min(p.B, 32768);
+  const dim3 grid((unsigned)ceil_div(p.L, p.tokens_per_cta), (unsigned)by, (unsigned)ceil_div(p.B, by));
+  if (p.lanes == 8)
+    castk::rotary_kernel<InT, OutT, kNorm, kHalf, 8><<<grid, castk::kRotaryThreads, 0, s>>>(p);
+  else if (p.lanes == 16)
+    castk::rotary_kernel<InT, OutT, kNorm, kHalf, 16><<<grid, castk::kRotaryThreads, 0, s>>>(p);
+  else
+    castk::rotary_kernel<InT, OutT, kNorm, kHalf, 32><<<grid, castk::kRotaryThreads, 0, s>>>(p);
+  CAST_CUDA_TRY(cudaGetLastError());
   return CAST_OK;
 }
 
 template <typename InT, typename OutT>
 static int launch_rotary(const castk::RotaryParams &p, bool norm, bool half, cudaStream_t s) {
-  const unsigned grid = (unsigned)((p.tokens + p.tokens_per_cta - 1) / p.tokens_per_cta);
-  if (norm && half)
-    castk::rotary_kernel<InT, OutT, true, true><<<grid, castk::kRotaryThreads, 0, s>>>(p);
-  else if (norm)
-    castk::rotary_kernel<InT, OutT, true, false><<<grid, castk::kRotaryThreads, 0, s>>>(p);
-  else if (half)
-    castk::rotary_kernel<InT, OutT, false, true><<<grid, castk::kRotaryThreads, 0, s>>>(p);
-  else
-    castk::rotary_kernel<InT, OutT, false, false><<<grid, castk::kRotaryThreads, 0, s>>>(p);
-  CAST_CUDA_TRY(cudaGetLastError());
-  return CAST_OK;
+  if (norm) return half ? launch_rotary<InT, OutT, true, true>(p, s) : launch_rotary<InT, OutT, true, false>(p, s);
+  return half ? launch_rotary<InT, OutT, false, true>(p, s) : launch_rotary<InT, OutT, false, false>(p, s);
 }
 
 static int launch_rotary(const castk::RotaryParams &p, int dtype, int out_dtype, bool norm, bool half,
@@ -1281,7 +1302,7 @@ extern "C" int cast_qk_norm_rope(const void *q, const void *k, const void *v, in
     return fail(CAST_ERR_ALIGNMENT, "tensors must start, and their strides step, on 16-byte boundaries");
   if ((st = current_device_sm100(nullptr))) return st;
   rotary_tensor(p.t[0], q, q_out, q_weight, Hq, strides, strides + 9);
-  rotary_tensor(p.t[1], k, k_out, k_weight, Hk, strides + 3, strides + 12);
+  rotary_tensor(p.t[1], k, k_out, k_weight, Hk, strides + 3, slots ? nullptr : strides + 12);
   if (v) rotary_tensor(p.t[2], v, v_out, nullptr, Hk, strides + 6, nullptr);
   p.weight_f32 = weight_fp32;
   p.weight_per_head = weight_per_head;

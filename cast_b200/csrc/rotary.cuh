@@ -22,13 +22,26 @@
 
 #include <cuda_fp16.h>
 
+#include "attention.cuh"
 #include "common.cuh"
 #include "compact.cuh"
 
 namespace castk {
 
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 constexpr int kRotaryThreads = 128;
-constexpr int kRotaryBatch = 4;  // heads in flight per lane
+#ifndef ROT_BATCH
+#define ROT_BATCH 3
+#define ROT_RUN 4
+#define ROT_MINB 8
+#endif
+constexpr int kRotaryBatch = ROT_BATCH;  // heads in flight per lane
+constexpr int kRotaryRun = ROT_RUN;    // tokens a lane takes one after the other
 
 // One tensor of a call: q, k and (copied only) v.
 struct RotaryTensor {
@@ -49,17 +62,18 @@ struct RotaryParams {
   long long n_slots;
   int table_rows, pos64, slots64, n_axes, axis_end0, axis_end1;
   int page;
-  long long tokens;  // B * L
-  int L, D, R;
-  int heads, lanes, slots_per_token, tokens_per_cta;  // lanes of one head; head groups of a token in a CTA
+  int B, L, D, R;
+  int lanes;                        // of one head: 8, 16 or 32
+  int slots_per_token, slots_log2;  // heads of one token at once, a power of two
+  int tokens_per_cta;
   int inverse, weight_f32, weight_per_head;
-  float eps;
+  float eps, inv_d;
 };
 
 // Eight consecutive values as loaded, and their float32 values.
 template <typename T>
 struct Eight {
-  uint4 w;
+  uint4 w = {};
   __device__ __forceinline__ void load(const T *p) { w = *reinterpret_cast<const uint4 *>(p); }
   __device__ __forceinline__ void values(float (&x)[8]) const;
 };
@@ -84,7 +98,7 @@ __device__ __forceinline__ void Eight<__half>::values(float (&x)[8]) const {
 }
 template <>
 struct Eight<float> {
-  float4 a, b;
+  float4 a = {}, b = {};
   __device__ __forceinline__ void load(const float *p) {
     a = *reinterpret_cast<const float4 *>(p);
     b = *reinterpret_cast<const float4 *>(p + 4);
@@ -117,158 +131,219 @@ __device__ __forceinline__ long long load_index(const void *p, int is64, long lo
               : (long long)__ldg(static_cast<const int32_t *>(p) + i);
 }
 
-template <typename InT, typename OutT, bool kNorm, bool kHalf>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
-  constexpr int kPairs = kHalf ? 8 : 4;  // table entries of a lane's eight columns
-  int *err = &g_cast_device_error;
-  const int group = threadIdx.x / p.lanes, c = threadIdx.x % p.lanes;
-  const long long token = (long long)blockIdx.x * p.tokens_per_cta + group / p.slots_per_token;
-  const bool live_token = group < p.slots_per_token * p.tokens_per_cta && token < p.tokens;
-  const int h0 = group % p.slots_per_token;
-  const bool live = live_token && 8 * c < p.D;
-  const int b = live_token ? (int)(token / p.L) : 0;
-  const int l = live_token ? (int)(token - (long long)b * p.L) : 0;
-
-  // ---- this lane's (cos, sin): none where its columns are not rotated
+// One tensor's heads of one token: this lane's eight columns of the heads
+// h0, h0 + step, ... below t.heads.  `turn`: rotate (q and k); `at`: the
+// destination row of head 0, nullptr: nothing is written.
+template <typename InT, typename OutT, bool kNorm, bool kHalf, int kLanes>
+struct RotaryLane {
+  static constexpr int kPairs = kHalf ? 8 : 4;  // table entries of a lane's eight columns
   float cs[kPairs], sn[kPairs];
-  const bool turns = live && 8 * c < p.R;
-  bool known = true;  // every position of this token is a row of the table
-  if (p.R > 0 && live_token) {
-    long long pos[3];
-#pragma unroll
-    for (int a = 0; a < 3; ++a) {
-      if (a < p.n_axes) {
-        pos[a] = p.positions ? load_index(p.positions, p.pos64, b * p.pos_batch_stride + (long long)l * p.n_axes + a)
-                             : p.first_position + l;
-        if (pos[a] < 0 || pos[a] >= p.table_rows) {
-          known = false;
-          pos[a] = 0;
-        }
-      } else {
-        pos[a] = pos[0];
-      }
-    }
-    if (!known && c == 0 && h0 == 0) atomicExch(err, (int)CAST_ERR_INVALID_ARGUMENT);
-    if (turns) {
-      const int half_pairs = p.R / 2;
-      const int p0 = kHalf ? (8 * c) % half_pairs : 4 * c;
-      const float2 *tab = reinterpret_cast<const float2 *>(p.table);
-      if (p.n_axes == 1) {
-        const float4 *row = reinterpret_cast<const float4 *>(tab + pos[0] * half_pairs + p0);
-#pragma unroll
-        for (int i = 0; i < kPairs / 2; ++i) {
-          const float4 w = __ldg(row + i);
-          cs[2 * i] = w.x, sn[2 * i] = w.y, cs[2 * i + 1] = w.z, sn[2 * i + 1] = w.w;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-          const int pr = p0 + i;
-          const long long r = pr < p.axis_end0 ? pos[0] : (pr < p.axis_end1 ? pos[1] : pos[2]);
-          const float2 w = __ldg(tab + r * half_pairs + pr);
-          cs[i] = w.x, sn[i] = w.y;
-        }
-      }
-      // (kHalf: the second value of a pair reads y_b = z_b c + z_a s, the first y_a = z_a c - z_b s)
-      const bool flip = (p.inverse != 0) != (kHalf && 8 * c < half_pairs);
-      if (flip) {
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) sn[i] = -sn[i];
-      }
-    }
-  }
-  const int half_chunks = p.R / 16;
-  const int partner = kHalf ? (threadIdx.x & 31) - c + (c < half_chunks ? c + half_chunks : c - half_chunks) : 0;
+  bool live, turns;
+  bool blank;  // this token's position is unknown: its q and k are zeros
+  int c, h0, step, partner;
 
-  long long slot = -1;
-  if (p.slots && live_token) {
-    slot = load_index(p.slots, p.slots64, token);
-    if (slot >= p.n_slots) {
-      if (c == 0 && h0 == 0) atomicExch(err, (int)CAST_ERR_INVALID_ARGUMENT);
-      slot = -1;
+  template <bool kBlank>
+  __device__ __forceinline__ void load(const RotaryParams &p, const RotaryTensor &t, const InT *row, int hb,
+                                       Eight<InT> (&raw)[kRotaryBatch]) const {
+    const InT *src = row + (long long)(hb + h0) * t.ss[2];
+#pragma unroll
+    for (int u = 0; u < kRotaryBatch; ++u) {
+      if (live && hb + u * step + h0 < t.heads) raw[u].load(src);
+      src += step * t.ss[2];
+    }
+    if (kBlank && blank) {
+#pragma unroll
+      for (int u = 0; u < kRotaryBatch; ++u) raw[u] = Eight<InT>{};
     }
   }
 
-  const int e1 = p.t[0].heads, e2 = e1 + p.t[1].heads;
-  for (int hb = 0; hb < p.heads; hb += p.slots_per_token * kRotaryBatch) {  // same trip count in the whole CTA
-    Eight<InT> raw[kRotaryBatch];
-#pragma unroll
-    for (int u = 0; u < kRotaryBatch; ++u) {
-      const int h = hb + u * p.slots_per_token + h0;
-      if (live && h < p.heads) {
-        const int ti = h < e1 ? 0 : (h < e2 ? 1 : 2);
-        const int th = h - (ti == 0 ? 0 : (ti == 1 ? e1 : e2));
-        const RotaryTensor &t = p.t[ti];
-        raw[u].load(static_cast<const InT *>(t.src) + b * t.ss[0] + l * t.ss[1] + th * t.ss[2] + 8 * c);
+  template <bool kTurn>
+  __device__ __forceinline__ void run(const RotaryParams &p, const RotaryTensor &t, const InT *row, OutT *at,
+                                      long long at_step, Eight<InT> (&raw)[kRotaryBatch]) const {
+    uint64_t w[4];  // the weight's eight values, in pairs
+    auto weight = [&](int h) {
+      const long long wo = (p.weight_per_head ? (long long)h * p.D : 0) + 8 * c;
+      float f[8];
+      if (p.weight_f32) {
+        Eight<float> e;
+        e.load(static_cast<const float *>(t.weight) + wo);
+        e.values(f);
+      } else {
+        Eight<InT> e;
+        e.load(static_cast<const InT *>(t.weight) + wo);
+        e.values(f);
       }
-    }
 #pragma unroll
-    for (int u = 0; u < kRotaryBatch; ++u) {
-      const int h = hb + u * p.slots_per_token + h0;
-      if (hb + u * p.slots_per_token >= p.heads) break;  // uniform
-      const bool on = live && h < p.heads;
-      const int ti = h < e1 ? 0 : (h < e2 ? 1 : 2);
-      const int th = h - (ti == 0 ? 0 : (ti == 1 ? e1 : e2));
-      const RotaryTensor &t = p.t[ti];
-      float x[8];
-      if (on) {
+      for (int i = 0; i < 4; ++i) w[i] = f2_pack(f[2 * i], f[2 * i + 1]);
+    };
+    const bool normed = kNorm && kTurn && t.weight != nullptr;
+    if (normed && live && !p.weight_per_head) weight(0);
+    for (int hb = 0; hb < t.heads; hb += step * kRotaryBatch) {  // same trip count in the whole CTA
+      if (hb > 0) load<kTurn>(p, t, row, hb, raw);
+      OutT *dst = at + (long long)(hb + h0) * at_step;
+#pragma unroll
+      for (int u = 0; u < kRotaryBatch; ++u, dst += step * at_step) {
+        if (hb + u * step >= t.heads) break;  // uniform
+        const int h = hb + u * step + h0;
+        const bool on = live && h < t.heads;
+        float x[8];  // (lanes without a head compute what they hold and write nothing)
         raw[u].values(x);
-      } else {
+        if (normed) {
+          uint64_t x2[4], sum2 = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-      }
-      if (kNorm) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
-        for (int s = p.lanes >> 1; s >= 1; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-        if (on && t.weight) {
-          const float r = rsqrtf(sum / (float)p.D + p.eps);
-          const long long wo = (p.weight_per_head ? (long long)th * p.D : 0) + 8 * c;
-          float w[8];
-          if (p.weight_f32) {
-            Eight<float> e;
-            e.load(static_cast<const float *>(t.weight) + wo);
-            e.values(w);
-          } else {
-            Eight<InT> e;
-            e.load(static_cast<const InT *>(t.weight) + wo);
-            e.values(w);
+          for (int i = 0; i < 4; ++i) {
+            x2[i] = f2_pack(x[2 * i], x[2 * i + 1]);
+            sum2 = f2_fma(x2[i], x2[i], sum2);
           }
+          float lo, hi;
+          f2_unpack(sum2, lo, hi);
+          float sum = lo + hi;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
+          for (int s = kLanes / 2; s >= 1; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+          const float r = rsqrtf(fmaf(sum, p.inv_d, p.eps));
+          const uint64_t r2 = f2_pack(r, r);
+          if (p.weight_per_head && on) weight(h);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) f2_unpack(f2_mul(f2_mul(x2[i], r2), w[i]), x[2 * i], x[2 * i + 1]);
         }
-      }
-      const bool rot = turns && ti < 2;
-      if (kHalf) {
+        if (kTurn && kHalf) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float o = __shfl_sync(0xffffffffu, x[i], partner & 31);
-          if (rot) x[i] = fmaf(x[i], cs[i], o * sn[i]);
+          for (int i = 0; i < 8; ++i) {
+            const float o = __shfl_sync(0xffffffffu, x[i], partner);
+            if (turns) x[i] = fmaf(x[i], cs[i], o * sn[i]);
+          }
+        } else if (kTurn && turns) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float a = x[2 * i], q = x[2 * i + 1];
+            x[2 * i] = fmaf(a, cs[i], -(q * sn[i]));
+            x[2 * i + 1] = fmaf(a, sn[i], q * cs[i]);
+          }
         }
-      } else if (rot) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float a = x[2 * i], q = x[2 * i + 1];
-          x[2 * i] = fmaf(a, cs[i], -(q * sn[i]));
-          x[2 * i + 1] = fmaf(a, sn[i], q * cs[i]);
-        }
+        if (on && at) store8(dst, x);
       }
-      if (!on) continue;
-      if (!known && ti < 2) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-      }
-      long long at;
-      if (p.slots && ti > 0) {
-        if (slot < 0) continue;
-        const long long pg = slot / p.page;
-        at = ((pg * t.heads + th) * p.page + (slot - pg * p.page)) * p.D;
-      } else {
-        at = b * t.ds[0] + l * t.ds[1] + th * t.ds[2];
-      }
-      store8(static_cast<OutT *>(t.dst) + at + 8 * c, x);
     }
+  }
+};
+
+template <typename InT, typename OutT, bool kNorm, bool kHalf, int kLanes>
+__global__ void __launch_bounds__(kRotaryThreads, ROT_MINB) rotary_kernel(const __grid_constant__ RotaryParams p) {
+  RotaryLane<InT, OutT, kNorm, kHalf, kLanes> f;
+  constexpr int kPairs = f.kPairs;
+  int *err = &g_cast_device_error;
+  f.c = threadIdx.x & (kLanes - 1);
+  const int c = f.c, group = threadIdx.x / kLanes;
+  f.step = p.slots_per_token;  // a power of two
+  f.h0 = group & (p.slots_per_token - 1);
+  const int b = blockIdx.y + blockIdx.z * gridDim.y;
+  if (b >= p.B) return;  // (whole CTAs)
+  const int half_pairs = p.R >> 1, half_chunks = p.R >> 4;
+  const int pair0 = kHalf ? (c < half_chunks ? 8 * c : 8 * (c - half_chunks)) : 4 * c;
+  const bool flip = (p.inverse != 0) != (kHalf && c < half_chunks);
+  f.partner = kHalf ? (((threadIdx.x & 31) - c + (c < half_chunks ? c + half_chunks : c - half_chunks)) & 31) : 0;
+
+  const InT *src[3];
+  OutT *dst[3];
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    src[i] = static_cast<const InT *>(p.t[i].src) + b * p.t[i].ss[0] + 8 * c;
+    dst[i] = static_cast<OutT *>(p.t[i].dst) + b * p.t[i].ds[0] + 8 * c;
+  }
+  Eight<InT> raw[kRotaryBatch] = {};  // zeros where a lane has no column: they enter a head's sum
+  const int l_end = min(p.L, (int)(blockIdx.x + 1) * p.tokens_per_cta);
+  for (int l = blockIdx.x * p.tokens_per_cta + (group >> p.slots_log2);; l += (kRotaryThreads / kLanes) >> p.slots_log2) {
+    // the lanes of a warp may have different tokens: it leaves together
+    if (!__any_sync(0xffffffffu, l < l_end)) break;
+    const bool live_token = l < l_end;
+    f.live = live_token && 8 * c < p.D;
+    f.turns = f.live && 8 * c < p.R;
+
+    // on its way while the position and then its table row are fetched
+    f.blank = false;
+    f.template load<false>(p, p.t[0], src[0] + l * p.t[0].ss[1], 0, raw);
+
+    // ---- this lane's (cos, sin): none where its columns are not rotated
+    if (p.R > 0) {
+      int pos[3] = {0, 0, 0};
+      bool known = true;  // every position of this token is a row of the table
+      if (live_token) {
+        if (!p.positions) {
+          pos[0] = (int)p.first_position + l;
+          known = pos[0] < p.table_rows;
+        } else {
+          const long long at = b * p.pos_batch_stride + (long long)l * p.n_axes;
+#pragma unroll
+          for (int a = 0; a < 3; ++a) {
+            if (a > 0 && p.n_axes == 1) break;
+            if (p.pos64) {
+              const long long v = __ldg(static_cast<const long long *>(p.positions) + at + a);
+              known = known && v >= 0 && v < p.table_rows;
+              pos[a] = (int)v;
+            } else {
+              pos[a] = __ldg(static_cast<const int32_t *>(p.positions) + at + a);
+              known = known && (uint32_t)pos[a] < (uint32_t)p.table_rows;
+            }
+          }
+        }
+      }
+      if (__any_sync(0xffffffffu, !known)) {
+        if (!known) {  // zeros, and said so
+          pos[0] = pos[1] = pos[2] = 0;
+          if (c == 0 && f.h0 == 0) atomicExch(err, (int)CAST_ERR_INVALID_ARGUMENT);
+          f.blank = true;
+#pragma unroll
+          for (int u = 0; u < kRotaryBatch; ++u) raw[u] = Eight<InT>{};
+        }
+      }
+      if (f.turns) {
+        const float2 *tab = reinterpret_cast<const float2 *>(p.table) + pair0;
+        if (p.n_axes == 1) {
+          const float4 *row = reinterpret_cast<const float4 *>(tab + pos[0] * half_pairs);
+#pragma unroll
+          for (int i = 0; i < kPairs / 2; ++i) {
+            const float4 w = __ldg(row + i);
+            f.cs[2 * i] = w.x, f.sn[2 * i] = w.y, f.cs[2 * i + 1] = w.z, f.sn[2 * i + 1] = w.w;
+          }
+        } else {
+          const float2 *row[3];
+#pragma unroll
+          for (int a = 0; a < 3; ++a) row[a] = tab + pos[a] * half_pairs;
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) {
+            const float2 w = __ldg((pair0 + i < p.axis_end0 ? row[0] : pair0 + i < p.axis_end1 ? row[1] : row[2]) + i);
+            f.cs[i] = w.x, f.sn[i] = w.y;
+          }
+        }
+        // (kHalf: the second value of a pair takes y_b = z_b c + z_a s, the first y_a = z_a c - z_b s)
+        if (flip) {
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) f.sn[i] = -f.sn[i];
+        }
+      }
+    }
+    f.template run<true>(p, p.t[0], src[0] + l * p.t[0].ss[1], dst[0] + l * p.t[0].ds[1], p.t[0].ds[2], raw);
+    if (p.t[1].heads == 0) continue;  // uniform
+
+    f.template load<true>(p, p.t[1], src[1] + l * p.t[1].ss[1], 0, raw);
+    if (!p.slots) {
+      f.template run<true>(p, p.t[1], src[1] + l * p.t[1].ss[1], dst[1] + l * p.t[1].ds[1], p.t[1].ds[2], raw);
+      continue;
+    }
+    // place of this token's key and value in the cache
+    long long place = -1;
+    if (live_token) {
+      const long long slot = load_index(p.slots, p.slots64, (long long)b * p.L + l);
+      if (slot >= p.n_slots) {
+        if (c == 0 && f.h0 == 0) atomicExch(err, (int)CAST_ERR_INVALID_ARGUMENT);
+      } else if (slot >= 0) {
+        const long long pg = slot <= 0x7fffffff ? (long long)((uint32_t)slot / (uint32_t)p.page) : slot / p.page;
+        place = (pg * p.t[1].heads * p.page + (slot - pg * p.page)) * p.D;
+      }
+    }
+    const long long head = (long long)p.page * p.D;
+    f.template run<true>(p, p.t[1], src[1] + l * p.t[1].ss[1], place < 0 ? nullptr : dst[1] + place, head, raw);
+    f.template load<false>(p, p.t[2], src[2] + l * p.t[2].ss[1], 0, raw);
+    f.template run<false>(p, p.t[2], src[2] + l * p.t[2].ss[1], place < 0 ? nullptr : dst[2] + place, head, raw);
   }
 }
 

@@ -45,8 +45,6 @@ def _check(name: str, t, ndim: int, dtypes, device=None) -> None:
         raise ValueError(f"{name}: the last dimension must be contiguous")
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, not {device}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} needs a gradient, which this operator has not (use torch.no_grad())")
 
 
 def _check_out(name: str, t, shape, dtype, device) -> None:
@@ -68,18 +66,45 @@ def _strides(t: torch.Tensor, order) -> list[int]:
     return [stride[d] if shape[d] > 1 else 0 for d in order]
 
 
-def _on(device: torch.device):
-    """The launch's device made current (entry points launch on the current one)."""
-    return torch.cuda.device(device)
+# Checked calls, by all that their checks look at (types, shapes, strides,
+# devices, options; no tensor, address or value): a call like an earlier one
+# is launched without checking it again.
+_PLANS_KEPT = 4096
+_fn: dict[str, object] = {}
 
 
-def _call(device: torch.device, name: str, *args) -> None:
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
-        _lib.call(name, *args, stream)
+def _sig(t):
+    return None if t is None else (t.dtype, t.shape, t.stride(), t.device)
+
+
+def _keep(plans: dict, key, plan):
+    if len(plans) >= _PLANS_KEPT:
+        plans.clear()
+    plans[key] = plan
+    return plan
+
+
+def _no_grad_needed(*tensors) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("an input needs a gradient, which this operator has not (use torch.no_grad())")
+
+
+def _launch(index: int, name: str, *args) -> None:
+    """Calls an entry point on the current stream of device ``index``, which
+    is made current for the call."""
+    fn = _fn.get(name)
+    if fn is None:
+        fn = _fn[name] = getattr(_lib.load(), name)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        status = fn(*args, stream)
     else:
-        with _on(device):
-            _lib.call(name, *args, stream)
+        with torch.cuda.device(index):
+            status = fn(*args, stream)
+    if status:
+        _lib.check(status, name)
 
 
 def rope_frequencies(rotary_dim: int, *, base: float = 10000.0, axes=None, scaling=None) -> torch.Tensor:
@@ -144,13 +169,13 @@ def rope_table(frequencies: torch.Tensor, positions: int, *, amplitude: float = 
 
 
 def _turns(table, positions, axes, b, l, d, interleaved, inverse, start, device):
-    """Checked arguments of the rotation, in the entry points' order:
-    ``(table, rows, positions, 64 bit, batch stride, first, axes), R, flags, held``."""
+    """Checked arguments of the rotation: ``(rows, 64 bit, batch stride, first,
+    axes), R, flags``."""
     flags = (1 if interleaved else 0) | (2 if inverse else 0)
     if table is None:
         if positions is not None or axes is not None:
             raise ValueError("positions and axes need a table")
-        return (None, 0, None, 0, 0, 0, None), 0, flags
+        return (0, 0, 0, 0, None), 0, flags
     _check("table", table, 3, (torch.float32,), device)
     if table.shape[2] != 2 or not table.is_contiguous():
         raise ValueError("table must be a contiguous [positions, pairs, 2]")
@@ -165,7 +190,7 @@ def _turns(table, positions, axes, b, l, d, interleaved, inverse, start, device)
     if positions is None:
         if start < 0 or start + l > table.shape[0]:
             raise ValueError(f"positions {start}..{start + l - 1} run past the table's {table.shape[0]}")
-        return (table.data_ptr(), table.shape[0], None, 0, 0, int(start), ax), r, flags
+        return (table.shape[0], 0, 0, int(start), ax), r, flags
     if start:
         raise ValueError("start is for calls without positions")
     shape = positions.shape
@@ -179,8 +204,26 @@ def _turns(table, positions, axes, b, l, d, interleaved, inverse, start, device)
     _check("positions", positions, len(shape), _POSITION_TYPES, device)
     if not positions.is_contiguous():
         raise ValueError("positions must be contiguous")
-    return (table.data_ptr(), table.shape[0], positions.data_ptr(), int(positions.dtype == torch.int64), batch, 0,
-            ax), r, flags
+    return (table.shape[0], int(positions.dtype == torch.int64), batch, 0, ax), r, flags
+
+
+_rope_plans: dict = {}
+_norm_plans: dict = {}
+
+
+def _rope_plan(x, table, positions, interleaved, axes, inverse, start, out):
+    _check("x", x, 4, DTYPES)
+    if table is None:
+        raise ValueError("table is required")
+    b, l, h, d = x.shape
+    dev = x.device
+    (rows, p64, batch, first, ax), r, flags = _turns(table, positions, axes, b, l, d, interleaved, inverse, start, dev)
+    if out is None:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    else:
+        _check_out("out", out, x.shape, x.dtype, dev)
+    strides = _Six(*_strides(x, (0, 1, 2)), *_strides(out, (0, 1, 2)))
+    return (x.numel() == 0, dev.index, DTYPES[x.dtype], rows, (p64, batch, first, ax, b, l, h, d, r, flags, strides))
 
 
 def rope(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor | None = None, *, interleaved: bool = True,
@@ -197,19 +240,83 @@ def rope(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor | None = 
     allowed.  A position that is no row of the table gives zeros and sets the
     device error word (:func:`cast_b200._lib.check_device`).
     """
-    _check("x", x, 4, DTYPES)
-    b, l, h, d = x.shape
-    dev = x.device
-    where, r, flags = _turns(table, positions, axes, b, l, d, interleaved, inverse, start, dev)
+    if axes is not None:
+        axes = tuple(axes)
+    try:
+        key = (_sig(x), _sig(table), _sig(positions), interleaved, axes, inverse, start, _sig(out))
+        plan = _rope_plans.get(key)
+    except AttributeError:
+        key = plan = None  # (not a tensor: the checks say so)
+    if plan is None:
+        plan = _keep(_rope_plans, key, _rope_plan(x, table, positions, interleaved, axes, inverse, start, out))
+    empty, index, dtype, rows, rest = plan
+    _no_grad_needed(x, table, out)
     if out is None:
-        out = torch.empty((b, l, h, d), dtype=x.dtype, device=dev)
-    else:
-        _check_out("out", out, x.shape, x.dtype, dev)
-    if x.numel() == 0:
-        return out
-    strides = _Six(*_strides(x, (0, 1, 2)), *_strides(out, (0, 1, 2)))
-    _call(dev, "cast_rope", x.data_ptr(), DTYPES[x.dtype], *where, b, l, h, d, r, flags, strides, out.data_ptr())
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    if not empty:
+        _launch(index, "cast_rope", x.data_ptr(), dtype, table.data_ptr(), rows,
+                None if positions is None else positions.data_ptr(), *rest, out.data_ptr())
     return out
+
+
+def _norm_plan(q, k, q_weight, k_weight, table, positions, interleaved, axes, start, out_dtype, qo, ko, v, cache, slots):
+    _check("q", q, 4, DTYPES)
+    dev, dtype = q.device, q.dtype
+    _check("k", k, 4, (dtype,), dev)
+    b, l, hq, d = q.shape
+    hk = k.shape[2]
+    if k.shape != (b, l, hk, d):
+        raise ValueError(f"k shape {tuple(k.shape)} incompatible with q {tuple(q.shape)}")
+    if out_dtype is None:
+        out_dtype = dtype
+    elif out_dtype not in DTYPES or (out_dtype != dtype and (dtype, out_dtype) != (torch.float32, torch.bfloat16)):
+        raise ValueError("out_dtype: the inputs' type, or bfloat16 of float32 inputs")
+    f32 = per_head = None
+    for name, w, h in (("q_weight", q_weight, hq), ("k_weight", k_weight, hk)):
+        if w is None:
+            continue
+        _check(name, w, w.ndim, (dtype, torch.float32), dev)
+        if tuple(w.shape) not in ((d,), (h, d)) or not w.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous [D] or [H,D], got {tuple(w.shape)}")
+        if f32 not in (None, w.dtype == torch.float32) or per_head not in (None, w.ndim == 2):
+            raise ValueError("q_weight and k_weight must have the same type and rank")
+        f32, per_head = w.dtype == torch.float32, w.ndim == 2
+    (rows, p64, batch, first, ax), r, flags = _turns(table, positions, axes, b, l, d, interleaved, False, start, dev)
+    if qo is not None:
+        _check_out("out[0]", qo, (b, hq, l, d), out_dtype, dev)
+    pages, page, slots64 = 0, 0, 0
+    if cache is not None:
+        if v is None or slots is None:
+            raise ValueError("a cache needs v and slots")
+        if ko is not None:
+            raise ValueError("the keys go to the cache: out is (q, None)")
+        _check("v", v, 4, (dtype,), dev)
+        if v.shape != k.shape:
+            raise ValueError(f"v shape {tuple(v.shape)} differs from k {tuple(k.shape)}")
+        kp, vp = cache
+        for name, t in (("k_pages", kp), ("v_pages", vp)):
+            _check(name, t, 4, (out_dtype,), dev)
+            if t.shape[1] != hk or t.shape[3] != d or t.shape != kp.shape or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous [n_pages,{hk},page,{d}], got {tuple(t.shape)}")
+        pages, page = kp.shape[0], kp.shape[2]
+        _check("slots", slots, 2, _POSITION_TYPES, dev)
+        if tuple(slots.shape) != (b, l) or not slots.is_contiguous():
+            raise ValueError(f"slots must be a contiguous {(b, l)}, got {tuple(slots.shape)}")
+        slots64 = int(slots.dtype == torch.int64)
+    elif v is not None or slots is not None:
+        raise ValueError("v and slots go with a cache")
+    elif ko is not None:
+        _check_out("out[1]", ko, (b, hk, l, d), out_dtype, dev)
+    empty = b * l == 0
+    if not empty and (hq == 0 or hk == 0 or d == 0 or (cache is not None and pages * page == 0)):
+        raise ValueError("no heads, or an empty cache")
+    strides = _Fifteen(*_strides(q, (0, 1, 2)), *_strides(k, (0, 1, 2)),
+                       *(_strides(v, (0, 1, 2)) if cache is not None else (0, 0, 0)),
+                       *((hq * l * d, d, l * d) if qo is None else _strides(qo, (0, 2, 1))),
+                       *((hk * l * d, d, l * d) if ko is None else _strides(ko, (0, 2, 1))))
+    return (empty, dev.index, out_dtype, (b, hq, l, d), (b, hk, l, d), (DTYPES[dtype], DTYPES[out_dtype]),
+            (int(bool(f32)), int(bool(per_head))), rows,
+            (p64, batch, first, ax, b, l, hq, hk, d, r, flags, strides), (slots64, pages, page))
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
@@ -234,70 +341,28 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     written; one past the end is not written and sets the device error word.
     Slots must differ from one another.
     """
-    _check("q", q, 4, DTYPES)
-    dev, dtype = q.device, q.dtype
-    _check("k", k, 4, (dtype,), dev)
-    b, l, hq, d = q.shape
-    hk = k.shape[2]
-    if k.shape != (b, l, hk, d):
-        raise ValueError(f"k shape {tuple(k.shape)} incompatible with q {tuple(q.shape)}")
-    if out_dtype is None:
-        out_dtype = dtype
-    elif out_dtype not in DTYPES or (out_dtype != dtype and (dtype, out_dtype) != (torch.float32, torch.bfloat16)):
-        raise ValueError("out_dtype: the inputs' type, or bfloat16 of float32 inputs")
-    f32 = per_head = None
-    for name, w, h in (("q_weight", q_weight, hq), ("k_weight", k_weight, hk)):
-        if w is None:
-            continue
-        _check(name, w, w.ndim, (dtype, torch.float32), dev)
-        if tuple(w.shape) not in ((d,), (h, d)) or not w.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous [D] or [H,D], got {tuple(w.shape)}")
-        if f32 not in (None, w.dtype == torch.float32) or per_head not in (None, w.ndim == 2):
-            raise ValueError("q_weight and k_weight must have the same type and rank")
-        f32, per_head = w.dtype == torch.float32, w.ndim == 2
-    where, r, flags = _turns(table, positions, axes, b, l, d, interleaved, False, start, dev)
-    qo = ko = None
-    if out is not None:
-        qo, ko = out
+    if axes is not None:
+        axes = tuple(axes)
+    qo, ko = (None, None) if out is None else out
+    kp, vp = (None, None) if cache is None else cache
+    try:
+        key = (_sig(q), _sig(k), _sig(q_weight), _sig(k_weight), _sig(table), _sig(positions), interleaved, axes, start,
+               out_dtype, _sig(qo), _sig(ko), _sig(v), _sig(kp), _sig(vp), _sig(slots))
+        plan = _norm_plans.get(key)
+    except AttributeError:
+        key = plan = None  # (not a tensor: the checks say so)
+    if plan is None:
+        plan = _keep(_norm_plans, key, _norm_plan(q, k, q_weight, k_weight, table, positions, interleaved, axes, start,
+                                                  out_dtype, qo, ko, v, cache, slots))
+    empty, index, out_dtype, q_shape, k_shape, types, weights, rows, rest, places = plan
+    _no_grad_needed(q, k, q_weight, k_weight, table, qo, ko, v, kp, vp)
     if qo is None:
-        qo = torch.empty((b, hq, l, d), dtype=out_dtype, device=dev)
-    else:
-        _check_out("out[0]", qo, (b, hq, l, d), out_dtype, dev)
-    vo, pages, page, slots64 = None, 0, 0, 0
-    if cache is not None:
-        if v is None or slots is None:
-            raise ValueError("a cache needs v and slots")
-        if ko is not None:
-            raise ValueError("the keys go to the cache: out is (q, None)")
-        _check("v", v, 4, (dtype,), dev)
-        if v.shape != k.shape:
-            raise ValueError(f"v shape {tuple(v.shape)} differs from k {tuple(k.shape)}")
-        ko, vo = cache
-        for name, t in (("k_pages", ko), ("v_pages", vo)):
-            _check(name, t, 4, (out_dtype,), dev)
-            if t.shape[1] != hk or t.shape[3] != d or t.shape != ko.shape or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous [n_pages,{hk},page,{d}], got {tuple(t.shape)}")
-        pages, page = ko.shape[0], ko.shape[2]
-        _check("slots", slots, 2, _POSITION_TYPES, dev)
-        if tuple(slots.shape) != (b, l) or not slots.is_contiguous():
-            raise ValueError(f"slots must be a contiguous {(b, l)}, got {tuple(slots.shape)}")
-        slots64 = int(slots.dtype == torch.int64)
-    elif v is not None or slots is not None:
-        raise ValueError("v and slots go with a cache")
-    elif ko is None:
-        ko = torch.empty((b, hk, l, d), dtype=out_dtype, device=dev)
-    else:
-        _check_out("out[1]", ko, (b, hk, l, d), out_dtype, dev)
-    result = (qo, ko) if cache is None else (qo, cache)
-    if b * l == 0 or d == 0:
-        return result
-    if ko.numel() == 0 or hq == 0:
-        raise ValueError("no heads, or an empty cache")
-    strides = _Fifteen(*_strides(q, (0, 1, 2)), *_strides(k, (0, 1, 2)),
-                       *(_strides(v, (0, 1, 2)) if cache is not None else (0, 0, 0)),
-                       *_strides(qo, (0, 2, 1)), *(_strides(ko, (0, 2, 1)) if cache is None else (0, 0, 0)))
-    P = _lib.ptr
-    _call(dev, "cast_qk_norm_rope", P(q), P(k), P(v), DTYPES[dtype], DTYPES[out_dtype], P(q_weight), P(k_weight),
-          int(bool(f32)), int(bool(per_head)), float(eps), *where, b, l, hq, hk, d, r, flags, strides, P(qo), P(ko),
-          P(vo), P(slots), slots64, pages, page)
-    return result
+        qo = q.new_empty(q_shape, dtype=out_dtype)
+    if cache is None and ko is None:
+        ko = q.new_empty(k_shape, dtype=out_dtype)
+    if not empty:
+        P = _lib.ptr
+        _launch(index, "cast_qk_norm_rope", q.data_ptr(), k.data_ptr(), P(v), *types, P(q_weight), P(k_weight), *weights,
+                eps, P(table), rows, P(positions), *rest, qo.data_ptr(), P(ko if cache is None else kp), P(vp), P(slots),
+                *places)
+    return (qo, ko) if cache is None else (qo, cache)

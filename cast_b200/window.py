@@ -27,13 +27,13 @@ import math
 import torch
 
 from . import _lib
-from .rotary import DTYPES, _call, _check, _check_out, _on, _strides
+from .rotary import DTYPES, _check, _check_out, _keep, _launch, _no_grad_needed, _sig, _strides
 
 _TYPES = (torch.bfloat16, torch.float16)
 _Twelve = ctypes.c_longlong * 12
 _FOREVER = 1 << 40
-# bytes of workspace a call of some shape takes on some device (asked of the library once)
-_ws_bytes: dict[tuple, int] = {}
+_plans: dict = {}
+_paged_plans: dict = {}
 
 
 def _rule(window, sinks, frame_tokens):
@@ -43,19 +43,12 @@ def _rule(window, sinks, frame_tokens):
     return min(window, _FOREVER), min(int(sinks), _FOREVER), int(frame_tokens)
 
 
-def _workspace(name: str, device: torch.device, *shape):
-    """A buffer of its own for this call (stream-ordered: the allocator hands
-    it on when the call's work is done), so calls on several streams and
-    captured graphs never share one."""
-    key = (name, device.index, *shape)
-    n = _ws_bytes.get(key)
-    if n is None:
-        with _on(device):
-            n = int(getattr(_lib.load(), name)(*shape))
-        if len(_ws_bytes) >= 4096:
-            _ws_bytes.clear()
-        _ws_bytes[key] = n
-    return (torch.empty(n, dtype=torch.uint8, device=device), n) if n else (None, 0)
+def _workspace_bytes(name: str, device: torch.device, *shape) -> int:
+    """Bytes of scratch memory of one call.  Each call takes a buffer of its
+    own (stream-ordered: the allocator hands it on when the call's work is
+    done), so calls on several streams and captured graphs never share one."""
+    with torch.cuda.device(device):
+        return int(getattr(_lib.load(), name)(*shape))
 
 
 def _lens(kv_lens, b, device):
@@ -69,6 +62,32 @@ def _heads(q, k, hk):
         raise ValueError(f"{q.shape[1]} query heads do not share {hk} key heads evenly")
     if q.shape[3] not in (64, 128) or k.shape[3] != q.shape[3]:
         raise ValueError(f"head vectors of 64 or 128 values, the same for all; got {q.shape[3]} and {k.shape[3]}")
+
+
+def _window_plan(q, k, v, window, sinks, frame_tokens, kv_lens, out):
+    _check("q", q, 4, _TYPES)
+    dev = q.device
+    _check("k", k, 4, (q.dtype,), dev)
+    _check("v", v, 4, (q.dtype,), dev)
+    b, hq, lq, d = q.shape
+    hk, lk = k.shape[1], k.shape[2]
+    _heads(q, k, hk)
+    if k.shape[0] != b or v.shape != k.shape:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)}")
+    if kv_lens is not None:
+        _lens(kv_lens, b, dev)
+    rule = _rule(window, sinks, frame_tokens)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        _check_out("out", out, q.shape, q.dtype, dev)
+    if q.numel() == 0 or lk == 0:
+        return q.numel() == 0, lk == 0, dev.index, 0, 0.0, (), ()
+    shape = (b, hq, hk, lq, lk, d)
+    n = _workspace_bytes("cast_window_attention_workspace_bytes", dev, *shape, *rule)
+    order = (0, 1, 2)
+    strides = _Twelve(*_strides(q, order), *_strides(k, order), *_strides(v, order), *_strides(out, order))
+    return False, False, dev.index, n, 1.0 / math.sqrt(d), DTYPES[q.dtype], (*shape, strides, *rule)
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int | None, sinks: int = 0,
@@ -85,34 +104,55 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     that sees nothing gives zeros.  A length outside ``[0, Lk]`` is clipped
     and sets the device error word.
     """
+    try:
+        key = (_sig(q), _sig(k), _sig(v), window, sinks, frame_tokens, _sig(kv_lens), _sig(out))
+        plan = _plans.get(key)
+    except AttributeError:
+        key = plan = None  # (not a tensor: the checks say so)
+    if plan is None:
+        plan = _keep(_plans, key, _window_plan(q, k, v, window, sinks, frame_tokens, kv_lens, out))
+    empty, blind, index, nbytes, scale, dtype, rest = plan
+    _no_grad_needed(q, k, v, out)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if empty:
+        return out
+    if blind:
+        return out.zero_()
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _launch(index, "cast_window_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype,
+            None if kv_lens is None else kv_lens.data_ptr(), *rest, scale if sm_scale is None else sm_scale,
+            out.data_ptr(), _lib.ptr(ws), nbytes)
+    return out
+
+
+def _paged_plan(q, k_pages, v_pages, block_table, kv_lens, window, sinks, frame_tokens, out):
     _check("q", q, 4, _TYPES)
     dev = q.device
-    _check("k", k, 4, (q.dtype,), dev)
-    _check("v", v, 4, (q.dtype,), dev)
+    _check("k_pages", k_pages, 4, (q.dtype,), dev)
+    _check("v_pages", v_pages, 4, (q.dtype,), dev)
     b, hq, lq, d = q.shape
-    hk, lk = k.shape[1], k.shape[2]
-    _heads(q, k, hk)
-    if k.shape[0] != b or v.shape != k.shape:
-        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit q {tuple(q.shape)}")
-    if kv_lens is not None:
-        _lens(kv_lens, b, dev)
+    pages, hk, page, _ = k_pages.shape
+    _heads(q, k_pages, hk)
+    if v_pages.shape != k_pages.shape:
+        raise ValueError(f"v_pages {tuple(v_pages.shape)} differs from k_pages {tuple(k_pages.shape)}")
+    _check("block_table", block_table, 2, (torch.int32,), dev)
+    if block_table.shape[0] != b or not block_table.is_contiguous():
+        raise ValueError(f"block_table must be a contiguous int32 [{b}, max_pages], got {tuple(block_table.shape)}")
+    _lens(kv_lens, b, dev)
     rule = _rule(window, sinks, frame_tokens)
     if out is None:
-        out = torch.empty((b, hq, lq, d), dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _check_out("out", out, q.shape, q.dtype, dev)
-    if q.numel() == 0:
-        return out
-    if lk == 0:
-        return out.zero_()
-    scale = 1.0 / math.sqrt(d) if sm_scale is None else float(sm_scale)
-    ws, nbytes = _workspace("cast_window_attention_workspace_bytes", dev, b, hq, hk, lq, lk, d, *rule)
+    max_pages = block_table.shape[1]
+    if q.numel() == 0 or max_pages * pages * page == 0:
+        return q.numel() == 0, max_pages * pages * page == 0, dev.index, 0, 0.0, (), (), ()
+    n = _workspace_bytes("cast_paged_window_attention_workspace_bytes", dev, b, hq, hk, lq, d, page, max_pages, *rule)
     order = (0, 1, 2)
-    strides = _Twelve(*_strides(q, order), *_strides(k, order), *_strides(v, order), *_strides(out, order))
-    P = _lib.ptr
-    _call(dev, "cast_window_attention", P(q), P(k), P(v), DTYPES[q.dtype], P(kv_lens), b, hq, hk, lq, lk, d, strides,
-          *rule, scale, P(out), P(ws), nbytes)
-    return out
+    strides = _Twelve(*_strides(q, order), *_strides(k_pages, order), *_strides(v_pages, order), *_strides(out, order))
+    return (False, False, dev.index, n, 1.0 / math.sqrt(d), DTYPES[q.dtype], (max_pages, pages, page),
+            (b, hq, hk, lq, d, strides, *rule))
 
 
 def paged_window_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
@@ -129,34 +169,25 @@ def paged_window_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     device error word, as a length outside ``[0, max_pages * page]`` does.
     Sessions may share pages (a common prefix).
     """
-    _check("q", q, 4, _TYPES)
-    dev = q.device
-    _check("k_pages", k_pages, 4, (q.dtype,), dev)
-    _check("v_pages", v_pages, 4, (q.dtype,), dev)
-    b, hq, lq, d = q.shape
-    pages, hk, page, _ = k_pages.shape
-    _heads(q, k_pages, hk)
-    if v_pages.shape != k_pages.shape:
-        raise ValueError(f"v_pages {tuple(v_pages.shape)} differs from k_pages {tuple(k_pages.shape)}")
-    _check("block_table", block_table, 2, (torch.int32,), dev)
-    if block_table.shape[0] != b or not block_table.is_contiguous():
-        raise ValueError(f"block_table must be a contiguous int32 [{b}, max_pages], got {tuple(block_table.shape)}")
-    _lens(kv_lens, b, dev)
-    rule = _rule(window, sinks, frame_tokens)
+    try:
+        key = (_sig(q), _sig(k_pages), _sig(v_pages), _sig(block_table), _sig(kv_lens), window, sinks, frame_tokens,
+               _sig(out))
+        plan = _paged_plans.get(key)
+    except AttributeError:
+        key = plan = None  # (not a tensor: the checks say so)
+    if plan is None:
+        plan = _keep(_paged_plans, key, _paged_plan(q, k_pages, v_pages, block_table, kv_lens, window, sinks,
+                                                    frame_tokens, out))
+    empty, blind, index, nbytes, scale, dtype, pages, rest = plan
+    _no_grad_needed(q, k_pages, v_pages, out)
     if out is None:
-        out = torch.empty((b, hq, lq, d), dtype=q.dtype, device=dev)
-    else:
-        _check_out("out", out, q.shape, q.dtype, dev)
-    if q.numel() == 0:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if empty:
         return out
-    max_pages = block_table.shape[1]
-    if max_pages == 0 or pages == 0 or page == 0:
+    if blind:
         return out.zero_()
-    scale = 1.0 / math.sqrt(d) if sm_scale is None else float(sm_scale)
-    ws, nbytes = _workspace("cast_paged_window_attention_workspace_bytes", dev, b, hq, hk, lq, d, page, max_pages, *rule)
-    order = (0, 1, 2)
-    strides = _Twelve(*_strides(q, order), *_strides(k_pages, order), *_strides(v_pages, order), *_strides(out, order))
-    P = _lib.ptr
-    _call(dev, "cast_paged_window_attention", P(q), P(k_pages), P(v_pages), DTYPES[q.dtype], P(block_table), max_pages,
-          pages, page, P(kv_lens), b, hq, hk, lq, d, strides, *rule, scale, P(out), P(ws), nbytes)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _launch(index, "cast_paged_window_attention", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), dtype,
+            block_table.data_ptr(), *pages, kv_lens.data_ptr(), *rest, scale if sm_scale is None else sm_scale,
+            out.data_ptr(), _lib.ptr(ws), nbytes)
     return out

@@ -106,3 +106,10 @@ def _paged(lib, **kw):
 def test_paged_window_attention_refused(lib, kw, status, text):
     assert _paged(lib, **kw) == status
     assert text in lib.cast_last_error_message()
+
+
+def test_python_refuses_what_is_no_tensor():
+    with pytest.raises(ValueError, match="CUDA"):
+        window.window_attention([1], None, None, window=4)
+    with pytest.raises(ValueError, match="CUDA"):
+        window.paged_window_attention(None, None, None, None, None, window=4)
