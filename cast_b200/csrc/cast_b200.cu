@@ -20,6 +20,7 @@
 #include "swap_router.cuh"
 #include "rotary.cuh"
 #include "window.cuh"
+#include "window_tiles.cuh"
 
 namespace cast {
 
@@ -1404,7 +1405,8 @@ static int window_dims_ok(int B, int Hq, int Hk, int Lq, int Lk, int D, long lon
   if (window <= 0 || sinks < 0 || frame <= 0)
     return fail(CAST_ERR_INVALID_ARGUMENT, "window %lld (at least 1), sinks %lld (at least 0), frame_tokens %d (at least 1)",
                 window, sinks, frame);
-  if ((long long)Hq / Hk * Lq >= (1ll << 30) || (long long)B * Hq >= (1ll << 24) || Lk >= (1 << 30))
+  if ((long long)Hq / Hk * Lq >= (1ll << 30) || (long long)B * Hq >= (1ll << 24) || Lk >= (1 << 30) ||
+      (long long)B * Hq * (Lq / 64 + 1) >= (1ll << 30))
     return fail(CAST_ERR_UNSUPPORTED, "size outside the kernels' index range");
   return CAST_OK;
 }
@@ -1455,11 +1457,175 @@ static int rows_params(castk::RowsParams &p, const void *q, const void *k, const
   return CAST_OK;
 }
 
+struct TilesPlan {
+  int pack = 1, pack_log2 = 0, head_groups = 1, q_tiles = 1, pairs = 1;
+  int n_items = 0, n_whole = 0, parts = 1;
+  size_t ws_bytes = 0;
+};
+
+// How the many-row kernel cuts a call: an item is a pair of query tiles of
+// one head group, one CTA an SM.  The items of the last, incomplete wave (or
+// of the last two) are cut along their keys into equal parts where that ends
+// sooner, counted in steps of 128 keys: an item costs its keys and about 4
+// steps to start and end, a part 2.5 more to leave and join its result.
+static TilesPlan tiles_plan(int B, int Hq, int Hk, int Lq, int Lk, long long window, long long sinks, int frame,
+                            int D, int n_sms) {
+  TilesPlan t;
+  const int group = Hq / Hk;
+  while (t.pack < 128 && group % (2 * t.pack) == 0) t.pack *= 2, ++t.pack_log2;
+  t.head_groups = Hq / t.pack;
+  const long long rows = (long long)t.pack * Lq;
+  t.q_tiles = (int)((rows + 127) / 128);
+  t.pairs = (t.q_tiles + 1) / 2;
+  t.n_items = B * t.head_groups * t.pairs;
+  const double tokens = std::min<double>(Lq, 256.0 / t.pack);
+  const double keys = std::min<double>(Lk, (double)(window + sinks) * frame + tokens + (frame > 1 ? frame : 0));
+  const double c = std::max(1.0, keys / 128) * (t.q_tiles == 1 ? 0.5 : 1.0);
+  const int waves = t.n_items / n_sms, rem = t.n_items % n_sms;
+  t.n_whole = t.n_items;
+  double best = (waves + (rem ? 1 : 0)) * (c + 4.0);
+  for (int q = 0; q <= 1 && q <= waves; ++q) {
+    const int cut = rem + q * n_sms;
+    if (cut == 0) continue;
+    for (int parts = 2; parts <= 128 && c / parts >= 2.0; ++parts) {
+      const double rounds = std::ceil((double)cut * parts / n_sms);
+      const double cost = (waves - q) * (c + 4.0) + rounds * (c / parts + 6.5) + 0.05 * parts;
+      if (cost < 0.97 * best) {
+        best = cost;
+        t.parts = parts;
+        t.n_whole = t.n_items - cut;
+      }
+    }
+  }
+  if (t.parts > 1)
+    t.ws_bytes = (size_t)(t.n_items - t.n_whole) * t.parts *
+                 (D == 128 ? castk::tiles_part_floats<128>() : castk::tiles_part_floats<64>()) * sizeof(float);
+  return t;
+}
+
+// Rows that a tile of the many-row kernel would hold mostly empty go to the
+// few-row kernel.
+static bool tiles_wanted(long long rows) { return rows > 32; }
+
+// A tiled map of 16-bit elements (strides in elements; the first dimension
+// is dense and 64 wide in the box); dimensions of one element may have any
+// stride.
+static int make_map_rows(CUtensorMap *map, const void *base, int dtype, int rank, const uint64_t *dims,
+                         const long long *strides, const uint32_t *box) {
+  EncodeTiledFn enc;
+  int st = get_encode_tiled(&enc);
+  if (st) return st;
+  cuuint64_t d[5], str[4];
+  cuuint32_t bx[5], es[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    bx[i] = box[i];
+    if (i > 0) str[i - 1] = (cuuint64_t)(strides[i - 1] > 0 ? strides[i - 1] : 8) * 2;
+  }
+  CUresult r = enc(map, dtype == kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+                   const_cast<void *>(base), d, str, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(CAST_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return CAST_OK;
+}
+
+// Whether the strides are such that tensor maps can hold them: steps of
+// dimensions with more than one element are positive and below 2^39 elements;
+// k and v may be shared by the batch or the heads (stride 0).
+static bool tiles_strides_ok(const castk::RowsParams &r) {
+  const long long most = 1ll << 38;
+  auto ok = [&](long long s, int n, bool shared) { return n == 1 || (s > 0 && s < most) || (shared && s == 0); };
+  return ok(r.qs[0], r.B, false) && ok(r.qs[1], r.Hq, false) && ok(r.qs[2], r.Lq, false) && ok(r.ks[0], r.B, true) &&
+         ok(r.ks[1], r.Hk, true) && ok(r.ks[2], r.lk, false) && ok(r.vs[0], r.B, true) && ok(r.vs[1], r.Hk, true) &&
+         ok(r.vs[2], r.lk, false);
+}
+
+template <typename T, int D>
+static int launch_tiles(const castk::RowsParams &r, const TilesPlan &plan, int dtype, float *part, cudaStream_t s) {
+  castk::TilesParams p;
+  memset(&p, 0, sizeof(p));
+  p.out = r.out, p.v = r.v;
+  for (int i = 0; i < 3; ++i) p.os[i] = r.os[i], p.vs[i] = r.vs[i];
+  p.kv_lens = r.kv_lens;
+  p.part = part;
+  p.rule = r.rule;
+  p.B = r.B, p.Hk = r.Hk, p.Lq = r.Lq, p.lk = r.lk;
+  p.pack = plan.pack, p.pack_log2 = plan.pack_log2;
+  p.heads = r.Hq;
+  p.head_groups = plan.head_groups;
+  p.groups_per_key = plan.head_groups / r.Hk;
+  p.rows = plan.pack * r.Lq;
+  p.q_tiles = plan.q_tiles, p.pairs = plan.pairs;
+  p.n_whole = plan.n_whole, p.parts = plan.parts;
+  p.scale_log2 = r.scale_log2;
+  const long long sink_keys = std::min<long long>(r.rule.sinks * r.rule.frame, r.lk);
+  p.sinks8 = (int)((sink_keys + 7) / 8 * 8);
+  auto many = [](long long stride, int n) { return n > 1 && stride != 0; };
+  p.k_batch = many(r.ks[0], r.B), p.k_head = many(r.ks[1], r.Hk);
+  p.v_batch = many(r.vs[0], r.B), p.v_head = many(r.vs[1], r.Hk);
+
+  CUtensorMap tm_q, tm_k[3], tm_v[3];
+  int st;
+  {
+    const uint64_t dims[5] = {(uint64_t)D, (uint64_t)plan.pack, (uint64_t)r.Lq, (uint64_t)plan.head_groups, (uint64_t)r.B};
+    const long long str[4] = {r.qs[1], r.qs[2], r.qs[1] * plan.pack, r.qs[0]};
+    const uint32_t box[5] = {64, (uint32_t)plan.pack, (uint32_t)(128 / plan.pack), 1, 1};
+    if ((st = make_map_rows(&tm_q, r.q, dtype, 5, dims, str, box))) return st;
+  }
+  const uint32_t tail = p.sinks8 % 128;
+  for (int i = 0; i < 3; ++i) {  // all 128 rows of a tile, the sinks' last rows, the rows beside them
+    if (i > 0 && tail == 0) {
+      tm_k[i] = tm_k[0], tm_v[i] = tm_v[0];  // never read
+      continue;
+    }
+    const uint32_t box[4] = {64, i == 0 ? 128u : (i == 1 ? tail : 128u - tail), 1, 1};
+    const uint64_t kd[4] = {(uint64_t)D, (uint64_t)r.lk, (uint64_t)(p.k_head ? r.Hk : 1), (uint64_t)(p.k_batch ? r.B : 1)};
+    const long long ks[3] = {r.ks[2], r.ks[1], r.ks[0]};
+    if ((st = make_map_rows(&tm_k[i], r.k, dtype, 4, kd, ks, box))) return st;
+    const uint64_t vd[4] = {(uint64_t)D, (uint64_t)r.lk, (uint64_t)(p.v_head ? r.Hk : 1), (uint64_t)(p.v_batch ? r.B : 1)};
+    const long long vs[3] = {r.vs[2], r.vs[1], r.vs[0]};
+    if ((st = make_map_rows(&tm_v[i], r.v, dtype, 4, vd, vs, box))) return st;
+  }
+  auto kernel = castk::window_tiles_kernel<T, D>;
+  constexpr int smem = castk::TilesSmem<D>::alloc;
+  static std::once_flag once;
+  static cudaError_t err = cudaSuccess;
+  std::call_once(once, [&] { err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+  CAST_CUDA_TRY(err);
+  const int cut = plan.n_items - plan.n_whole;
+  kernel<<<plan.n_whole + cut * plan.parts, castk::kTilesThreads, smem, s>>>(tm_q, tm_k[0], tm_v[0], tm_k[1], tm_v[1],
+                                                                            tm_k[2], tm_v[2], p);
+  CAST_CUDA_TRY(cudaGetLastError());
+  if (cut > 0) {
+    castk::window_tiles_join_kernel<T, D><<<cut * 2 * (D / castk::kJoinCols), 128 * castk::kJoinGroups, 0, s>>>(p);
+    CAST_CUDA_TRY(cudaGetLastError());
+  }
+  return CAST_OK;
+}
+
+static int tiles_call(const castk::RowsParams &r, const TilesPlan &plan, int dtype, int D, void *workspace,
+                      size_t workspace_bytes, cudaStream_t s) {
+  if (plan.ws_bytes) {
+    if (!workspace || workspace_bytes < plan.ws_bytes)
+      return fail(CAST_ERR_WORKSPACE, "workspace of %zu bytes < %zu required", workspace ? workspace_bytes : 0, plan.ws_bytes);
+    if (!aligned16(workspace)) return fail(CAST_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+  }
+  float *part = plan.ws_bytes ? static_cast<float *>(workspace) : nullptr;
+  if (dtype == kBf16)
+    return D == 128 ? launch_tiles<__nv_bfloat16, 128>(r, plan, dtype, part, s)
+                    : launch_tiles<__nv_bfloat16, 64>(r, plan, dtype, part, s);
+  return D == 128 ? launch_tiles<__half, 128>(r, plan, dtype, part, s) : launch_tiles<__half, 64>(r, plan, dtype, part, s);
+}
+
 extern "C" size_t cast_window_attention_workspace_bytes(int B, int Hq, int Hk, int Lq, int Lk, int D,
                                                         long long window, long long sinks, int frame_tokens) {
   int n_sms = 0;
   if (window_dims_ok(B, Hq, Hk, Lq, Lk, D, window, sinks, frame_tokens) || current_device_sm100(&n_sms)) return 0;
-  return rows_plan(B, Hk, Hq / Hk, Lq, Lk, window, sinks, frame_tokens, D, n_sms).ws_bytes;
+  // (which kernel runs also depends on the strides: room for either)
+  size_t n = rows_plan(B, Hk, Hq / Hk, Lq, Lk, window, sinks, frame_tokens, D, n_sms).ws_bytes;
+  if (tiles_wanted((long long)(Hq / Hk) * Lq))
+    n = std::max(n, tiles_plan(B, Hq, Hk, Lq, Lk, window, sinks, frame_tokens, D, n_sms).ws_bytes);
+  return n;
 }
 
 extern "C" int cast_window_attention(const void *q, const void *k, const void *v, int dtype,
@@ -1474,6 +1640,9 @@ extern "C" int cast_window_attention(const void *q, const void *k, const void *v
   if (st) return st;
   int n_sms = 0;
   if ((st = current_device_sm100(&n_sms))) return st;
+  if (tiles_wanted(p.rows) && tiles_strides_ok(p))
+    return tiles_call(p, tiles_plan(B, Hq, Hk, Lq, Lk, window, sinks, frame_tokens, D, n_sms), dtype, D, workspace,
+                      workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
   const RowsPlan plan = rows_plan(B, Hk, p.group, Lq, Lk, window, sinks, frame_tokens, D, n_sms);
   return rows_call(p, plan, false, dtype, D, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
 }

@@ -1,0 +1,759 @@
+// Sliding-window attention for many query rows: tcgen05 products with TMEM
+// accumulators over the keys that the rows of a tile see.
+//
+// The mathematics and the list of keys are those of window.cuh.  One CTA
+// computes one or two 128-row query tiles: the `pack` query heads that share
+// a key head lie side by side in the rows (row = token * pack + head), so a
+// pair of tiles covers 256 / pack tokens and their windows differ by little.
+// Keys go by in tiles of 128 places of the list (8-row-aligned, so that the
+// sinks' last rows and the window's first ones share a tile: two TMA boxes).
+// Warp roles, TMEM columns, the 64-key softmax steps with a lazily moved
+// maximum and the two issuers are those of attention.cuh:
+//   warps 0-3, 4-7  softmax and epilogue of query tile 0, 1
+//   warp 8          TMA of Q and the K ring; warp 10: of the V ring
+//   warps 9, 11     one MMA-issuing thread each, for tile 0, 1
+// A single query tile is shared: each issuer and softmax warpgroup takes half
+// of its key tiles, and warpgroup 0 joins the halves.
+//
+// Masks cost only where they are: a warp whose 32 rows all see a step's 64
+// keys runs the unmasked step, one that sees none of them writes zeros without
+// an exponential, and key tiles that lie outside one query tile's own span
+// are skipped by its issuer.  A V row meets the zero weights of rows that do
+// not see it, and 0 * inf is NaN, so warp 10 goes over the V tiles that are
+// not wholly visible before they are used: rows that nobody sees become zeros;
+// in rows that only some see, infinities and NaN become zeros and are given
+// back to the rows that see them when these are written.
+#pragma once
+
+#include "window.cuh"
+
+namespace castk {
+
+constexpr int kTilesThreads = 384;
+constexpr int kTilesPartCols = 4;  // m, l, flag of a part's rows beside its O
+
+template <int D>
+struct TilesSmem {
+  static constexpr int tile = 128 * D * 2;  // one Q, K or V tile
+  static constexpr int kStages = D == 128 ? 2 : 4;
+  static constexpr int vStages = D == 128 ? 3 : 4;
+  static constexpr int k_off = 2 * tile;
+  static constexpr int v_off = k_off + kStages * tile;
+  static constexpr int bars = v_off + vStages * tile;
+  // q_full, k_full/empty, v_full/empty/raw, s_full[4], p_full[4], pv_done[4], drain[2], merge
+  static constexpr int n_bars = 1 + 2 * kStages + 3 * vStages + 12 + 2 + 1;
+  static constexpr int tmem_slot = bars + 8 * n_bars;
+  static constexpr int alloc = tmem_slot + 16 + 1024;
+};
+
+struct TilesParams {
+  void *out;
+  const void *v;
+  long long os[3], vs[3];
+  const int32_t *kv_lens;
+  float *part;
+  WindowRule rule;
+  int B, Hk, Lq, lk;
+  int pack, pack_log2;       // heads side by side in the rows of a tile, a power of two
+  int heads;                 // Hq
+  int head_groups;           // Hq / pack
+  int groups_per_key;        // head groups that share a key head
+  int rows, q_tiles, pairs;  // rows = pack * Lq of one head group
+  int n_whole, parts;        // items [0, n_whole) whole, the later ones in `parts` parts each
+  int sinks8;                // sinks of a session long enough to have a gap, rounded up to 8
+  int k_batch, k_head, v_batch, v_head;  // 0 where that dimension's stride is 0 (one box for all), else 1
+  float scale_log2;
+};
+
+template <int D>
+__host__ __device__ constexpr long long tiles_part_floats() {
+  return 2ll * 128 * (D + kTilesPartCols);
+}
+
+template <typename T>
+struct TilesType;
+template <>
+struct TilesType<__nv_bfloat16> {
+  static constexpr uint32_t fmt = 1;
+  static constexpr float kShift = 0.0f, kSlack = 8.0f, kSumLimit = 65536.0f;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
+  static __device__ __forceinline__ float add_lo(uint32_t u, float x) { return add_bf16_lo(u, x); }
+  static __device__ __forceinline__ float add_hi(uint32_t u, float x) { return add_bf16_hi(u, x); }
+};
+template <>
+struct TilesType<__half> {
+  // P = 2^(s - m + 8): a step's P sum to 2^15 at most before the maximum
+  // moves, and weights down to 2^-32 of the largest count
+  static constexpr uint32_t fmt = 0;
+  static constexpr float kShift = 8.0f, kSlack = 4.0f, kSumLimit = 32768.0f;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return Half2<__half>::pack(a, b); }
+  static __device__ __forceinline__ float add_lo(uint32_t u, float x) {
+    float r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tadd.rn.f32.f16 %0, lo, %2;\n\t}" : "=f"(r) : "r"(u), "f"(x));
+    return r;
+  }
+  static __device__ __forceinline__ float add_hi(uint32_t u, float x) {
+    float r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tadd.rn.f32.f16 %0, hi, %2;\n\t}" : "=f"(r) : "r"(u), "f"(x));
+    return r;
+  }
+};
+
+__device__ __forceinline__ void tma_load_5d(void *dst, const CUtensorMap *map, uint64_t *bar, int c0, int c1, int c2,
+                                            int c3, int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(castdev::smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(castdev::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+      : "memory");
+}
+
+// Bits n0 .. n0+31 of the interval [lo, hi).
+__device__ __forceinline__ uint32_t interval_mask(int lo, int hi, int n0) {
+  const int a = min(max(lo - n0, 0), 32), b = min(max(hi - n0, 0), 32);
+  const uint32_t below_b = b >= 32 ? 0xffffffffu : (1u << b) - 1u;
+  const uint32_t below_a = a >= 32 ? 0xffffffffu : (1u << a) - 1u;
+  return below_b & ~below_a;
+}
+
+// One 64-key step's P = 2^(S c2 - base) in pairs in v[0..31]; returns their sum as rounded.
+template <typename T, bool kMasked>
+__device__ __forceinline__ float tiles_probs(uint32_t (&v)[64], const uint32_t (&seen)[2], float c2, float base) {
+  using X = TilesType<T>;
+  const uint64_t c2x2 = f2_pack(c2, c2), nbx2 = f2_pack(-base, -base);
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < 32; ++c) {
+    float x0, x1;
+    f2_unpack(f2_fma(f2_pack(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])), c2x2, nbx2), x0, x1);
+    float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
+    if (kMasked) {
+      const uint32_t w = seen[c / 16];
+      e0 = ((w >> ((2 * c) % 32)) & 1u) ? e0 : 0.0f;
+      e1 = ((w >> ((2 * c + 1) % 32)) & 1u) ? e1 : 0.0f;
+    }
+    const uint32_t pk = X::pack(e0, e1);
+    acc[2 * (c & 3)] = X::add_lo(pk, acc[2 * (c & 3)]);
+    acc[2 * (c & 3) + 1] = X::add_hi(pk, acc[2 * (c & 3) + 1]);
+    v[c] = pk;
+  }
+  return ((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7]));
+}
+
+// The MMA issuer of one query tile: key tiles t_lo .. t_hi - 1 of its own
+// order; the tiles before and after (of a pair's common list) are handed back
+// unread.  Returns false if a wait gave up.
+template <typename T, int D>
+__device__ __forceinline__ bool tiles_issuer(int i, RingMap ring, uint32_t tmem, uint32_t sbase, int n_all, int t_lo,
+                                             int t_hi, uint64_t *q_full, uint64_t *k_full, uint64_t *k_empty,
+                                             uint64_t *v_full, uint64_t *v_empty, uint64_t *s_full, uint64_t *p_full,
+                                             uint64_t *pv_done, int *err) {
+  using S = TilesSmem<D>;
+  constexpr int KS = S::kStages, VS = S::vStages;
+  constexpr uint32_t fmt = TilesType<T>::fmt;
+  constexpr uint32_t idesc_s = castdev::make_idesc(1, fmt, fmt, 0, 0, 128, 64);
+  constexpr uint32_t idesc_pv = castdev::make_idesc(1, fmt, fmt, 0, 1, 128, D);
+  const DescW qd = desc_words(sbase + (ring.split ? 0 : i * S::tile), 16);
+  const DescW kd = desc_words(sbase + S::k_off, 16);
+  const DescW vd = desc_words(sbase + S::v_off, 16384);
+  const uint32_t o_col = tmem + i * 128, s_col = tmem + 256 + i * 128;
+  uint64_t *my_s_full = s_full + 2 * i, *my_p_full = p_full + 2 * i, *my_pv_done = pv_done + 2 * i;
+
+  auto issue_s = [&](int r, int half) {
+    const uint32_t d = s_col + half * 64;
+    const uint32_t ko = (uint32_t)(r % KS) * S::tile + half * 8192;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      const uint32_t off = (s >> 2) * 16384 + (s & 3) * 32;
+      castdev::mma_f16_ss(d, qd.at(off), kd.at(ko + off), idesc_s, s > 0);
+    }
+  };
+  // (a stage is handed back only once it is this tile's: its barrier's phase
+  // would otherwise count an arrival of another turn)
+  auto skip = [&](int t) {
+    const int r = ring.pos(t);
+    if (!castdev::mbar_wait(&k_full[r % KS], (r / KS) & 1, err)) return false;
+    castdev::mbar_arrive(&k_empty[r % KS]);
+    if (!castdev::mbar_wait(&v_full[r % VS], (r / VS) & 1, err)) return false;
+    castdev::mbar_arrive(&v_empty[r % VS]);
+    return true;
+  };
+  for (int t = 0; t < t_lo; ++t)
+    if (!skip(t)) return false;
+  if (t_lo < t_hi) {
+    int rk = ring.pos(t_lo);  // ring position of the next key tile to multiply
+    if (!castdev::mbar_wait(q_full, 0, err) || !castdev::mbar_wait(&k_full[rk % KS], (rk / KS) & 1, err)) return false;
+    castdev::tc_fence_after();
+    issue_s(rk, 0);
+    castdev::tc_commit(&my_s_full[0]);
+    issue_s(rk, 1);
+    castdev::tc_commit(&my_s_full[1]);
+    castdev::tc_commit(&k_empty[rk % KS]);
+    for (int t = t_lo; t < t_hi; ++t) {
+      const int rv = ring.pos(t), vs = rv % VS;
+      const bool more = t + 1 < t_hi;
+      if (more) rk = ring.pos(t + 1);
+      if (!castdev::mbar_wait(&v_full[vs], (rv / VS) & 1, err)) return false;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (!castdev::mbar_wait(&my_p_full[half], (t - t_lo) & 1, err)) return false;
+        castdev::tc_fence_after();
+        const uint32_t vo = vs * S::tile + half * 8192, pa = s_col + half * 64;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          castdev::mma_f16_ts(o_col, pa + 8 * s, vd.at(vo + 2048 * s), idesc_pv, ((t - t_lo) | half | s) != 0);
+        castdev::tc_commit(&my_pv_done[half]);
+        if (more) {
+          if (half == 0) {
+            if (!castdev::mbar_wait(&k_full[rk % KS], (rk / KS) & 1, err)) return false;
+            castdev::tc_fence_after();
+          }
+          issue_s(rk, half);
+          castdev::tc_commit(&my_s_full[half]);
+        }
+      }
+      castdev::tc_commit(&v_empty[vs]);
+      if (more) castdev::tc_commit(&k_empty[rk % KS]);
+    }
+  }
+  for (int t = max(t_lo, t_hi); t < n_all; ++t)
+    if (!skip(t)) return false;
+  return true;
+}
+
+// Gives a row the infinities and NaN of the values that it sees and not every
+// row of its item does (columns c0 .. c0 + N - 1); they were taken out of the
+// V tiles.  Far off the usual path: a loop over the item's keys.
+template <typename T, int N>
+__device__ __noinline__ void tiles_give_back(const TilesParams &p, const WindowSpan &span, int b, int hk, int lo, int hi,
+                                             int c0, float (&y)[N]) {
+  if (hi == 0) return;
+  const T *v = static_cast<const T *>(p.v) + b * p.vs[0] + hk * p.vs[1] + c0;
+  for (int n = 0; n < span.n; ++n) {
+    const int key = span.key(n);
+    if (!span.some(key) || !window_sees(key, lo, hi, span.sinks)) continue;
+    for (int c = 0; c < N; ++c) {
+      const float u = (float)v[key * p.vs[2] + c];
+      if (!isfinite(u)) y[c] += u;
+    }
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTilesThreads, 1)
+    window_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_k_sink,
+                        const __grid_constant__ CUtensorMap tm_v_sink, const __grid_constant__ CUtensorMap tm_k_rest,
+                        const __grid_constant__ CUtensorMap tm_v_rest, const __grid_constant__ TilesParams p) {
+  using S = TilesSmem<D>;
+  using X = TilesType<T>;
+  constexpr int KS = S::kStages, VS = S::vStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem =
+      reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t *bar = reinterpret_cast<uint64_t *>(smem + S::bars);
+  uint64_t *q_full = bar;
+  uint64_t *k_full = bar + 1;
+  uint64_t *k_empty = k_full + KS;
+  uint64_t *v_full = k_empty + KS;
+  uint64_t *v_empty = v_full + VS;
+  uint64_t *v_raw = v_empty + VS;  // a V tile has landed and is gone over before v_full
+  uint64_t *s_full = v_raw + VS;
+  uint64_t *p_full = s_full + 4;
+  uint64_t *pv_done = p_full + 4;
+  uint64_t *mma_drain = pv_done + 4;
+  uint64_t *merge_bar = mma_drain + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + S::tmem_slot);
+  volatile uint32_t *bad_flag = tmem_slot + 1;  // an infinity or NaN was taken out of a V tile
+  int *err = reinterpret_cast<int *>(tmem_slot + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // ---- the item, and which part of its key tiles
+  int x = blockIdx.x, part = 0, n_parts = 1;
+  if (x >= p.n_whole) {
+    part = (x - p.n_whole) % p.parts;
+    x = p.n_whole + (x - p.n_whole) / p.parts;
+    n_parts = p.parts;
+  }
+  const int bhg = x / p.pairs;
+  const int pair = p.pairs - 1 - (x - bhg * p.pairs);  // later rows see more keys: first
+  const int b = bhg / p.head_groups, hg = bhg - b * p.head_groups;
+  const int hk = hg / p.groups_per_key;
+  const int t0 = 2 * pair;
+  const int nq = min(2, p.q_tiles - t0);
+  const int row0 = t0 * 128, row_end = min(p.rows, row0 + nq * 128);
+  int len = p.kv_lens ? p.kv_lens[b] : p.lk;
+  if (len < 0 || len > p.lk) {  // a session longer than its keys: nothing past them is read
+    if (threadIdx.x == 0) atomicExch(&g_cast_device_error, (int)CAST_ERR_INVALID_ARGUMENT);
+    len = min(max(len, 0), p.lk);
+  }
+  const WindowSpan span = window_span(p.rule, len, p.Lq, row0 >> p.pack_log2, (row_end - 1) >> p.pack_log2);
+  // places: [0, s_n) sinks, [s_n, s8) nothing, from s8 the keys from span.base on
+  const int s8 = span.s_n > 0 ? p.sinks8 : 0;
+  const int n_places = span.n - span.s_n + s8;
+  const int n_tiles = span.n > 0 ? (n_places + 127) / 128 : 0;
+  const int kt_lo = (int)((long long)part * n_tiles / n_parts);
+  const int n_kv = (int)((long long)(part + 1) * n_tiles / n_parts) - kt_lo;
+  const bool split = nq == 1 && n_kv >= 2;
+  const int n_a = split ? (n_kv + 1) / 2 : n_kv;
+  const int n_b = split ? n_kv - n_a : n_kv;
+  const int n_groups = split ? 2 : nq;
+  const RingMap ring0{split ? 1 : 0, 0, n_a, n_b};
+  // Own key tiles of query tile i of a pair, [first, end) of this CTA's; a
+  // tile in which it sees nothing may be among them.
+  auto own = [&](int i, int &first, int &end) {
+    first = 0;
+    end = i == 0 ? n_a : n_b;
+    if (nq < 2) return;
+    const int r0 = row0 + i * 128, r1 = min(p.rows, r0 + 128);
+    const WindowSpan s = window_span(p.rule, len, p.Lq, r0 >> p.pack_log2, (r1 - 1) >> p.pack_log2);
+    if (s.n == 0) {
+      end = 0;
+      return;
+    }
+    // places [a, z) hold every key it sees
+    const int a = span.sinks > 0 ? 0 : max(0, s8 + s.lo0 - span.base), z = s8 + s.hi1 - span.base;
+    first = min(max(a / 128 - kt_lo, 0), end);
+    end = max(first, min(end, (z + 127) / 128 - kt_lo));
+  };
+
+  if (warp == kProducerWarp && lane == 0) {
+    *err = 0;
+    *bad_flag = 0;
+    for (int i = 0; i < S::n_bars; ++i) castdev::mbar_init(&bar[i], 1);
+    for (int i = 0; i < 4; ++i) castdev::mbar_init(&p_full[i], 4);
+    castdev::mbar_init(merge_bar, 4);
+    for (int i = 0; i < KS; ++i) castdev::mbar_init(&k_empty[i], split ? 1 : nq);
+    for (int i = 0; i < VS; ++i) castdev::mbar_init(&v_empty[i], split ? 1 : nq);
+    castdev::fence_barrier_init();
+    castdev::tma_prefetch_desc(&tm_q);
+    castdev::tma_prefetch_desc(&tm_k);
+    castdev::tma_prefetch_desc(&tm_v);
+    if (n_kv > 0) {
+      castdev::mbar_arrive_expect_tx(q_full, nq * S::tile);
+      for (int i = 0; i < nq; ++i)
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h)
+          tma_load_5d(smem + i * S::tile + h * 16384, &tm_q, q_full, 64 * h, 0, (row0 + i * 128) >> p.pack_log2, hg, b);
+    }
+  }
+  if (warp == kMmaWarp) {
+    castdev::tmem_alloc(tmem_slot, 512);
+    castdev::tmem_relinquish();
+  }
+  __syncthreads();
+  castdev::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // Starts the copies of the tile of 128 places from place n0 on.
+  auto start = [&](uint8_t *dst, uint64_t *full, int n0, const CUtensorMap *whole, const CUtensorMap *sink,
+                   const CUtensorMap *rest, int head, int batch) {
+    if (n0 >= s8 || n0 + 128 <= s8) {
+      const int key = n0 >= s8 ? span.base + n0 - s8 : n0;
+#pragma unroll
+      for (int h = 0; h < D / 64; ++h) castdev::tma_load_4d(dst + h * 16384, whole, full, 64 * h, key, head, batch);
+    } else {
+      const int r = s8 - n0;
+#pragma unroll
+      for (int h = 0; h < D / 64; ++h) {
+        castdev::tma_load_4d(dst + h * 16384, sink, full, 64 * h, n0, head, batch);
+        castdev::tma_load_4d(dst + h * 16384 + r * 128, rest, full, 64 * h, span.base, head, batch);
+      }
+    }
+  };
+
+  if (warp >= 8) {
+    if (warp == kProducerWarp) {
+      if (lane == 0 && n_kv > 0) {
+        int issued = 0;
+        for (int j = 0; j < n_kv; ++j) {
+          const int n0 = (kt_lo + ring0.key_tile(j)) * 128, ks = j % KS;
+          if (j >= KS && !castdev::mbar_wait(&k_empty[ks], ((j / KS) - 1) & 1, err)) break;
+          castdev::mbar_arrive_expect_tx(&k_full[ks], S::tile);
+          start(smem + S::k_off + ks * S::tile, &k_full[ks], n0, &tm_k, &tm_k_sink, &tm_k_rest, hk * p.k_head,
+                b * p.k_batch);
+          issued = j + 1;
+        }
+        castdev::mbar_wait_drain(q_full, 0, err);
+        for (int j = max(0, issued - KS); j < issued; ++j)
+          castdev::mbar_wait_drain(&k_full[j % KS], (j / KS) & 1, err);
+      }
+    } else if (warp == kVProducerWarp) {
+      // whole warp: lane 0 starts the copies, all go over tiles that are not wholly visible
+      uint32_t raw_phase = 0;  // bit per stage
+      // every row sees place n (sinks and the keys of all rows)
+      auto all_see = [&](int n) {
+        return !span.unplaced && (n < min(span.sinks, span.hi0) || (n >= s8 + span.lo1 - span.base && n < s8 + span.hi0 - span.base));
+      };
+      auto any_sees = [&](int n) { return n < n_places && (n < span.s_n || n >= s8); };
+      // (both ends of a run of 128 places: visible ones are one or two intervals)
+      auto ragged = [&](int n0) {
+        if (span.unplaced || n0 + 128 > n_places) return true;
+        const int a = min(span.sinks, span.hi0), l = s8 + span.lo1 - span.base, h = s8 + span.hi0 - span.base;
+        return !(n0 + 128 <= a || (n0 >= l && n0 + 128 <= h) || (a >= l && n0 + 128 <= h));
+      };
+      auto go_over = [&](int j) -> bool {
+        const int n0 = (kt_lo + ring0.key_tile(j)) * 128, vs = j % VS;
+        const bool ok = castdev::mbar_wait(&v_raw[vs], (raw_phase >> vs) & 1, err);
+        if (!__all_sync(0xffffffffu, ok)) return false;
+        raw_phase ^= 1u << vs;
+        uint8_t *tile = smem + S::v_off + vs * S::tile;
+        bool bad = false;
+#pragma unroll 4
+        for (int r = lane >> 3; r < 128; r += 4) {  // eight lanes a row of 128 bytes
+          const int n = n0 + r;
+          if (all_see(n)) continue;
+          const bool some = any_sees(n);
+#pragma unroll
+          for (int h = 0; h < D / 64; ++h) {
+            uint4 *w = reinterpret_cast<uint4 *>(tile + h * 16384 + r * 128) + (lane & 7);
+            if (!some) {
+              *w = make_uint4(0u, 0u, 0u, 0u);
+            } else {
+              uint4 u = *w;
+              const uint32_t b0 = Half2<T>::bad(u.x), b1 = Half2<T>::bad(u.y), b2 = Half2<T>::bad(u.z),
+                             b3 = Half2<T>::bad(u.w);
+              if (b0 | b1 | b2 | b3) {
+                bad = true;
+                *w = make_uint4(u.x & ~b0, u.y & ~b1, u.z & ~b2, u.w & ~b3);
+              }
+            }
+          }
+        }
+        if (bad) *bad_flag = 1;
+        castdev::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) castdev::mbar_arrive(&v_full[vs]);
+        return true;
+      };
+      int issued = 0, looked = 0;  // tiles started; tiles gone over
+      bool ok = true;
+      for (int j = 0; ok && j < n_kv; ++j) {
+        const int n0 = (kt_lo + ring0.key_tile(j)) * 128, vs = j % VS;
+        ok = j < VS || castdev::mbar_wait(&v_empty[vs], ((j / VS) - 1) & 1, err);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        uint64_t *full = ragged(n0) ? &v_raw[vs] : &v_full[vs];
+        if (lane == 0) {
+          castdev::mbar_arrive_expect_tx(full, S::tile);
+          start(smem + S::v_off + vs * S::tile, full, n0, &tm_v, &tm_v_sink, &tm_v_rest, hk * p.v_head, b * p.v_batch);
+        }
+        issued = j + 1;
+        if (j > 0) {
+          if (ragged((kt_lo + ring0.key_tile(j - 1)) * 128)) ok = go_over(j - 1);
+          looked = j;
+        }
+      }
+      if (ok && issued > 0 && ragged((kt_lo + ring0.key_tile(issued - 1)) * 128)) ok = go_over(issued - 1);
+      if (ok) looked = issued;
+      // every copy lands before the CTA leaves: those gone over have; the
+      // others' own barriers say so
+      if (lane == 0)
+        for (int j = max(0, issued - VS); j < issued; ++j) {
+          const int vs = j % VS;
+          if (!ragged((kt_lo + ring0.key_tile(j)) * 128))
+            castdev::mbar_wait_drain(&v_full[vs], (j / VS) & 1, err);
+          else if (j >= looked)
+            castdev::mbar_wait_drain(&v_raw[vs], (raw_phase >> vs) & 1, err);
+        }
+    } else {
+      const int i = warp == kMmaWarp ? 0 : 1;
+      if (lane == 0 && n_kv > 0 && i < n_groups) {
+        const RingMap ring{split ? 1 : 0, i, n_a, n_b};
+        int first, end;
+        own(i, first, end);
+        tiles_issuer<T, D>(i, ring, tmem, castdev::smem_u32(smem), i == 0 ? n_a : n_b, first, end, q_full, k_full,
+                           k_empty, v_full, v_empty, s_full, p_full, pv_done, err);
+        castdev::tc_commit(&mma_drain[i]);
+        castdev::mbar_wait_drain(&mma_drain[i], 0, err);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int ti = warp >> 2;
+    const int lrow = (warp & 3) * 32 + lane;
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t o_addr = tmem + lane_off + ti * 128;
+    const uint32_t s_addr = tmem + lane_off + 256 + ti * 128;
+    const bool active = ti < n_groups;
+    int first = 0, end = 0;
+    if (active) own(ti, first, end);
+    const int my_steps = 2 * (end - first);
+    const int start_tile = kt_lo + ((split && ti == 1) ? n_a : 0) + first;
+    const int row = row0 + (split ? 0 : ti) * 128 + lrow;
+    const bool row_valid = active && row < p.rows;
+    const int token = row >> p.pack_log2, head = hg * p.pack + (row & (p.pack - 1));
+    // this row's places: [0, near) and [from, to)
+    int lo = 0, hi = 0, near = 0, from = 0, to = 0;
+    const int pos = len - p.Lq + token;
+    if (row_valid && pos >= 0) {
+      window_bounds(p.rule, len, pos, lo, hi);
+      near = min(span.sinks, hi);
+      from = s8 + lo - span.base;
+      to = s8 + hi - span.base;
+    }
+    // (a row that will see nothing must not keep its warp on the slow path)
+    float m_run = hi > 0 ? -INFINITY : 0.0f, l_run = 0.0f;
+    bool ok = true;
+    const float c2 = p.scale_log2;
+    for (int h = 0; active && h < my_steps; ++h) {
+      const int half = h & 1;
+      const int n0 = start_tile * 128 + h * 64;
+      const bool all = n0 + 64 <= near || (n0 >= from && n0 + 64 <= to) || !row_valid;
+      const bool none = (n0 >= near && (n0 + 64 <= from || n0 >= to)) || !row_valid;
+      const bool full_step = __all_sync(0xffffffffu, all);
+      const bool empty_step = __all_sync(0xffffffffu, none);
+      uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+      if (!full_step) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+          seen[w] = interval_mask(0, near, n0 + 32 * w) | interval_mask(from, to, n0 + 32 * w);
+      }
+      ok = __all_sync(0xffffffffu, castdev::mbar_wait(&s_full[ti * 2 + half], (h >> 1) & 1, err));
+      if (!ok) break;
+      castdev::tc_fence_after();
+      const uint32_t sb = s_addr + 64 * half;
+      uint32_t v[64];
+      float sum = 0.0f;
+      if (empty_step) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] = 0u;
+      } else {
+        castdev::tmem_ld32(sb, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+        castdev::tmem_ld32(sb + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+        castdev::tmem_wait_ld();
+        bool slow = __any_sync(0xffffffffu, m_run == -INFINITY);
+        if (!slow) {
+          sum = full_step ? tiles_probs<T, false>(v, seen, c2, m_run - X::kShift)
+                          : tiles_probs<T, true>(v, seen, c2, m_run - X::kShift);
+          slow = __any_sync(0xffffffffu, !(sum <= X::kSumLimit));
+          if (slow) {
+            castdev::tmem_ld32(sb, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+            castdev::tmem_ld32(sb + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+            castdev::tmem_wait_ld();
+          }
+        }
+        if (__builtin_expect(slow, 0)) {
+          const float m_step = full_step ? row_max<false, false>(v, seen, c2) : row_max<false, true>(v, seen, c2);
+          float o_scale = 1.0f;
+          if (m_step > m_run + X::kSlack || m_run == -INFINITY) {
+            const float m_new = fmaxf(m_run, m_step);
+            o_scale = (m_run == -INFINITY) ? (m_new == -INFINITY ? 1.0f : 0.0f) : fast_exp2(m_run - m_new);
+            l_run *= o_scale;
+            m_run = m_new;
+          }
+          if (h > 0 && __any_sync(0xffffffffu, o_scale != 1.0f)) {
+            const int hp = h - 1;
+            ok = __all_sync(0xffffffffu, castdev::mbar_wait(&pv_done[ti * 2 + (hp & 1)], (hp >> 1) & 1, err));
+            if (!ok) break;
+            castdev::tc_fence_after();
+#pragma unroll 1
+            for (int cc = 0; cc < D / 32; ++cc) {
+              uint32_t o[32];
+              castdev::tmem_ld32(o_addr + 32 * cc, o);
+              castdev::tmem_wait_ld();
+#pragma unroll
+              for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * o_scale);
+              castdev::tmem_st32(o_addr + 32 * cc, o);
+            }
+          }
+          const float base = (m_run == -INFINITY) ? 0.0f : m_run - X::kShift;
+          sum = full_step ? tiles_probs<T, false>(v, seen, c2, base) : tiles_probs<T, true>(v, seen, c2, base);
+        }
+      }
+      castdev::tmem_st32(sb, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+      l_run += sum;
+      castdev::tmem_wait_st();
+      castdev::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) castdev::mbar_arrive(&p_full[ti * 2 + half]);
+    }
+    if (hi == 0) {  // a row that sees nothing is nothing (and its maximum is none)
+      m_run = -INFINITY;
+      l_run = 0.0f;
+    }
+    // ------------------------------------------------------------ epilogue
+    if (active && ok && my_steps > 0) {
+      const int hl = my_steps - 1;
+      ok = __all_sync(0xffffffffu, castdev::mbar_wait(&pv_done[ti * 2 + (hl & 1)], (hl >> 1) & 1, err));
+      castdev::tc_fence_after();
+    }
+    if (split && ti == 1) {
+      if (ok) {
+        castdev::tmem_st1(s_addr, __float_as_uint(m_run));
+        castdev::tmem_st1(s_addr + 1, __float_as_uint(l_run));
+        castdev::tmem_wait_st();
+      }
+      castdev::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) castdev::mbar_arrive(merge_bar);
+    } else if (active) {
+      float scale0 = 1.0f, scale1 = 0.0f;
+      const uint32_t o1_addr = tmem + lane_off + 128;
+      if (split && ok) {
+        ok = __all_sync(0xffffffffu, castdev::mbar_wait(merge_bar, 0, err));
+        castdev::tc_fence_after();
+        const uint32_t s1_addr = tmem + lane_off + 256 + 128;
+        const float m1 = __uint_as_float(castdev::tmem_ld1(s1_addr));
+        const float l1 = __uint_as_float(castdev::tmem_ld1(s1_addr + 1));
+        castdev::tmem_wait_ld();
+        const float m = fmaxf(m_run, m1);
+        scale0 = m_run == -INFINITY ? 0.0f : fast_exp2(m_run - m);
+        scale1 = m1 == -INFINITY ? 0.0f : fast_exp2(m1 - m);
+        l_run = l_run * scale0 + l1 * scale1;
+        m_run = m;
+      }
+      auto load_o = [&](int cc, uint32_t (&o)[32]) {
+        if (my_steps > 0) {
+          castdev::tmem_ld32(o_addr + 32 * cc, o);
+          if (split) {
+            uint32_t o1[32];
+            castdev::tmem_ld32(o1_addr + 32 * cc, o1);
+            castdev::tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              o[c] = __float_as_uint(fmaf(__uint_as_float(o1[c]), scale1, __uint_as_float(o[c]) * scale0));
+          } else {
+            castdev::tmem_wait_ld();
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) o[c] = 0u;
+        }
+      };
+      const bool bad = *bad_flag != 0;
+      if (n_parts == 1) {
+        if (ok) {
+          const float inv = l_run != 0.0f ? 1.0f / l_run : 0.0f;  // (a NaN sum stays one)
+          T *dst = static_cast<T *>(p.out) + b * p.os[0] + head * p.os[1] + token * p.os[2];
+#pragma unroll 1
+          for (int cc = 0; cc < D / 32; ++cc) {
+            uint32_t o[32];
+            __syncwarp();
+            load_o(cc, o);
+            float y[32];
+#pragma unroll
+            for (int c = 0; c < 32; ++c) y[c] = hi > 0 ? __uint_as_float(o[c]) * inv : 0.0f;
+            if (row_valid) {
+              if (__builtin_expect(bad, 0)) {
+                float z[32];
+                for (int c = 0; c < 32; ++c) z[c] = y[c];
+                tiles_give_back<T>(p, span, b, hk, lo, hi, 32 * cc, z);
+                for (int c = 0; c < 32; ++c) y[c] = z[c];
+              }
+              uint4 w[4];
+              uint32_t *wp = reinterpret_cast<uint32_t *>(w);
+#pragma unroll
+              for (int c = 0; c < 16; ++c) wp[c] = X::pack(y[2 * c], y[2 * c + 1]);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) reinterpret_cast<uint4 *>(dst + 32 * cc)[c] = w[c];
+            }
+          }
+        }
+      } else if (ok) {
+        // this part's O, maximum and sum: [tile][column][row], then [tile][m, l, flag][row]
+        float *slot = p.part + (long long)(blockIdx.x - p.n_whole) * tiles_part_floats<D>();
+        float *tail = slot + 2 * 128 * D + ti * (128 * kTilesPartCols) + lrow;
+        if (row_valid) {
+          tail[0] = hi > 0 ? m_run : -INFINITY;
+          tail[128] = l_run;
+          tail[256] = __int_as_float(bad ? 1 : 0);
+        }
+        if (my_steps > 0) {
+#pragma unroll 1
+          for (int cc = 0; cc < D / 32; ++cc) {
+            uint32_t o[32];
+            __syncwarp();
+            load_o(cc, o);
+            float *dst = slot + ti * (128 * D) + 32 * cc * 128 + lrow;
+            if (row_valid) {
+#pragma unroll
+              for (int c = 0; c < 32; ++c) dst[c * 128] = __uint_as_float(o[c]);
+            }
+          }
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    castdev::tc_fence_after();
+    castdev::tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the parts of the cut items: one CTA for eight columns of a query
+// tile; thread (row, g) takes every kJoinGroups-th part.
+constexpr int kJoinGroups = 4, kJoinCols = 8;
+template <typename T, int D>
+__global__ void __launch_bounds__(128 * kJoinGroups) window_tiles_join_kernel(const __grid_constant__ TilesParams p) {
+  __shared__ float acc_s[kJoinGroups][kJoinCols + 1][128];
+  constexpr int cuts = D / kJoinCols;
+  const int cut = blockIdx.x % cuts, ti = blockIdx.x / cuts % 2, item = blockIdx.x / (2 * cuts);
+  const int row_in = threadIdx.x & 127, g = threadIdx.x >> 7;
+  const int x = p.n_whole + item;
+  const int bhg = x / p.pairs, pair = p.pairs - 1 - (x - bhg * p.pairs);
+  const int b = bhg / p.head_groups, hg = bhg - b * p.head_groups;
+  const int t0 = 2 * pair, row0 = t0 * 128, row_end = min(p.rows, row0 + min(2, p.q_tiles - t0) * 128);
+  const int row = row0 + ti * 128 + row_in;
+  if (row0 + ti * 128 >= p.rows) return;  // (whole CTAs)
+  const bool on = row < p.rows;
+  const float *base = p.part + (long long)item * p.parts * tiles_part_floats<D>();
+  const float *tails = base + 2 * 128 * D + ti * (128 * kTilesPartCols) + row_in;
+  float m = -INFINITY;
+  bool bad = false;
+  if (on)
+    for (int j = 0; j < p.parts; ++j) m = fmaxf(m, tails[j * tiles_part_floats<D>()]);
+  float l = 0.0f, a[kJoinCols];
+#pragma unroll
+  for (int c = 0; c < kJoinCols; ++c) a[c] = 0.0f;
+  if (on) {
+#pragma unroll 4
+    for (int j = g; j < p.parts; j += kJoinGroups) {
+      const float *tail = tails + j * tiles_part_floats<D>();
+      const float mj = tail[0];
+      bad = bad || __float_as_int(tail[256]) != 0;
+      if (mj == -INFINITY) continue;  // nothing seen: its O may not be written
+      const float f = fast_exp2(mj - m);
+      const float *o = base + j * tiles_part_floats<D>() + ti * (128 * D) + cut * kJoinCols * 128 + row_in;
+      l = fmaf(tail[128], f, l);
+#pragma unroll
+      for (int c = 0; c < kJoinCols; ++c) a[c] = fmaf(o[c * 128], f, a[c]);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kJoinCols; ++c) acc_s[g][c][row_in] = a[c];
+  acc_s[g][kJoinCols][row_in] = l;
+  const bool any_bad = __syncthreads_or(bad);
+  if (g != 0 || !on) return;
+  float y[kJoinCols];
+  l = 0.0f;
+#pragma unroll
+  for (int c = 0; c < kJoinCols; ++c) y[c] = 0.0f;
+#pragma unroll
+  for (int j = 0; j < kJoinGroups; ++j) {
+    l += acc_s[j][kJoinCols][row_in];
+#pragma unroll
+    for (int c = 0; c < kJoinCols; ++c) y[c] += acc_s[j][c][row_in];
+  }
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+  for (int c = 0; c < kJoinCols; ++c) y[c] *= inv;
+  const int token = row >> p.pack_log2, head = hg * p.pack + (row & (p.pack - 1));
+  if (any_bad) {
+    const int len = min(max(p.kv_lens ? p.kv_lens[b] : p.lk, 0), p.lk);
+    const WindowSpan span = window_span(p.rule, len, p.Lq, row0 >> p.pack_log2, (row_end - 1) >> p.pack_log2);
+    int lo = 0, hi = 0;
+    const int pos = len - p.Lq + token;
+    if (pos >= 0) window_bounds(p.rule, len, pos, lo, hi);
+    float z[kJoinCols];
+    for (int c = 0; c < kJoinCols; ++c) z[c] = y[c];
+    tiles_give_back<T>(p, span, b, hg / p.groups_per_key, lo, hi, cut * kJoinCols, z);
+    for (int c = 0; c < kJoinCols; ++c) y[c] = z[c];
+  }
+  T *dst = static_cast<T *>(p.out) + b * p.os[0] + head * p.os[1] + token * p.os[2] + cut * kJoinCols;
+  *reinterpret_cast<uint4 *>(dst) =
+      make_uint4(TilesType<T>::pack(y[0], y[1]), TilesType<T>::pack(y[2], y[3]), TilesType<T>::pack(y[4], y[5]),
+                 TilesType<T>::pack(y[6], y[7]));
+}
+
+}  // namespace castk
