@@ -21,6 +21,7 @@
 #include "rotary.cuh"
 #include "window.cuh"
 #include "window_tiles.cuh"
+#include "window_one.cuh"
 
 namespace cast {
 
@@ -1457,7 +1458,9 @@ static int rows_params(castk::RowsParams &p, const void *q, const void *k, const
   return CAST_OK;
 }
 
+static bool use_one() { static const char *e = getenv("CAST_WINDOW_ONE"); return !e || e[0] != '0'; }
 struct TilesPlan {
+  bool one = false;
   int pack = 1, pack_log2 = 0, head_groups = 1, q_tiles = 1, pairs = 1;
   int n_items = 0, n_whole = 0, parts = 1;
   size_t ws_bytes = 0;
@@ -1477,10 +1480,13 @@ static TilesPlan tiles_plan(int B, int Hq, int Hk, int Lq, int Lk, long long win
   const long long rows = (long long)t.pack * Lq;
   t.q_tiles = (int)((rows + 127) / 128);
   t.pairs = (t.q_tiles + 1) / 2;
-  t.n_items = B * t.head_groups * t.pairs;
+  t.one = use_one();
+  const int slots = t.one ? 2 * n_sms : n_sms;
+  n_sms = slots;
+  t.n_items = B * t.head_groups * (t.one ? t.q_tiles : t.pairs);
   const double tokens = std::min<double>(Lq, 256.0 / t.pack);
   const double keys = std::min<double>(Lk, (double)(window + sinks) * frame + tokens + (frame > 1 ? frame : 0));
-  const double c = std::max(1.0, keys / 128) * (t.q_tiles == 1 ? 0.5 : 1.0);
+  const double c = std::max(1.0, keys / 128) * (t.q_tiles == 1 && !t.one ? 0.5 : 1.0);
   const int waves = t.n_items / n_sms, rem = t.n_items % n_sms;
   t.n_whole = t.n_items;
   double best = (waves + (rem ? 1 : 0)) * (c + 4.0);
@@ -1499,7 +1505,8 @@ static TilesPlan tiles_plan(int B, int Hq, int Hk, int Lq, int Lk, long long win
   }
   if (t.parts > 1)
     t.ws_bytes = (size_t)(t.n_items - t.n_whole) * t.parts *
-                 (D == 128 ? castk::tiles_part_floats<128>() : castk::tiles_part_floats<64>()) * sizeof(float);
+                 (t.one ? (D == 128 ? castk::one_part_floats<128>() : castk::one_part_floats<64>())
+                        : (D == 128 ? castk::tiles_part_floats<128>() : castk::tiles_part_floats<64>())) * sizeof(float);
   return t;
 }
 
@@ -1572,13 +1579,14 @@ static int launch_tiles(const castk::RowsParams &r, const TilesPlan &plan, int d
     const uint32_t box[5] = {64, (uint32_t)plan.pack, (uint32_t)(128 / plan.pack), 1, 1};
     if ((st = make_map_rows(&tm_q, r.q, dtype, 5, dims, str, box))) return st;
   }
-  const uint32_t tail = p.sinks8 % 128;
+  const uint32_t kt = plan.one ? castk::OneSmem<D>::keys : 128;
+  const uint32_t tail = p.sinks8 % kt;
   for (int i = 0; i < 3; ++i) {  // all 128 rows of a tile, the sinks' last rows, the rows beside them
     if (i > 0 && tail == 0) {
       tm_k[i] = tm_k[0], tm_v[i] = tm_v[0];  // never read
       continue;
     }
-    const uint32_t box[4] = {64, i == 0 ? 128u : (i == 1 ? tail : 128u - tail), 1, 1};
+    const uint32_t box[4] = {64, i == 0 ? kt : (i == 1 ? tail : kt - tail), 1, 1};
     const uint64_t kd[4] = {(uint64_t)D, (uint64_t)r.lk, (uint64_t)(p.k_head ? r.Hk : 1), (uint64_t)(p.k_batch ? r.B : 1)};
     const long long ks[3] = {r.ks[2], r.ks[1], r.ks[0]};
     if ((st = make_map_rows(&tm_k[i], r.k, dtype, 4, kd, ks, box))) return st;
@@ -1586,13 +1594,38 @@ static int launch_tiles(const castk::RowsParams &r, const TilesPlan &plan, int d
     const long long vs[3] = {r.vs[2], r.vs[1], r.vs[0]};
     if ((st = make_map_rows(&tm_v[i], r.v, dtype, 4, vd, vs, box))) return st;
   }
+  const int cut = plan.n_items - plan.n_whole;
+  if (plan.one) {
+    auto kernel = castk::window_one_kernel<T, D>;
+    constexpr int smem = castk::OneSmem<D>::alloc;
+    static std::once_flag once;
+    static cudaError_t err = cudaSuccess;
+    static int regs = 0;
+    std::call_once(once, [&] {
+      err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      cudaFuncAttributes fa;
+      if (err == cudaSuccess) err = cudaFuncGetAttributes(&fa, kernel);
+      if (err == cudaSuccess) regs = fa.numRegs;
+    });
+    CAST_CUDA_TRY(err);
+    // the softmax warps' larger share comes out of what the block was launched with
+    if (regs * castk::kOneThreads < 128 * (castk::kOneRegsSoft + castk::kOneRegsRest))
+      return fail(CAST_ERR_UNSUPPORTED, "window kernel built with %d registers a thread", regs);
+    kernel<<<plan.n_whole + cut * plan.parts, castk::kOneThreads, smem, s>>>(tm_q, tm_k[0], tm_v[0], tm_k[1], tm_v[1],
+                                                                            tm_k[2], tm_v[2], p);
+    CAST_CUDA_TRY(cudaGetLastError());
+    if (cut > 0) {
+      castk::window_one_join_kernel<T, D><<<cut * (D / castk::kJoinCols), 128 * castk::kJoinGroups, 0, s>>>(p);
+      CAST_CUDA_TRY(cudaGetLastError());
+    }
+    return CAST_OK;
+  }
   auto kernel = castk::window_tiles_kernel<T, D>;
   constexpr int smem = castk::TilesSmem<D>::alloc;
   static std::once_flag once;
   static cudaError_t err = cudaSuccess;
   std::call_once(once, [&] { err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
   CAST_CUDA_TRY(err);
-  const int cut = plan.n_items - plan.n_whole;
   kernel<<<plan.n_whole + cut * plan.parts, castk::kTilesThreads, smem, s>>>(tm_q, tm_k[0], tm_v[0], tm_k[1], tm_v[1],
                                                                             tm_k[2], tm_v[2], p);
   CAST_CUDA_TRY(cudaGetLastError());

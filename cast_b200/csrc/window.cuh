@@ -91,7 +91,12 @@ struct Half2<__nv_bfloat16> {
   static __device__ __forceinline__ float2 unpack(uint32_t u) {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
   }
-  static __device__ __forceinline__ __nv_bfloat16 round(float x) { return __float2bfloat16_rn(x); }
+  // u * 0 + acc in both halves
+  static __device__ __forceinline__ uint32_t fma0(uint32_t u, uint32_t acc) {
+    uint32_t r;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(u), "r"(0u), "r"(acc));
+    return r;
+  }
   // whether either half is an infinity or NaN
   static __device__ __forceinline__ uint32_t bad(uint32_t u) {
     return ((u & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) | ((u & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u);
@@ -115,7 +120,11 @@ struct Half2<__half> {
   static __device__ __forceinline__ float2 unpack(uint32_t u) {
     return __half22float2(*reinterpret_cast<const __half2 *>(&u));
   }
-  static __device__ __forceinline__ __half round(float x) { return __float2half_rn(x); }
+  static __device__ __forceinline__ uint32_t fma0(uint32_t u, uint32_t acc) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(u), "r"(0u), "r"(acc));
+    return r;
+  }
   static __device__ __forceinline__ uint32_t bad(uint32_t u) {
     return ((u & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u) | ((u & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u);
   }
