@@ -21,7 +21,6 @@
 #include "rotary.cuh"
 #include "window.cuh"
 #include "window_tiles.cuh"
-#include "window_one.cuh"
 
 namespace cast {
 
@@ -1458,43 +1457,37 @@ static int rows_params(castk::RowsParams &p, const void *q, const void *k, const
   return CAST_OK;
 }
 
-static bool use_one() { static const char *e = getenv("CAST_WINDOW_ONE"); return !e || e[0] != '0'; }
 struct TilesPlan {
-  bool one = false;
-  int pack = 1, pack_log2 = 0, head_groups = 1, q_tiles = 1, pairs = 1;
+  int pack = 1, pack_log2 = 0, head_groups = 1, q_tiles = 1;
   int n_items = 0, n_whole = 0, parts = 1;
   size_t ws_bytes = 0;
 };
 
-// How the many-row kernel cuts a call: an item is a pair of query tiles of
-// one head group, one CTA an SM.  The items of the last, incomplete wave (or
-// of the last two) are cut along their keys into equal parts where that ends
-// sooner, counted in steps of 128 keys: an item costs its keys and about 4
-// steps to start and end, a part 2.5 more to leave and join its result.
+// How the many-row kernel cuts a call: an item is a query tile of one head
+// group, and two CTAs run on an SM.  The items of the last, incomplete wave
+// (or of the last two) are cut along their keys into equal parts where that
+// ends sooner, counted in steps of 128 keys: an item costs its keys and about
+// 4 steps to start and end, a part 2.5 more to leave and join its result.
 static TilesPlan tiles_plan(int B, int Hq, int Hk, int Lq, int Lk, long long window, long long sinks, int frame,
                             int D, int n_sms) {
   TilesPlan t;
-  const int group = Hq / Hk;
+  const int group = Hq / Hk, slots = 2 * n_sms;
   while (t.pack < 128 && group % (2 * t.pack) == 0) t.pack *= 2, ++t.pack_log2;
   t.head_groups = Hq / t.pack;
   const long long rows = (long long)t.pack * Lq;
   t.q_tiles = (int)((rows + 127) / 128);
-  t.pairs = (t.q_tiles + 1) / 2;
-  t.one = use_one();
-  const int slots = t.one ? 2 * n_sms : n_sms;
-  n_sms = slots;
-  t.n_items = B * t.head_groups * (t.one ? t.q_tiles : t.pairs);
-  const double tokens = std::min<double>(Lq, 256.0 / t.pack);
+  t.n_items = B * t.head_groups * t.q_tiles;
+  const double tokens = std::min<double>(Lq, 128.0 / t.pack);
   const double keys = std::min<double>(Lk, (double)(window + sinks) * frame + tokens + (frame > 1 ? frame : 0));
-  const double c = std::max(1.0, keys / 128) * (t.q_tiles == 1 && !t.one ? 0.5 : 1.0);
-  const int waves = t.n_items / n_sms, rem = t.n_items % n_sms;
+  const double c = std::max(1.0, keys / 128);
+  const int waves = t.n_items / slots, rem = t.n_items % slots;
   t.n_whole = t.n_items;
   double best = (waves + (rem ? 1 : 0)) * (c + 4.0);
   for (int q = 0; q <= 1 && q <= waves; ++q) {
-    const int cut = rem + q * n_sms;
+    const int cut = rem + q * slots;
     if (cut == 0) continue;
     for (int parts = 2; parts <= 128 && c / parts >= 2.0; ++parts) {
-      const double rounds = std::ceil((double)cut * parts / n_sms);
+      const double rounds = std::ceil((double)cut * parts / slots);
       const double cost = (waves - q) * (c + 4.0) + rounds * (c / parts + 6.5) + 0.05 * parts;
       if (cost < 0.97 * best) {
         best = cost;
@@ -1505,8 +1498,7 @@ static TilesPlan tiles_plan(int B, int Hq, int Hk, int Lq, int Lk, long long win
   }
   if (t.parts > 1)
     t.ws_bytes = (size_t)(t.n_items - t.n_whole) * t.parts *
-                 (t.one ? (D == 128 ? castk::one_part_floats<128>() : castk::one_part_floats<64>())
-                        : (D == 128 ? castk::tiles_part_floats<128>() : castk::tiles_part_floats<64>())) * sizeof(float);
+                 (D == 128 ? castk::tiles_part_floats<128>() : castk::tiles_part_floats<64>()) * sizeof(float);
   return t;
 }
 
@@ -1556,13 +1548,12 @@ static int launch_tiles(const castk::RowsParams &r, const TilesPlan &plan, int d
   p.kv_lens = r.kv_lens;
   p.part = part;
   p.rule = r.rule;
-  p.B = r.B, p.Hk = r.Hk, p.Lq = r.Lq, p.lk = r.lk;
+  p.Lq = r.Lq, p.lk = r.lk;
   p.pack = plan.pack, p.pack_log2 = plan.pack_log2;
-  p.heads = r.Hq;
   p.head_groups = plan.head_groups;
   p.groups_per_key = plan.head_groups / r.Hk;
   p.rows = plan.pack * r.Lq;
-  p.q_tiles = plan.q_tiles, p.pairs = plan.pairs;
+  p.q_tiles = plan.q_tiles;
   p.n_whole = plan.n_whole, p.parts = plan.parts;
   p.scale_log2 = r.scale_log2;
   const long long sink_keys = std::min<long long>(r.rule.sinks * r.rule.frame, r.lk);
@@ -1579,9 +1570,9 @@ static int launch_tiles(const castk::RowsParams &r, const TilesPlan &plan, int d
     const uint32_t box[5] = {64, (uint32_t)plan.pack, (uint32_t)(128 / plan.pack), 1, 1};
     if ((st = make_map_rows(&tm_q, r.q, dtype, 5, dims, str, box))) return st;
   }
-  const uint32_t kt = plan.one ? castk::OneSmem<D>::keys : 128;
+  const uint32_t kt = castk::TilesSmem<D>::keys;
   const uint32_t tail = p.sinks8 % kt;
-  for (int i = 0; i < 3; ++i) {  // all 128 rows of a tile, the sinks' last rows, the rows beside them
+  for (int i = 0; i < 3; ++i) {  // all rows of a key tile, the sinks' last rows, the rows beside them
     if (i > 0 && tail == 0) {
       tm_k[i] = tm_k[0], tm_v[i] = tm_v[0];  // never read
       continue;
@@ -1594,43 +1585,27 @@ static int launch_tiles(const castk::RowsParams &r, const TilesPlan &plan, int d
     const long long vs[3] = {r.vs[2], r.vs[1], r.vs[0]};
     if ((st = make_map_rows(&tm_v[i], r.v, dtype, 4, vd, vs, box))) return st;
   }
-  const int cut = plan.n_items - plan.n_whole;
-  if (plan.one) {
-    auto kernel = castk::window_one_kernel<T, D>;
-    constexpr int smem = castk::OneSmem<D>::alloc;
-    static std::once_flag once;
-    static cudaError_t err = cudaSuccess;
-    static int regs = 0;
-    std::call_once(once, [&] {
-      err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-      cudaFuncAttributes fa;
-      if (err == cudaSuccess) err = cudaFuncGetAttributes(&fa, kernel);
-      if (err == cudaSuccess) regs = fa.numRegs;
-    });
-    CAST_CUDA_TRY(err);
-    // the softmax warps' larger share comes out of what the block was launched with
-    if (regs * castk::kOneThreads < 128 * (castk::kOneRegsSoft + castk::kOneRegsRest))
-      return fail(CAST_ERR_UNSUPPORTED, "window kernel built with %d registers a thread", regs);
-    kernel<<<plan.n_whole + cut * plan.parts, castk::kOneThreads, smem, s>>>(tm_q, tm_k[0], tm_v[0], tm_k[1], tm_v[1],
-                                                                            tm_k[2], tm_v[2], p);
-    CAST_CUDA_TRY(cudaGetLastError());
-    if (cut > 0) {
-      castk::window_one_join_kernel<T, D><<<cut * (D / castk::kJoinCols), 128 * castk::kJoinGroups, 0, s>>>(p);
-      CAST_CUDA_TRY(cudaGetLastError());
-    }
-    return CAST_OK;
-  }
   auto kernel = castk::window_tiles_kernel<T, D>;
   constexpr int smem = castk::TilesSmem<D>::alloc;
   static std::once_flag once;
   static cudaError_t err = cudaSuccess;
-  std::call_once(once, [&] { err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+  static int regs = 0;
+  std::call_once(once, [&] {
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaFuncAttributes fa;
+    if (err == cudaSuccess) err = cudaFuncGetAttributes(&fa, kernel);
+    if (err == cudaSuccess) regs = fa.numRegs;
+  });
   CAST_CUDA_TRY(err);
+  // the softmax warps' larger share comes out of what the block was launched with
+  if (regs * castk::kTilesThreads < 128 * (castk::kTilesRegsSoft + castk::kTilesRegsRest))
+    return fail(CAST_ERR_UNSUPPORTED, "window kernel built with %d registers a thread", regs);
+  const int cut = plan.n_items - plan.n_whole;
   kernel<<<plan.n_whole + cut * plan.parts, castk::kTilesThreads, smem, s>>>(tm_q, tm_k[0], tm_v[0], tm_k[1], tm_v[1],
                                                                             tm_k[2], tm_v[2], p);
   CAST_CUDA_TRY(cudaGetLastError());
   if (cut > 0) {
-    castk::window_tiles_join_kernel<T, D><<<cut * 2 * (D / castk::kJoinCols), 128 * castk::kJoinGroups, 0, s>>>(p);
+    castk::window_tiles_join_kernel<T, D><<<cut * (D / castk::kJoinCols), 128 * castk::kJoinGroups, 0, s>>>(p);
     CAST_CUDA_TRY(cudaGetLastError());
   }
   return CAST_OK;

@@ -2,49 +2,66 @@
 // accumulators over the keys that the rows of a tile see.
 //
 // The mathematics and the list of keys are those of window.cuh.  One CTA
-// computes one or two 128-row query tiles: the `pack` query heads that share
-// a key head lie side by side in the rows (row = token * pack + head), so a
-// pair of tiles covers 256 / pack tokens and their windows differ by little.
-// Keys go by in tiles of 128 places of the list (8-row-aligned, so that the
-// sinks' last rows and the window's first ones share a tile: two TMA boxes).
-// Warp roles, TMEM columns, the 64-key softmax steps with a lazily moved
-// maximum and the two issuers are those of attention.cuh:
-//   warps 0-3, 4-7  softmax and epilogue of query tile 0, 1
-//   warp 8          TMA of Q and the K ring; warp 10: of the V ring
-//   warps 9, 11     one MMA-issuing thread each, for tile 0, 1
-// A single query tile is shared: each issuer and softmax warpgroup takes half
-// of its key tiles, and warpgroup 0 joins the halves.
+// computes one 128-row query tile, and two CTAs share an SM: the start and end
+// of one overlap the steps of the other, which a short window has few of.  The
+// `pack` query heads that share a key head lie side by side in the rows (row =
+// token * pack + head), so a tile covers 128 / pack tokens and their windows
+// differ by little.  Keys go by in tiles of 64 places of the list (8-row
+// aligned, so that the sinks' last rows and the window's first ones share a
+// tile: two TMA boxes).  Step h is one key tile:
+//   S(h) = Q K_h^T       tcgen05, f32 in one of two 64-column TMEM buffers
+//   P(h) = 2^(S c - m)   one softmax thread a row, written over S(h) in pairs
+//   O   += P(h) V_h      tcgen05, A = P from TMEM
+// with the lazily moved maximum and the single pass of attention.cuh.
+//   warps 0-3  softmax and epilogue (TMEM lanes 0..127)
+//   warp 4     TMA of Q and the K ring      warp 5  MMA issuer (one thread)
+//   warp 6     TMA of the V ring            warp 7  idle
 //
-// Masks cost only where they are: a warp whose 32 rows all see a step's 64
-// keys runs the unmasked step, one that sees none of them writes zeros without
-// an exponential, and key tiles that lie outside one query tile's own span
-// are skipped by its issuer.  A V row meets the zero weights of rows that do
-// not see it, and 0 * inf is NaN, so warp 10 goes over the V tiles that are
-// not wholly visible before they are used: rows that nobody sees become zeros;
-// in rows that only some see, infinities and NaN become zeros and are given
-// back to the rows that see them when these are written.
+// Masks cost only where they are: a warp whose 32 rows all see a step's keys
+// runs the unmasked step, and one that sees none of them writes zeros without
+// an exponential.  A V row meets the zero weights of rows that do not see it,
+// and 0 * inf is NaN, so warp 6 goes over the V tiles that are not wholly
+// visible before they are used: rows that nobody sees become zeros; in rows
+// that only some see, infinities and NaN become zeros and are given back to
+// the rows that see them when these are written.
 #pragma once
 
 #include "window.cuh"
 
 namespace castk {
 
-constexpr int kTilesThreads = 384;
-constexpr int kTilesPartCols = 4;  // m, l, flag of a part's rows beside its O
+constexpr int kTilesThreads = 256;
+// Registers of a thread of the softmax warps and of the others:
+// 128 (200 + 56) = 256 * 128, the block's share of the SM at launch.
+constexpr int kTilesRegsSoft = 200, kTilesRegsRest = 56;
+constexpr int kTilesPartCols = 4;  // m, l, flag (and nothing) of a part's rows beside its O
 
 template <int D>
 struct TilesSmem {
-  static constexpr int tile = 128 * D * 2;  // one Q, K or V tile
-  static constexpr int kStages = D == 128 ? 2 : 4;
-  static constexpr int vStages = D == 128 ? 3 : 4;
-  static constexpr int k_off = 2 * tile;
-  static constexpr int v_off = k_off + kStages * tile;
-  static constexpr int bars = v_off + vStages * tile;
-  // q_full, k_full/empty, v_full/empty/raw, s_full[4], p_full[4], pv_done[4], drain[2], merge
-  static constexpr int n_bars = 1 + 2 * kStages + 3 * vStages + 12 + 2 + 1;
+  static constexpr int keys = 64;  // of one K or V tile: one step
+  static constexpr int q_tile = 128 * D * 2;
+  static constexpr int tile = keys * D * 2;
+  static constexpr int half = keys * 128;  // 64 columns of a tile
+  // Two stages each: K of step h is free when S of step h is done (s_full) and
+  // V when P V is (pv_done), so neither ring has barriers of its own for that.
+  static constexpr int stages = 2;
+  static constexpr int k_off = q_tile;
+  static constexpr int v_off = k_off + stages * tile;
+  static constexpr int bars = v_off + stages * tile;
+  // q_full, then [2] each: k_full, v_full, v_raw, s_full, p_full, pv_done; drain
+  static constexpr int n_bars = 1 + 6 * 2 + 1;
   static constexpr int tmem_slot = bars + 8 * n_bars;
-  static constexpr int alloc = tmem_slot + 16 + 1024;
+  static constexpr int alloc = tmem_slot + 16;
 };
+
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 struct TilesParams {
   void *out;
@@ -53,21 +70,21 @@ struct TilesParams {
   const int32_t *kv_lens;
   float *part;
   WindowRule rule;
-  int B, Hk, Lq, lk;
-  int pack, pack_log2;       // heads side by side in the rows of a tile, a power of two
-  int heads;                 // Hq
-  int head_groups;           // Hq / pack
-  int groups_per_key;        // head groups that share a key head
-  int rows, q_tiles, pairs;  // rows = pack * Lq of one head group
-  int n_whole, parts;        // items [0, n_whole) whole, the later ones in `parts` parts each
-  int sinks8;                // sinks of a session long enough to have a gap, rounded up to 8
+  int Lq, lk;
+  int pack, pack_log2;   // heads side by side in the rows of a tile, a power of two
+  int head_groups;       // Hq / pack
+  int groups_per_key;    // head groups that share a key head
+  int rows, q_tiles;     // rows = pack * Lq of one head group
+  int n_whole, parts;    // items [0, n_whole) whole, the later ones in `parts` parts each
+  int sinks8;            // sinks of a session long enough to have a gap, rounded up to 8
   int k_batch, k_head, v_batch, v_head;  // 0 where that dimension's stride is 0 (one box for all), else 1
   float scale_log2;
 };
 
+// A part's result: O [column][row], then [m, l, flag][row].
 template <int D>
 __host__ __device__ constexpr long long tiles_part_floats() {
-  return 2ll * 128 * (D + kTilesPartCols);
+  return 128ll * (D + kTilesPartCols);
 }
 
 template <typename T>
@@ -116,7 +133,10 @@ __device__ __forceinline__ uint32_t interval_mask(int lo, int hi, int n0) {
   return below_b & ~below_a;
 }
 
-// One 64-key step's P = 2^(S c2 - base) in pairs in v[0..31]; returns their sum as rounded.
+// One 64-key step's P = 2^(S c2 - base) in pairs in v[0..31]; returns their sum
+// as rounded.  (Taking an eighth to a half of the exponentials to the FMA pipe
+// with a polynomial of degree 3 was slower: 321 to 340 us against 313 for 24
+// heads of 3520 queries over 7920 keys; it takes ten issue slots for each.)
 template <typename T, bool kMasked>
 __device__ __forceinline__ float tiles_probs(uint32_t (&v)[64], const uint32_t (&seen)[2], float c2, float base) {
   using X = TilesType<T>;
@@ -140,84 +160,49 @@ __device__ __forceinline__ float tiles_probs(uint32_t (&v)[64], const uint32_t (
   return ((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7]));
 }
 
-// The MMA issuer of one query tile: key tiles t_lo .. t_hi - 1 of its own
-// order; the tiles before and after (of a pair's common list) are handed back
-// unread.  Returns false if a wait gave up.
+// Issues the products of one query tile over n 64-key steps.  S of step h + 2
+// goes into the buffer that P of step h came from, right after P V of step h.
+// What can be waited for ahead (V of this step, K of the one after the next)
+// is, so that only P stands between the softmax and the tensor core.
 template <typename T, int D>
-__device__ __forceinline__ bool tiles_issuer(int i, RingMap ring, uint32_t tmem, uint32_t sbase, int n_all, int t_lo,
-                                             int t_hi, uint64_t *q_full, uint64_t *k_full, uint64_t *k_empty,
-                                             uint64_t *v_full, uint64_t *v_empty, uint64_t *s_full, uint64_t *p_full,
-                                             uint64_t *pv_done, int *err) {
+__device__ __forceinline__ bool tiles_issuer(uint32_t tmem, uint32_t sbase, int n, uint64_t *q_full, uint64_t *k_full,
+                                           uint64_t *v_full, uint64_t *s_full, uint64_t *p_full, uint64_t *pv_done,
+                                           int *err) {
   using S = TilesSmem<D>;
-  constexpr int KS = S::kStages, VS = S::vStages;
   constexpr uint32_t fmt = TilesType<T>::fmt;
   constexpr uint32_t idesc_s = castdev::make_idesc(1, fmt, fmt, 0, 0, 128, 64);
   constexpr uint32_t idesc_pv = castdev::make_idesc(1, fmt, fmt, 0, 1, 128, D);
-  const DescW qd = desc_words(sbase + (ring.split ? 0 : i * S::tile), 16);
+  const DescW qd = desc_words(sbase, 16);
   const DescW kd = desc_words(sbase + S::k_off, 16);
-  const DescW vd = desc_words(sbase + S::v_off, 16384);
-  const uint32_t o_col = tmem + i * 128, s_col = tmem + 256 + i * 128;
-  uint64_t *my_s_full = s_full + 2 * i, *my_p_full = p_full + 2 * i, *my_pv_done = pv_done + 2 * i;
-
-  auto issue_s = [&](int r, int half) {
-    const uint32_t d = s_col + half * 64;
-    const uint32_t ko = (uint32_t)(r % KS) * S::tile + half * 8192;
+  const DescW vd = desc_words(sbase + S::v_off, S::half);
+  const uint32_t s_col = tmem + 128;
+  auto issue_s = [&](int buf) {
+    const uint32_t d = s_col + buf * 64, ko = buf * S::tile;
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      const uint32_t off = (s >> 2) * 16384 + (s & 3) * 32;
-      castdev::mma_f16_ss(d, qd.at(off), kd.at(ko + off), idesc_s, s > 0);
-    }
+    for (int s = 0; s < D / 16; ++s)
+      castdev::mma_f16_ss(d, qd.at((s >> 2) * 16384 + (s & 3) * 32), kd.at(ko + (s >> 2) * S::half + (s & 3) * 32),
+                          idesc_s, s > 0);
+    castdev::tc_commit(&s_full[buf]);
   };
-  // (a stage is handed back only once it is this tile's: its barrier's phase
-  // would otherwise count an arrival of another turn)
-  auto skip = [&](int t) {
-    const int r = ring.pos(t);
-    if (!castdev::mbar_wait(&k_full[r % KS], (r / KS) & 1, err)) return false;
-    castdev::mbar_arrive(&k_empty[r % KS]);
-    if (!castdev::mbar_wait(&v_full[r % VS], (r / VS) & 1, err)) return false;
-    castdev::mbar_arrive(&v_empty[r % VS]);
-    return true;
-  };
-  for (int t = 0; t < t_lo; ++t)
-    if (!skip(t)) return false;
-  if (t_lo < t_hi) {
-    int rk = ring.pos(t_lo);  // ring position of the next key tile to multiply
-    if (!castdev::mbar_wait(q_full, 0, err) || !castdev::mbar_wait(&k_full[rk % KS], (rk / KS) & 1, err)) return false;
+  if (!castdev::mbar_wait(q_full, 0, err)) return false;
+  for (int h = 0; h < min(n, 2); ++h) {
+    if (!castdev::mbar_wait(&k_full[h], 0, err)) return false;
     castdev::tc_fence_after();
-    issue_s(rk, 0);
-    castdev::tc_commit(&my_s_full[0]);
-    issue_s(rk, 1);
-    castdev::tc_commit(&my_s_full[1]);
-    castdev::tc_commit(&k_empty[rk % KS]);
-    for (int t = t_lo; t < t_hi; ++t) {
-      const int rv = ring.pos(t), vs = rv % VS;
-      const bool more = t + 1 < t_hi;
-      if (more) rk = ring.pos(t + 1);
-      if (!castdev::mbar_wait(&v_full[vs], (rv / VS) & 1, err)) return false;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        if (!castdev::mbar_wait(&my_p_full[half], (t - t_lo) & 1, err)) return false;
-        castdev::tc_fence_after();
-        const uint32_t vo = vs * S::tile + half * 8192, pa = s_col + half * 64;
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-          castdev::mma_f16_ts(o_col, pa + 8 * s, vd.at(vo + 2048 * s), idesc_pv, ((t - t_lo) | half | s) != 0);
-        castdev::tc_commit(&my_pv_done[half]);
-        if (more) {
-          if (half == 0) {
-            if (!castdev::mbar_wait(&k_full[rk % KS], (rk / KS) & 1, err)) return false;
-            castdev::tc_fence_after();
-          }
-          issue_s(rk, half);
-          castdev::tc_commit(&my_s_full[half]);
-        }
-      }
-      castdev::tc_commit(&v_empty[vs]);
-      if (more) castdev::tc_commit(&k_empty[rk % KS]);
-    }
+    issue_s(h);
   }
-  for (int t = max(t_lo, t_hi); t < n_all; ++t)
-    if (!skip(t)) return false;
+  for (int h = 0; h < n; ++h) {
+    const int buf = h & 1, phase = (h >> 1) & 1;
+    const bool more = h + 2 < n;
+    if (!castdev::mbar_wait(&v_full[buf], phase, err)) return false;
+    if (more && !castdev::mbar_wait(&k_full[buf], phase ^ 1, err)) return false;
+    if (!castdev::mbar_wait(&p_full[buf], phase, err)) return false;
+    castdev::tc_fence_after();
+    const uint32_t vo = buf * S::tile, pa = s_col + buf * 64;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) castdev::mma_f16_ts(tmem, pa + 8 * s, vd.at(vo + 2048 * s), idesc_pv, (h | s) != 0);
+    castdev::tc_commit(&pv_done[buf]);
+    if (more) issue_s(buf);
+  }
   return true;
 }
 
@@ -240,29 +225,25 @@ __device__ __noinline__ void tiles_give_back(const TilesParams &p, const WindowS
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kTilesThreads, 1)
+__global__ void __launch_bounds__(kTilesThreads, 2)
     window_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_k_sink,
                         const __grid_constant__ CUtensorMap tm_v_sink, const __grid_constant__ CUtensorMap tm_k_rest,
                         const __grid_constant__ CUtensorMap tm_v_rest, const __grid_constant__ TilesParams p) {
   using S = TilesSmem<D>;
   using X = TilesType<T>;
-  constexpr int KS = S::kStages, VS = S::vStages;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t *smem =
-      reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  constexpr int KT = S::keys;
+  extern __shared__ __align__(1024) uint8_t smem_tiles[];
+  uint8_t *smem = smem_tiles;
   uint64_t *bar = reinterpret_cast<uint64_t *>(smem + S::bars);
   uint64_t *q_full = bar;
   uint64_t *k_full = bar + 1;
-  uint64_t *k_empty = k_full + KS;
-  uint64_t *v_full = k_empty + KS;
-  uint64_t *v_empty = v_full + VS;
-  uint64_t *v_raw = v_empty + VS;  // a V tile has landed and is gone over before v_full
-  uint64_t *s_full = v_raw + VS;
-  uint64_t *p_full = s_full + 4;
-  uint64_t *pv_done = p_full + 4;
-  uint64_t *mma_drain = pv_done + 4;
-  uint64_t *merge_bar = mma_drain + 2;
+  uint64_t *v_full = k_full + 2;
+  uint64_t *v_raw = v_full + 2;  // a V tile has landed and is gone over before v_full
+  uint64_t *s_full = v_raw + 2;
+  uint64_t *p_full = s_full + 2;
+  uint64_t *pv_done = p_full + 2;
+  uint64_t *mma_drain = pv_done + 2;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + S::tmem_slot);
   volatile uint32_t *bad_flag = tmem_slot + 1;  // an infinity or NaN was taken out of a V tile
   int *err = reinterpret_cast<int *>(tmem_slot + 2);
@@ -275,13 +256,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
     x = p.n_whole + (x - p.n_whole) / p.parts;
     n_parts = p.parts;
   }
-  const int bhg = x / p.pairs;
-  const int pair = p.pairs - 1 - (x - bhg * p.pairs);  // later rows see more keys: first
+  const int bhg = x / p.q_tiles;
+  const int qt = p.q_tiles - 1 - (x - bhg * p.q_tiles);  // later rows see more keys: first
   const int b = bhg / p.head_groups, hg = bhg - b * p.head_groups;
   const int hk = hg / p.groups_per_key;
-  const int t0 = 2 * pair;
-  const int nq = min(2, p.q_tiles - t0);
-  const int row0 = t0 * 128, row_end = min(p.rows, row0 + nq * 128);
+  const int row0 = qt * 128, row_end = min(p.rows, row0 + 128);
   int len = p.kv_lens ? p.kv_lens[b] : p.lk;
   if (len < 0 || len > p.lk) {  // a session longer than its keys: nothing past them is read
     if (threadIdx.x == 0) atomicExch(&g_cast_device_error, (int)CAST_ERR_INVALID_ARGUMENT);
@@ -291,136 +270,132 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
   // places: [0, s_n) sinks, [s_n, s8) nothing, from s8 the keys from span.base on
   const int s8 = span.s_n > 0 ? p.sinks8 : 0;
   const int n_places = span.n - span.s_n + s8;
-  const int n_tiles = span.n > 0 ? (n_places + 127) / 128 : 0;
+  const int n_tiles = span.n > 0 ? (n_places + KT - 1) / KT : 0;
   const int kt_lo = (int)((long long)part * n_tiles / n_parts);
   const int n_kv = (int)((long long)(part + 1) * n_tiles / n_parts) - kt_lo;
-  const bool split = nq == 1 && n_kv >= 2;
-  const int n_a = split ? (n_kv + 1) / 2 : n_kv;
-  const int n_b = split ? n_kv - n_a : n_kv;
-  const int n_groups = split ? 2 : nq;
-  const RingMap ring0{split ? 1 : 0, 0, n_a, n_b};
-  // Own key tiles of query tile i of a pair, [first, end) of this CTA's; a
-  // tile in which it sees nothing may be among them.
-  auto own = [&](int i, int &first, int &end) {
-    first = 0;
-    end = i == 0 ? n_a : n_b;
-    if (nq < 2) return;
-    const int r0 = row0 + i * 128, r1 = min(p.rows, r0 + 128);
-    const WindowSpan s = window_span(p.rule, len, p.Lq, r0 >> p.pack_log2, (r1 - 1) >> p.pack_log2);
-    if (s.n == 0) {
-      end = 0;
-      return;
-    }
-    // places [a, z) hold every key it sees
-    const int a = span.sinks > 0 ? 0 : max(0, s8 + s.lo0 - span.base), z = s8 + s.hi1 - span.base;
-    first = min(max(a / 128 - kt_lo, 0), end);
-    end = max(first, min(end, (z + 127) / 128 - kt_lo));
-  };
+  constexpr int kKWarp = 4, kMWarp = 5, kVWarp = 6;
 
-  if (warp == kProducerWarp && lane == 0) {
+  if (warp == kKWarp && lane == 0) {
     *err = 0;
     *bad_flag = 0;
     for (int i = 0; i < S::n_bars; ++i) castdev::mbar_init(&bar[i], 1);
-    for (int i = 0; i < 4; ++i) castdev::mbar_init(&p_full[i], 4);
-    castdev::mbar_init(merge_bar, 4);
-    for (int i = 0; i < KS; ++i) castdev::mbar_init(&k_empty[i], split ? 1 : nq);
-    for (int i = 0; i < VS; ++i) castdev::mbar_init(&v_empty[i], split ? 1 : nq);
+    for (int i = 0; i < 2; ++i) castdev::mbar_init(&p_full[i], 4);
     castdev::fence_barrier_init();
     castdev::tma_prefetch_desc(&tm_q);
     castdev::tma_prefetch_desc(&tm_k);
     castdev::tma_prefetch_desc(&tm_v);
     if (n_kv > 0) {
-      castdev::mbar_arrive_expect_tx(q_full, nq * S::tile);
-      for (int i = 0; i < nq; ++i)
+      castdev::mbar_arrive_expect_tx(q_full, S::q_tile);
 #pragma unroll
-        for (int h = 0; h < D / 64; ++h)
-          tma_load_5d(smem + i * S::tile + h * 16384, &tm_q, q_full, 64 * h, 0, (row0 + i * 128) >> p.pack_log2, hg, b);
+      for (int h = 0; h < D / 64; ++h)
+        tma_load_5d(smem + h * 16384, &tm_q, q_full, 64 * h, 0, row0 >> p.pack_log2, hg, b);
     }
   }
-  if (warp == kMmaWarp) {
-    castdev::tmem_alloc(tmem_slot, 512);
+  if (warp == kMWarp) {
+    castdev::tmem_alloc(tmem_slot, 256);
     castdev::tmem_relinquish();
   }
   __syncthreads();
   castdev::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // Starts the copies of the tile of 128 places from place n0 on.
+  // Starts the copies of the tile of KT places from place n0 on.
   auto start = [&](uint8_t *dst, uint64_t *full, int n0, const CUtensorMap *whole, const CUtensorMap *sink,
                    const CUtensorMap *rest, int head, int batch) {
-    if (n0 >= s8 || n0 + 128 <= s8) {
+    if (n0 >= s8 || n0 + KT <= s8) {
       const int key = n0 >= s8 ? span.base + n0 - s8 : n0;
 #pragma unroll
-      for (int h = 0; h < D / 64; ++h) castdev::tma_load_4d(dst + h * 16384, whole, full, 64 * h, key, head, batch);
+      for (int h = 0; h < D / 64; ++h) castdev::tma_load_4d(dst + h * S::half, whole, full, 64 * h, key, head, batch);
     } else {
       const int r = s8 - n0;
 #pragma unroll
       for (int h = 0; h < D / 64; ++h) {
-        castdev::tma_load_4d(dst + h * 16384, sink, full, 64 * h, n0, head, batch);
-        castdev::tma_load_4d(dst + h * 16384 + r * 128, rest, full, 64 * h, span.base, head, batch);
+        castdev::tma_load_4d(dst + h * S::half, sink, full, 64 * h, n0, head, batch);
+        castdev::tma_load_4d(dst + h * S::half + r * 128, rest, full, 64 * h, span.base, head, batch);
       }
     }
   };
 
-  if (warp >= 8) {
-    if (warp == kProducerWarp) {
+  if (warp >= 4) {
+    regs_dec<kTilesRegsRest>();
+    if (warp == kKWarp) {
       if (lane == 0 && n_kv > 0) {
         int issued = 0;
         for (int j = 0; j < n_kv; ++j) {
-          const int n0 = (kt_lo + ring0.key_tile(j)) * 128, ks = j % KS;
-          if (j >= KS && !castdev::mbar_wait(&k_empty[ks], ((j / KS) - 1) & 1, err)) break;
+          const int n0 = (kt_lo + j) * KT, ks = j & 1;
+          if (j >= 2 && !castdev::mbar_wait(&s_full[ks], ((j >> 1) - 1) & 1, err)) break;
           castdev::mbar_arrive_expect_tx(&k_full[ks], S::tile);
           start(smem + S::k_off + ks * S::tile, &k_full[ks], n0, &tm_k, &tm_k_sink, &tm_k_rest, hk * p.k_head,
                 b * p.k_batch);
           issued = j + 1;
         }
         castdev::mbar_wait_drain(q_full, 0, err);
-        for (int j = max(0, issued - KS); j < issued; ++j)
-          castdev::mbar_wait_drain(&k_full[j % KS], (j / KS) & 1, err);
+        for (int j = max(0, issued - 2); j < issued; ++j)
+          castdev::mbar_wait_drain(&k_full[j & 1], (j >> 1) & 1, err);
       }
-    } else if (warp == kVProducerWarp) {
+    } else if (warp == kVWarp) {
       // whole warp: lane 0 starts the copies, all go over tiles that are not wholly visible
       uint32_t raw_phase = 0;  // bit per stage
       // every row sees place n (sinks and the keys of all rows)
       auto all_see = [&](int n) {
         return !span.unplaced && (n < min(span.sinks, span.hi0) || (n >= s8 + span.lo1 - span.base && n < s8 + span.hi0 - span.base));
       };
-      auto any_sees = [&](int n) { return n < n_places && (n < span.s_n || n >= s8); };
-      // (both ends of a run of 128 places: visible ones are one or two intervals)
+      // (both ends of a run of KT places: visible ones are one or two intervals)
       auto ragged = [&](int n0) {
-        if (span.unplaced || n0 + 128 > n_places) return true;
+        if (span.unplaced || n0 + KT > n_places) return true;
         const int a = min(span.sinks, span.hi0), l = s8 + span.lo1 - span.base, h = s8 + span.hi0 - span.base;
-        return !(n0 + 128 <= a || (n0 >= l && n0 + 128 <= h) || (a >= l && n0 + 128 <= h));
+        return !(n0 + KT <= a || (n0 >= l && n0 + KT <= h) || (a >= l && n0 + KT <= h));
       };
       auto go_over = [&](int j) -> bool {
-        const int n0 = (kt_lo + ring0.key_tile(j)) * 128, vs = j % VS;
+        const int n0 = (kt_lo + j) * KT, vs = j & 1;
         const bool ok = castdev::mbar_wait(&v_raw[vs], (raw_phase >> vs) & 1, err);
         if (!__all_sync(0xffffffffu, ok)) return false;
         raw_phase ^= 1u << vs;
         uint8_t *tile = smem + S::v_off + vs * S::tile;
-        bool bad = false;
-#pragma unroll 4
-        for (int r = lane >> 3; r < 128; r += 4) {  // eight lanes a row of 128 bytes
-          const int n = n0 + r;
-          if (all_see(n)) continue;
-          const bool some = any_sees(n);
+        // rows that nobody sees: places [s_n, s8) and from n_places on
+        auto zero = [&](int from, int to) {
+          for (int r = max(from, 0) + (lane >> 3); r < min(to, KT); r += 4)
 #pragma unroll
-          for (int h = 0; h < D / 64; ++h) {
-            uint4 *w = reinterpret_cast<uint4 *>(tile + h * 16384 + r * 128) + (lane & 7);
-            if (!some) {
-              *w = make_uint4(0u, 0u, 0u, 0u);
-            } else {
-              uint4 u = *w;
+            for (int h = 0; h < D / 64; ++h)
+              reinterpret_cast<uint4 *>(tile + h * S::half + r * 128)[lane & 7] = make_uint4(0u, 0u, 0u, 0u);
+        };
+        if (s8 > span.s_n) zero(span.s_n - n0, s8 - n0);
+        zero(n_places - n0, KT);
+        __syncwarp();
+        // 0 * x is NaN for the values looked for, and only for them
+        uint32_t acc = 0;
+        const uint4 *w = reinterpret_cast<const uint4 *>(tile) + lane;
+#pragma unroll
+        for (int i0 = 0; i0 < S::tile / 512; i0 += 8) {
+          uint4 u[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) u[i] = w[(i0 + i) * 32];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            acc = Half2<T>::fma0(u[i].x, acc);
+            acc = Half2<T>::fma0(u[i].y, acc);
+            acc = Half2<T>::fma0(u[i].z, acc);
+            acc = Half2<T>::fma0(u[i].w, acc);
+          }
+        }
+        if (__any_sync(0xffffffffu, Half2<T>::bad(acc) != 0)) {
+          bool bad = false;
+          for (int r = lane >> 3; r < KT; r += 4) {  // eight lanes a row of 128 bytes
+            if (all_see(n0 + r)) continue;
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h) {
+              uint4 *q = reinterpret_cast<uint4 *>(tile + h * S::half + r * 128) + (lane & 7);
+              const uint4 u = *q;
               const uint32_t b0 = Half2<T>::bad(u.x), b1 = Half2<T>::bad(u.y), b2 = Half2<T>::bad(u.z),
                              b3 = Half2<T>::bad(u.w);
               if (b0 | b1 | b2 | b3) {
                 bad = true;
-                *w = make_uint4(u.x & ~b0, u.y & ~b1, u.z & ~b2, u.w & ~b3);
+                *q = make_uint4(u.x & ~b0, u.y & ~b1, u.z & ~b2, u.w & ~b3);
               }
             }
           }
+          if (bad) *bad_flag = 1;
         }
-        if (bad) *bad_flag = 1;
         castdev::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) castdev::mbar_arrive(&v_full[vs]);
@@ -428,59 +403,51 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
       };
       int issued = 0, looked = 0;  // tiles started; tiles gone over
       bool ok = true;
-      for (int j = 0; ok && j < n_kv; ++j) {
-        const int n0 = (kt_lo + ring0.key_tile(j)) * 128, vs = j % VS;
-        ok = j < VS || castdev::mbar_wait(&v_empty[vs], ((j / VS) - 1) & 1, err);
-        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      auto issue = [&](int j) {
+        const int n0 = (kt_lo + j) * KT, vs = j & 1;
         uint64_t *full = ragged(n0) ? &v_raw[vs] : &v_full[vs];
         if (lane == 0) {
           castdev::mbar_arrive_expect_tx(full, S::tile);
           start(smem + S::v_off + vs * S::tile, full, n0, &tm_v, &tm_v_sink, &tm_v_rest, hk * p.v_head, b * p.v_batch);
         }
         issued = j + 1;
-        if (j > 0) {
-          if (ragged((kt_lo + ring0.key_tile(j - 1)) * 128)) ok = go_over(j - 1);
-          looked = j;
-        }
+      };
+      if (n_kv > 1) issue(0);
+      for (int j = 0; ok && j < n_kv; ++j) {
+        if (j >= 2) ok = __all_sync(0xffffffffu, castdev::mbar_wait(&pv_done[j & 1], ((j >> 1) - 1) & 1, err));
+        if (!ok) break;
+        const int next = j == 0 && n_kv > 1 ? 1 : j;  // the first two are started together
+        if (next >= issued) issue(next);
+        if (ragged((kt_lo + j) * KT)) ok = go_over(j);
+        if (ok) looked = j + 1;
       }
-      if (ok && issued > 0 && ragged((kt_lo + ring0.key_tile(issued - 1)) * 128)) ok = go_over(issued - 1);
-      if (ok) looked = issued;
       // every copy lands before the CTA leaves: those gone over have; the
       // others' own barriers say so
       if (lane == 0)
-        for (int j = max(0, issued - VS); j < issued; ++j) {
-          const int vs = j % VS;
-          if (!ragged((kt_lo + ring0.key_tile(j)) * 128))
-            castdev::mbar_wait_drain(&v_full[vs], (j / VS) & 1, err);
+        for (int j = max(0, issued - 2); j < issued; ++j) {
+          const int vs = j & 1;
+          if (!ragged((kt_lo + j) * KT))
+            castdev::mbar_wait_drain(&v_full[vs], (j >> 1) & 1, err);
           else if (j >= looked)
             castdev::mbar_wait_drain(&v_raw[vs], (raw_phase >> vs) & 1, err);
         }
-    } else {
-      const int i = warp == kMmaWarp ? 0 : 1;
-      if (lane == 0 && n_kv > 0 && i < n_groups) {
-        const RingMap ring{split ? 1 : 0, i, n_a, n_b};
-        int first, end;
-        own(i, first, end);
-        tiles_issuer<T, D>(i, ring, tmem, castdev::smem_u32(smem), i == 0 ? n_a : n_b, first, end, q_full, k_full,
-                           k_empty, v_full, v_empty, s_full, p_full, pv_done, err);
-        castdev::tc_commit(&mma_drain[i]);
-        castdev::mbar_wait_drain(&mma_drain[i], 0, err);
+    } else if (warp == kMWarp) {
+      if (lane == 0 && n_kv > 0) {
+        tiles_issuer<T, D>(tmem, castdev::smem_u32(smem), n_kv, q_full, k_full, v_full, s_full, p_full, pv_done, err);
+        castdev::tc_commit(mma_drain);
+        castdev::mbar_wait_drain(mma_drain, 0, err);
       }
     }
   } else {
     // ------------------------------------------------------------ softmax
-    const int ti = warp >> 2;
-    const int lrow = (warp & 3) * 32 + lane;
-    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t o_addr = tmem + lane_off + ti * 128;
-    const uint32_t s_addr = tmem + lane_off + 256 + ti * 128;
-    const bool active = ti < n_groups;
-    int first = 0, end = 0;
-    if (active) own(ti, first, end);
-    const int my_steps = 2 * (end - first);
-    const int start_tile = kt_lo + ((split && ti == 1) ? n_a : 0) + first;
-    const int row = row0 + (split ? 0 : ti) * 128 + lrow;
-    const bool row_valid = active && row < p.rows;
+    regs_inc<kTilesRegsSoft>();
+    const int lrow = warp * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+    const uint32_t o_addr = tmem + lane_off;
+    const uint32_t s_addr = tmem + lane_off + 128;
+    const int my_steps = n_kv;
+    const int row = row0 + lrow;
+    const bool row_valid = row < p.rows;
     const int token = row >> p.pack_log2, head = hg * p.pack + (row & (p.pack - 1));
     // this row's places: [0, near) and [from, to)
     int lo = 0, hi = 0, near = 0, from = 0, to = 0;
@@ -491,24 +458,30 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
       from = s8 + lo - span.base;
       to = s8 + hi - span.base;
     }
+    // what all rows of the warp see, and what none does (rows past the end are left out)
+    const int big = 1 << 30;
+    const int w_near_lo = __reduce_min_sync(0xffffffffu, row_valid ? near : big);
+    const int w_near_hi = __reduce_max_sync(0xffffffffu, near);
+    const int w_from_lo = __reduce_min_sync(0xffffffffu, row_valid ? from : big);
+    const int w_from_hi = __reduce_max_sync(0xffffffffu, from);
+    const int w_to_lo = __reduce_min_sync(0xffffffffu, row_valid ? to : big);
+    const int w_to_hi = __reduce_max_sync(0xffffffffu, to);
     // (a row that will see nothing must not keep its warp on the slow path)
     float m_run = hi > 0 ? -INFINITY : 0.0f, l_run = 0.0f;
     bool ok = true;
     const float c2 = p.scale_log2;
-    for (int h = 0; active && h < my_steps; ++h) {
+    for (int h = 0; h < my_steps; ++h) {
       const int half = h & 1;
-      const int n0 = start_tile * 128 + h * 64;
-      const bool all = n0 + 64 <= near || (n0 >= from && n0 + 64 <= to) || !row_valid;
-      const bool none = (n0 >= near && (n0 + 64 <= from || n0 >= to)) || !row_valid;
-      const bool full_step = __all_sync(0xffffffffu, all);
-      const bool empty_step = __all_sync(0xffffffffu, none);
+      const int n0 = kt_lo * KT + h * 64;
+      const bool full_step = n0 + 64 <= w_near_lo || (n0 >= w_from_hi && n0 + 64 <= w_to_lo);
+      const bool empty_step = n0 >= w_near_hi && (n0 + 64 <= w_from_lo || n0 >= w_to_hi);
       uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
       if (!full_step) {
 #pragma unroll
         for (int w = 0; w < 2; ++w)
           seen[w] = interval_mask(0, near, n0 + 32 * w) | interval_mask(from, to, n0 + 32 * w);
       }
-      ok = __all_sync(0xffffffffu, castdev::mbar_wait(&s_full[ti * 2 + half], (h >> 1) & 1, err));
+      ok = __all_sync(0xffffffffu, castdev::mbar_wait(&s_full[half], (h >> 1) & 1, err));
       if (!ok) break;
       castdev::tc_fence_after();
       const uint32_t sb = s_addr + 64 * half;
@@ -543,7 +516,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
           }
           if (h > 0 && __any_sync(0xffffffffu, o_scale != 1.0f)) {
             const int hp = h - 1;
-            ok = __all_sync(0xffffffffu, castdev::mbar_wait(&pv_done[ti * 2 + (hp & 1)], (hp >> 1) & 1, err));
+            ok = __all_sync(0xffffffffu, castdev::mbar_wait(&pv_done[hp & 1], (hp >> 1) & 1, err));
             if (!ok) break;
             castdev::tc_fence_after();
 #pragma unroll 1
@@ -565,56 +538,23 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
       castdev::tmem_wait_st();
       castdev::tc_fence_before();
       __syncwarp();
-      if (lane == 0) castdev::mbar_arrive(&p_full[ti * 2 + half]);
+      if (lane == 0) castdev::mbar_arrive(&p_full[half]);
     }
     if (hi == 0) {  // a row that sees nothing is nothing (and its maximum is none)
       m_run = -INFINITY;
       l_run = 0.0f;
     }
     // ------------------------------------------------------------ epilogue
-    if (active && ok && my_steps > 0) {
+    if (ok && my_steps > 0) {
       const int hl = my_steps - 1;
-      ok = __all_sync(0xffffffffu, castdev::mbar_wait(&pv_done[ti * 2 + (hl & 1)], (hl >> 1) & 1, err));
+      ok = __all_sync(0xffffffffu, castdev::mbar_wait(&pv_done[hl & 1], (hl >> 1) & 1, err));
       castdev::tc_fence_after();
     }
-    if (split && ti == 1) {
-      if (ok) {
-        castdev::tmem_st1(s_addr, __float_as_uint(m_run));
-        castdev::tmem_st1(s_addr + 1, __float_as_uint(l_run));
-        castdev::tmem_wait_st();
-      }
-      castdev::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) castdev::mbar_arrive(merge_bar);
-    } else if (active) {
-      float scale0 = 1.0f, scale1 = 0.0f;
-      const uint32_t o1_addr = tmem + lane_off + 128;
-      if (split && ok) {
-        ok = __all_sync(0xffffffffu, castdev::mbar_wait(merge_bar, 0, err));
-        castdev::tc_fence_after();
-        const uint32_t s1_addr = tmem + lane_off + 256 + 128;
-        const float m1 = __uint_as_float(castdev::tmem_ld1(s1_addr));
-        const float l1 = __uint_as_float(castdev::tmem_ld1(s1_addr + 1));
-        castdev::tmem_wait_ld();
-        const float m = fmaxf(m_run, m1);
-        scale0 = m_run == -INFINITY ? 0.0f : fast_exp2(m_run - m);
-        scale1 = m1 == -INFINITY ? 0.0f : fast_exp2(m1 - m);
-        l_run = l_run * scale0 + l1 * scale1;
-        m_run = m;
-      }
+    {
       auto load_o = [&](int cc, uint32_t (&o)[32]) {
         if (my_steps > 0) {
           castdev::tmem_ld32(o_addr + 32 * cc, o);
-          if (split) {
-            uint32_t o1[32];
-            castdev::tmem_ld32(o1_addr + 32 * cc, o1);
-            castdev::tmem_wait_ld();
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              o[c] = __float_as_uint(fmaf(__uint_as_float(o1[c]), scale1, __uint_as_float(o[c]) * scale0));
-          } else {
-            castdev::tmem_wait_ld();
-          }
+          castdev::tmem_wait_ld();
         } else {
 #pragma unroll
           for (int c = 0; c < 32; ++c) o[c] = 0u;
@@ -652,7 +592,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
       } else if (ok) {
         // this part's O, maximum and sum: [tile][column][row], then [tile][m, l, flag][row]
         float *slot = p.part + (long long)(blockIdx.x - p.n_whole) * tiles_part_floats<D>();
-        float *tail = slot + 2 * 128 * D + ti * (128 * kTilesPartCols) + lrow;
+        float *tail = slot + 128 * D + lrow;
         if (row_valid) {
           tail[0] = hi > 0 ? m_run : -INFINITY;
           tail[128] = l_run;
@@ -664,7 +604,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
             uint32_t o[32];
             __syncwarp();
             load_o(cc, o);
-            float *dst = slot + ti * (128 * D) + 32 * cc * 128 + lrow;
+            float *dst = slot + 32 * cc * 128 + lrow;
             if (row_valid) {
 #pragma unroll
               for (int c = 0; c < 32; ++c) dst[c * 128] = __uint_as_float(o[c]);
@@ -675,9 +615,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
     }
   }
   __syncthreads();
-  if (warp == kMmaWarp) {
+  if (warp == kMWarp) {
     castdev::tc_fence_after();
-    castdev::tmem_dealloc(tmem, 512);
+    castdev::tmem_dealloc(tmem, 256);
   }
 }
 
@@ -688,17 +628,16 @@ template <typename T, int D>
 __global__ void __launch_bounds__(128 * kJoinGroups) window_tiles_join_kernel(const __grid_constant__ TilesParams p) {
   __shared__ float acc_s[kJoinGroups][kJoinCols + 1][128];
   constexpr int cuts = D / kJoinCols;
-  const int cut = blockIdx.x % cuts, ti = blockIdx.x / cuts % 2, item = blockIdx.x / (2 * cuts);
+  const int cut = blockIdx.x % cuts, item = blockIdx.x / cuts;
   const int row_in = threadIdx.x & 127, g = threadIdx.x >> 7;
   const int x = p.n_whole + item;
-  const int bhg = x / p.pairs, pair = p.pairs - 1 - (x - bhg * p.pairs);
+  const int bhg = x / p.q_tiles, qt = p.q_tiles - 1 - (x - bhg * p.q_tiles);
   const int b = bhg / p.head_groups, hg = bhg - b * p.head_groups;
-  const int t0 = 2 * pair, row0 = t0 * 128, row_end = min(p.rows, row0 + min(2, p.q_tiles - t0) * 128);
-  const int row = row0 + ti * 128 + row_in;
-  if (row0 + ti * 128 >= p.rows) return;  // (whole CTAs)
+  const int row0 = qt * 128, row_end = min(p.rows, row0 + 128);
+  const int row = row0 + row_in;
   const bool on = row < p.rows;
   const float *base = p.part + (long long)item * p.parts * tiles_part_floats<D>();
-  const float *tails = base + 2 * 128 * D + ti * (128 * kTilesPartCols) + row_in;
+  const float *tails = base + 128 * D + row_in;
   float m = -INFINITY;
   bool bad = false;
   if (on)
@@ -714,7 +653,7 @@ __global__ void __launch_bounds__(128 * kJoinGroups) window_tiles_join_kernel(co
       bad = bad || __float_as_int(tail[256]) != 0;
       if (mj == -INFINITY) continue;  // nothing seen: its O may not be written
       const float f = fast_exp2(mj - m);
-      const float *o = base + j * tiles_part_floats<D>() + ti * (128 * D) + cut * kJoinCols * 128 + row_in;
+      const float *o = base + j * tiles_part_floats<D>() + cut * kJoinCols * 128 + row_in;
       l = fmaf(tail[128], f, l);
 #pragma unroll
       for (int c = 0; c < kJoinCols; ++c) a[c] = fmaf(o[c * 128], f, a[c]);
