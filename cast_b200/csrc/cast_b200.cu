@@ -1341,6 +1341,7 @@ static RowsPlan rows_plan(long long B, int Hk, int group, int Lq, int capacity, 
   const long long most = std::max<long long>(1, (long long)(span / 128));
   const long long want = std::max<long long>(1, 2ll * n_sms / items);
   long long n = std::min(most, want);
+  { static const char *e = getenv("CAST_ROWS_SPLIT"); if (e) n = std::min<long long>(std::max<long long>(1,(long long)(span/16)), atoi(e)); }
   if (n <= castk::kRowsMaxCluster) {
     long long c = 1;
     while (2 * c <= n) c *= 2;

@@ -159,6 +159,9 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // --------------------------------------------------------------- few rows
 constexpr int kRowsWarps = 4;
 constexpr int kRowsStages = 3;
@@ -206,22 +209,23 @@ __device__ __forceinline__ const T *rows_value(const RowsParams &p, int b, int h
   return pg < 0 || pg >= p.n_pages ? nullptr : v + pg * p.vs[0] + (key % p.page) * p.vs[2];
 }
 
-// Joins the parts' (O, m, l) of rows r0 .. r_end - 1, normalises and writes
-// share `rank` of `ranks` of them; part(j) is the j-th part's buffer, rows of
-// D + 4 floats: O, m, l and whether the part took an infinity or NaN out of a
-// value that only some rows see.
+// Joins the parts' (O, m, l) of rows first, first + step, ... of a tile's
+// n_rows, normalises and writes them; part(r, j) is the j-th part's row: O, m,
+// l and whether the part took an infinity or NaN out of a value that only some
+// rows see.
 template <typename T, int D, int MT, bool kPaged, typename Part>
 __device__ __forceinline__ void window_write(const RowsParams &p, const WindowSpan &span, int b, int hk, int r0,
-                                             int r_end, int rank, int ranks, const Part &part, int thread,
+                                             int n_rows, int first, int step, const Part &part, int thread,
                                              int threads) {
-  constexpr int kRow = D + 4;
-  for (int x = rank * threads + thread; x < (r_end - r0) * (D / 4); x += ranks * threads) {
-    const int r = x / (D / 4), c = (x % (D / 4)) * 4;
+  const int mine = first < n_rows ? (n_rows - first + step - 1) / step : 0;
+  for (int x = thread; x < mine * (D / 4); x += threads) {
+    const int r = first + x / (D / 4) * step, c = (x % (D / 4)) * 4;
     float m = -INFINITY, bad = 0.0f;
-    for (int j = 0; j < p.n_split; ++j) m = fmaxf(m, part(j)[r * kRow + D]);
+    for (int j = 0; j < p.n_split; ++j) m = fmaxf(m, part(r, j)[D]);
     float l = 0.0f, a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
     for (int j = 0; j < p.n_split; ++j) {
-      const float *row = part(j) + r * kRow;
+      const float *row = part(r, j);
       const float4 tail = *reinterpret_cast<const float4 *>(row + D);
       const float f = tail.x == -INFINITY ? 0.0f : fast_exp2(tail.x - m);
       const float4 v = *reinterpret_cast<const float4 *>(row + c);
@@ -281,6 +285,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
   const int g_hi = (int)((long long)groups * (split + 1) / p.n_split);
   const bool partial = span.lo0 != span.lo1 || span.hi0 != span.hi1 || span.unplaced;
   if (threadIdx.x == 0) flag_bad = 0;
+  if (p.n_split > 1 && !p.part) cluster_arrive();  // (waited for before the first push)
   __syncthreads();
 
   // ---- Q fragments: row r = lane / 4 (+ 8), columns 2 (lane % 4) (+ 8) of each 16
@@ -522,10 +527,11 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
   if (saw_bad) flag_bad = 1;
   __syncthreads();
 
-  // ---- join the warps: (O, m, l) of each in shared memory, rows of D + 4 floats
+  // ---- join the warps: (O, m, l) of each row in shared memory, rows of D + 4 floats
   constexpr int kRow = D + 4;
+  const int n_rows = r_end - r0;
   float *js = reinterpret_cast<float *>(smem_rows);
-  float *own = reinterpret_cast<float *>(smem_rows + (S::ring > S::join ? S::ring : S::join));
+  float *box = reinterpret_cast<float *>(smem_rows + (S::ring > S::join ? S::ring : S::join));
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -533,7 +539,9 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
       float l = l_run[mt][hh];
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
-      float *row = js + (warp * R + 16 * mt + lane / 4 + 8 * hh) * kRow;
+      const int r = 16 * mt + lane / 4 + 8 * hh;
+      if (r >= n_rows) continue;
+      float *row = js + (warp * R + r) * kRow;
 #pragma unroll
       for (int j = 0; j < D / 8; ++j)
         *reinterpret_cast<float2 *>(row + 8 * j + 2 * (lane % 4)) = make_float2(o[mt][j][2 * hh], o[mt][j][2 * hh + 1]);
@@ -543,8 +551,15 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
       }
     }
   __syncthreads();
-  float *part = p.part ? p.part + (long long)blockIdx.x * (R * kRow) : own;
-  for (int x = threadIdx.x; x < R * (D / 4); x += blockDim.x) {
+  // Row r of every CTA of the cluster goes to CTA r % n_split, place
+  // (r / n_split) n_split + split of its box (16 MT rows in all), which
+  // joins them: one barrier between the pushes and the joins, and nobody's
+  // memory is touched after it.
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const bool push = p.n_split > 1 && !p.part;
+  if (push) cluster_wait();  // every CTA of the cluster runs
+  for (int x = threadIdx.x; x < n_rows * (D / 4); x += blockDim.x) {
     const int r = x / (D / 4), c = (x % (D / 4)) * 4;
     float m = -INFINITY;
 #pragma unroll
@@ -559,26 +574,21 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
       l = fmaf(row[D + 1], f, l);
       a.x = fmaf(v.x, f, a.x), a.y = fmaf(v.y, f, a.y), a.z = fmaf(v.z, f, a.z), a.w = fmaf(v.w, f, a.w);
     }
-    *reinterpret_cast<float4 *>(part + r * kRow + c) = a;
-    if (c == 0) {
-      part[r * kRow + D] = m;
-      part[r * kRow + D + 1] = l;
-      part[r * kRow + D + 2] = __int_as_float(flag_bad);
-    }
+    float *dst = push ? cluster.map_shared_rank(box, r % p.n_split) + (r / p.n_split * p.n_split + split) * kRow
+                      : (p.part ? p.part + (long long)blockIdx.x * (R * kRow) : box) + r * kRow;
+    *reinterpret_cast<float4 *>(dst + c) = a;
+    if (c == 0) *reinterpret_cast<float4 *>(dst + D) = make_float4(m, l, __int_as_float(flag_bad), 0.0f);
   }
   if (p.part) return;  // window_rows_join_kernel joins the CTAs
-
-  // ---- join the cluster's CTAs and write
-  namespace cg = cooperative_groups;
-  cg::cluster_group cluster = cg::this_cluster();
-  if (p.n_split > 1)
-    cluster.sync();
-  else
+  if (push) {
+    cluster_arrive();
+    cluster_wait();
+  } else {
     __syncthreads();
-  window_write<T, D, MT, kPaged>(p, span, b, hk, r0, r_end, split, p.n_split,
-                                 [&](int j) { return p.n_split > 1 ? cluster.map_shared_rank(own, j) : own; },
+  }
+  window_write<T, D, MT, kPaged>(p, span, b, hk, r0, n_rows, push ? split : 0, push ? p.n_split : 1,
+                                 [&](int r, int j) { return box + (push ? r / p.n_split * p.n_split + j : r) * kRow; },
                                  (int)threadIdx.x, (int)blockDim.x);
-  if (p.n_split > 1) cluster.sync();  // no CTA leaves while its memory is read
 }
 
 // Joins the parts that window_rows_kernel left in p.part: kJoinShare CTAs for
@@ -594,9 +604,9 @@ __global__ void __launch_bounds__(128) window_rows_join_kernel(const __grid_cons
   const int len = min(max(p.kv_lens ? p.kv_lens[b] : p.lk, 0), p.lk);
   const WindowSpan span = window_span(p.rule, len, p.Lq, r0 / p.group, (r_end - 1) / p.group);
   const float *base = p.part + (long long)item * p.n_split * (R * (D + 4));
-  window_write<T, D, MT, kPaged>(p, span, b, hk, r0, r_end, blockIdx.x % kJoinShare, kJoinShare,
-                                 [&](int j) { return base + (long long)j * (R * (D + 4)); }, (int)threadIdx.x,
-                                 (int)blockDim.x);
+  window_write<T, D, MT, kPaged>(p, span, b, hk, r0, r_end - r0, blockIdx.x % kJoinShare, kJoinShare,
+                                 [&](int r, int j) { return base + ((long long)j * R + r) * (D + 4); },
+                                 (int)threadIdx.x, (int)blockDim.x);
 }
 
 }  // namespace castk

@@ -84,11 +84,8 @@ def _keep(plans: dict, key, plan):
     return plan
 
 
-def _no_grad_needed(*tensors) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise ValueError("an input needs a gradient, which this operator has not (use torch.no_grad())")
+def _no_gradient():
+    raise ValueError("an input needs a gradient, which this operator has not (use torch.no_grad())")
 
 
 def _launch(index: int, name: str, *args) -> None:
@@ -243,14 +240,17 @@ def rope(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor | None = 
     if axes is not None:
         axes = tuple(axes)
     try:
-        key = (_sig(x), _sig(table), _sig(positions), interleaved, axes, inverse, start, _sig(out))
+        key = (x.dtype, x.shape, x.stride(), x.device, table.dtype, table.shape, table.stride(), table.device,
+               None if positions is None else _sig(positions), None if out is None else _sig(out), interleaved, axes,
+               inverse, start)
         plan = _rope_plans.get(key)
     except AttributeError:
         key = plan = None  # (not a tensor: the checks say so)
     if plan is None:
         plan = _keep(_rope_plans, key, _rope_plan(x, table, positions, interleaved, axes, inverse, start, out))
     empty, index, dtype, rows, rest = plan
-    _no_grad_needed(x, table, out)
+    if torch.is_grad_enabled() and (x.requires_grad or table.requires_grad):
+        _no_gradient()
     if out is None:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
     if not empty:
@@ -346,8 +346,14 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     qo, ko = (None, None) if out is None else out
     kp, vp = (None, None) if cache is None else cache
     try:
-        key = (_sig(q), _sig(k), _sig(q_weight), _sig(k_weight), _sig(table), _sig(positions), interleaved, axes, start,
-               out_dtype, _sig(qo), _sig(ko), _sig(v), _sig(kp), _sig(vp), _sig(slots))
+        key = (q.dtype, q.shape, q.stride(), q.device, k.dtype, k.shape, k.stride(), k.device,
+               None if q_weight is None else (q_weight.dtype, q_weight.shape, q_weight.stride(), q_weight.device),
+               None if k_weight is None else (k_weight.dtype, k_weight.shape, k_weight.stride(), k_weight.device),
+               None if table is None else (table.dtype, table.shape, table.stride(), table.device),
+               None if positions is None else (positions.dtype, positions.shape, positions.stride(), positions.device),
+               None if out is None else (_sig(qo), _sig(ko)),
+               None if cache is v is slots is None else (_sig(v), _sig(kp), _sig(vp), _sig(slots)),
+               interleaved, axes, start, out_dtype)
         plan = _norm_plans.get(key)
     except AttributeError:
         key = plan = None  # (not a tensor: the checks say so)
@@ -355,14 +361,16 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
         plan = _keep(_norm_plans, key, _norm_plan(q, k, q_weight, k_weight, table, positions, interleaved, axes, start,
                                                   out_dtype, qo, ko, v, cache, slots))
     empty, index, out_dtype, q_shape, k_shape, types, weights, rows, rest, places = plan
-    _no_grad_needed(q, k, q_weight, k_weight, table, qo, ko, v, kp, vp)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or any(
+            t is not None and t.requires_grad for t in (q_weight, k_weight, table, v, kp, vp))):
+        _no_gradient()
     if qo is None:
-        qo = q.new_empty(q_shape, dtype=out_dtype)
+        qo = q.new_empty(q_shape) if out_dtype is q.dtype else q.new_empty(q_shape, dtype=out_dtype)
     if cache is None and ko is None:
-        ko = q.new_empty(k_shape, dtype=out_dtype)
+        ko = q.new_empty(k_shape) if out_dtype is q.dtype else q.new_empty(k_shape, dtype=out_dtype)
     if not empty:
         P = _lib.ptr
         _launch(index, "cast_qk_norm_rope", q.data_ptr(), k.data_ptr(), P(v), *types, P(q_weight), P(k_weight), *weights,
-                eps, P(table), rows, P(positions), *rest, qo.data_ptr(), P(ko if cache is None else kp), P(vp), P(slots),
+                eps, P(table), rows, P(positions), *rest, qo.data_ptr(), (ko if cache is None else kp).data_ptr(), P(vp), P(slots),
                 *places)
     return (qo, ko) if cache is None else (qo, cache)

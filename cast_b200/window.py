@@ -27,7 +27,7 @@ import math
 import torch
 
 from . import _lib
-from .rotary import DTYPES, _check, _check_out, _keep, _launch, _no_grad_needed, _sig, _strides
+from .rotary import DTYPES, _check, _check_out, _keep, _launch, _no_gradient, _sig, _strides
 
 _TYPES = (torch.bfloat16, torch.float16)
 _Twelve = ctypes.c_longlong * 12
@@ -105,14 +105,17 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     and sets the device error word.
     """
     try:
-        key = (_sig(q), _sig(k), _sig(v), window, sinks, frame_tokens, _sig(kv_lens), _sig(out))
+        key = (q.dtype, q.shape, q.stride(), q.device, k.dtype, k.shape, k.stride(), k.device, v.dtype, v.shape,
+               v.stride(), v.device, None if kv_lens is None else _sig(kv_lens), None if out is None else _sig(out),
+               window, sinks, frame_tokens)
         plan = _plans.get(key)
     except AttributeError:
         key = plan = None  # (not a tensor: the checks say so)
     if plan is None:
         plan = _keep(_plans, key, _window_plan(q, k, v, window, sinks, frame_tokens, kv_lens, out))
     empty, blind, index, nbytes, scale, dtype, rest = plan
-    _no_grad_needed(q, k, v, out)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        _no_gradient()
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if empty:
@@ -170,8 +173,10 @@ def paged_window_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     Sessions may share pages (a common prefix).
     """
     try:
-        key = (_sig(q), _sig(k_pages), _sig(v_pages), _sig(block_table), _sig(kv_lens), window, sinks, frame_tokens,
-               _sig(out))
+        key = (q.dtype, q.shape, q.stride(), q.device, k_pages.dtype, k_pages.shape, k_pages.stride(), k_pages.device,
+               v_pages.dtype, v_pages.shape, v_pages.stride(), v_pages.device, block_table.dtype, block_table.shape,
+               block_table.stride(), block_table.device, _sig(kv_lens),
+               None if out is None else _sig(out), window, sinks, frame_tokens)
         plan = _paged_plans.get(key)
     except AttributeError:
         key = plan = None  # (not a tensor: the checks say so)
@@ -179,7 +184,8 @@ def paged_window_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
         plan = _keep(_paged_plans, key, _paged_plan(q, k_pages, v_pages, block_table, kv_lens, window, sinks,
                                                     frame_tokens, out))
     empty, blind, index, nbytes, scale, dtype, pages, rest = plan
-    _no_grad_needed(q, k_pages, v_pages, out)
+    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
+        _no_gradient()
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if empty:
