@@ -1418,6 +1418,8 @@ static int rows_call(castk::RowsParams &p, const RowsPlan &plan, bool paged, int
     return fail(CAST_ERR_UNSUPPORTED, "size outside the kernels' grid");
   p.row_tiles = plan.row_tiles;
   p.n_split = plan.n_split;
+  p.by_tiles.set(p.row_tiles);
+  p.by_split.set(p.n_split);
   p.part = nullptr;
   if (plan.ws_bytes) {
     if (!workspace || workspace_bytes < plan.ws_bytes)
@@ -1447,13 +1449,14 @@ static int rows_params(castk::RowsParams &p, const void *q, const void *k, const
     p.os[i] = strides[9 + i];
   }
   p.kv_lens = kv_lens;
-  // (no key lies 2^31 frames back, so larger windows and sinks are the same)
-  p.rule.window = std::min(window, 1ll << 31);
-  p.rule.sinks = std::min(sinks, 1ll << 31);
-  p.rule.frame = frame;
+  p.rule.set(window, sinks, frame);
   p.B = B, p.Hq = Hq, p.Hk = Hk, p.Lq = Lq, p.lk = Lk;
   p.group = Hq / Hk;
   p.rows = p.group * Lq;
+  p.by_hk.set(Hk);
+  p.by_group.set(p.group);
+  p.by_page.set(1);
+  p.same_strides = p.ks[0] == p.vs[0] && p.ks[1] == p.vs[1] && p.ks[2] == p.vs[2];
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   return CAST_OK;
 }
@@ -1535,7 +1538,7 @@ static int make_map_rows(CUtensorMap *map, const void *base, int dtype, int rank
 static bool tiles_strides_ok(const castk::RowsParams &r) {
   const long long most = 1ll << 38;
   auto ok = [&](long long s, int n, bool shared) { return n == 1 || (s > 0 && s < most) || (shared && s == 0); };
-  return ok(r.qs[0], r.B, false) && ok(r.qs[1], r.Hq, false) && ok(r.qs[2], r.Lq, false) && ok(r.ks[0], r.B, true) &&
+  return ok(r.os[0], r.B, false) && ok(r.os[1], r.Hq, false) && ok(r.os[2], r.Lq, false) && ok(r.qs[0], r.B, false) && ok(r.qs[1], r.Hq, false) && ok(r.qs[2], r.Lq, false) && ok(r.ks[0], r.B, true) &&
          ok(r.ks[1], r.Hk, true) && ok(r.ks[2], r.lk, false) && ok(r.vs[0], r.B, true) && ok(r.vs[1], r.Hk, true) &&
          ok(r.vs[2], r.lk, false);
 }
@@ -1557,19 +1560,23 @@ static int launch_tiles(const castk::RowsParams &r, const TilesPlan &plan, int d
   p.q_tiles = plan.q_tiles;
   p.n_whole = plan.n_whole, p.parts = plan.parts;
   p.scale_log2 = r.scale_log2;
-  const long long sink_keys = std::min<long long>(r.rule.sinks * r.rule.frame, r.lk);
-  p.sinks8 = (int)((sink_keys + 7) / 8 * 8);
+  p.by_tiles.set(p.q_tiles);
+  p.by_groups.set(p.head_groups);
+  p.by_keys.set(p.groups_per_key);
+  p.sinks8 = (std::min(r.rule.sink_keys, r.lk) + 7) / 8 * 8;
   auto many = [](long long stride, int n) { return n > 1 && stride != 0; };
   p.k_batch = many(r.ks[0], r.B), p.k_head = many(r.ks[1], r.Hk);
   p.v_batch = many(r.vs[0], r.B), p.v_head = many(r.vs[1], r.Hk);
 
-  CUtensorMap tm_q, tm_k[3], tm_v[3];
+  CUtensorMap tm_q, tm_o, tm_k[3], tm_v[3];
   int st;
   {
     const uint64_t dims[5] = {(uint64_t)D, (uint64_t)plan.pack, (uint64_t)r.Lq, (uint64_t)plan.head_groups, (uint64_t)r.B};
     const long long str[4] = {r.qs[1], r.qs[2], r.qs[1] * plan.pack, r.qs[0]};
     const uint32_t box[5] = {64, (uint32_t)plan.pack, (uint32_t)(128 / plan.pack), 1, 1};
     if ((st = make_map_rows(&tm_q, r.q, dtype, 5, dims, str, box))) return st;
+    const long long ostr[4] = {r.os[1], r.os[2], r.os[1] * plan.pack, r.os[0]};
+    if ((st = make_map_rows(&tm_o, r.out, dtype, 5, dims, ostr, box))) return st;
   }
   const uint32_t kt = castk::TilesSmem<D>::keys;
   const uint32_t tail = p.sinks8 % kt;
@@ -1603,7 +1610,7 @@ static int launch_tiles(const castk::RowsParams &r, const TilesPlan &plan, int d
     return fail(CAST_ERR_UNSUPPORTED, "window kernel built with %d registers a thread", regs);
   const int cut = plan.n_items - plan.n_whole;
   kernel<<<plan.n_whole + cut * plan.parts, castk::kTilesThreads, smem, s>>>(tm_q, tm_k[0], tm_v[0], tm_k[1], tm_v[1],
-                                                                            tm_k[2], tm_v[2], p);
+                                                                            tm_k[2], tm_v[2], tm_o, p);
   CAST_CUDA_TRY(cudaGetLastError());
   if (cut > 0) {
     castk::window_tiles_join_kernel<T, D><<<cut * (D / castk::kJoinCols), 128 * castk::kJoinGroups, 0, s>>>(p);
@@ -1687,6 +1694,7 @@ extern "C" int cast_paged_window_attention(const void *q, const void *k_pages, c
   if ((st = current_device_sm100(&n_sms))) return st;
   p.block_table = block_table;
   p.page = page, p.max_pages = max_pages, p.n_pages = n_pages;
+  p.by_page.set(page);
   const RowsPlan plan = rows_plan(B, Hk, p.group, Lq, (int)cap, window, sinks, frame_tokens, D, n_sms);
   return rows_call(p, plan, true, dtype, D, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
 }

@@ -17,15 +17,44 @@
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "attention.cuh"
 #include "common.cuh"
 
 namespace castk {
 
 // ------------------------------------------------------------------ masks
+// n / d for 0 <= n < 2^31 by a product: with l = ceil(log2 d),
+// floor(2^(31 + l) / d) + 1 exceeds 2^(31 + l) / d by at most 1, which moves
+// the quotient of n < 2^31 by less than 1 / d (d = 1: n itself).
+struct FastDiv {
+  uint32_t d, mul, shift;
+  void set(uint32_t v) {
+    d = v;
+    uint32_t l = 0;
+    while ((1ull << l) < v) ++l;
+    mul = v == 1 ? 0u : (uint32_t)((1ull << (31 + l)) / v + 1);
+    shift = l - 1;
+  }
+  __device__ __forceinline__ int div(int n) const {
+    return d == 1 ? n : (int)(__umulhi((uint32_t)n, mul) >> shift);
+  }
+};
+
+// Frames, and keys of the sinks; lengths and positions are below 2^30, and so
+// are the numbers here (what is larger means the same as 2^30), so that no
+// bound of a window passes 31 bits.
 struct WindowRule {
-  long long window, sinks;  // in frames
-  int frame;
+  int window, frame, sink_keys;
+  FastDiv by_frame;
+  void set(long long window_frames, long long sink_frames, int frame_tokens) {
+    const long long most = 1ll << 30;
+    window = (int)std::min(window_frames, most);
+    frame = (int)std::min<long long>(frame_tokens, most);
+    sink_keys = (int)std::min(std::min(sink_frames, most) * frame, most);
+    by_frame.set((uint32_t)frame);
+  }
 };
 
 // What the rows of one tile see of a session of `len` keys.
@@ -46,11 +75,10 @@ struct WindowSpan {
 };
 
 __device__ __forceinline__ void window_bounds(const WindowRule &r, int len, int p, int &lo, int &hi) {
-  const long long f = p / r.frame;
-  const long long h = (f + 1) * r.frame;
-  hi = h < len ? (int)h : len;
-  const long long l = f + 1 - r.window;  // first visible frame
-  lo = l <= 0 ? 0 : (int)min(l * r.frame, (long long)len);
+  const int f = r.by_frame.div(p);
+  hi = min((f + 1) * r.frame, len);
+  const int l = f + 1 - r.window;  // first visible frame
+  lo = l <= 0 ? 0 : min(l * r.frame, len);
 }
 
 // Rows i0 .. i1 (inclusive) of lq queries.
@@ -58,7 +86,7 @@ __device__ __forceinline__ WindowSpan window_span(const WindowRule &r, int len, 
   WindowSpan s;
   s.len = len;
   s.lq = lq;
-  s.sinks = (int)min(r.sinks * r.frame, (long long)len);
+  s.sinks = min(r.sink_keys, len);
   s.s_n = s.base = s.n = s.lo0 = s.hi0 = s.lo1 = s.hi1 = 0;
   s.unplaced = len - lq + i0 < 0;
   const int p1 = len - lq + i1;
@@ -179,6 +207,8 @@ struct RowsParams {
   int page, max_pages, n_pages;
   int group, rows, row_tiles;            // rows = group * Lq of one key head
   int n_split;
+  int same_strides;                      // k and v have the same
+  FastDiv by_split, by_tiles, by_hk, by_group, by_page;
   float scale_log2;
 };
 
@@ -266,11 +296,9 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
   extern __shared__ __align__(1024) uint8_t smem_rows[];
   __shared__ int flag_bad;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = blockIdx.x % p.n_split;
-  const int item = blockIdx.x / p.n_split;
-  const int rt = item % p.row_tiles;
-  const int bh = item / p.row_tiles;
-  const int b = bh / p.Hk, hk = bh - b * p.Hk;
+  const int item = p.by_split.div(blockIdx.x), split = blockIdx.x - item * p.n_split;
+  const int bh = p.by_tiles.div(item), rt = item - bh * p.row_tiles;
+  const int b = p.by_hk.div(bh), hk = bh - b * p.Hk;
   const int r0 = rt * R;  // first row: token r / group, head r % group
   const int r_end = min(p.rows, r0 + R);
   int len = p.kv_lens ? p.kv_lens[b] : p.lk;
@@ -278,11 +306,11 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
     if (threadIdx.x == 0) atomicExch(&g_cast_device_error, (int)CAST_ERR_INVALID_ARGUMENT);
     len = min(max(len, 0), p.lk);
   }
-  const WindowSpan span = window_span(p.rule, len, p.Lq, r0 / p.group, (r_end - 1) / p.group);
+  const WindowSpan span = window_span(p.rule, len, p.Lq, p.by_group.div(r0), p.by_group.div(r_end - 1));
   const int groups = (span.n + 15) / 16;
-  // this CTA's groups of 16 keys
-  const int g_lo = (int)((long long)groups * split / p.n_split);
-  const int g_hi = (int)((long long)groups * (split + 1) / p.n_split);
+  // this CTA's groups of 16 keys: an equal share, the first ones one more
+  const int share = p.by_split.div(groups), more = groups - share * p.n_split;
+  const int g_lo = split * share + min(split, more), g_hi = g_lo + share + (split < more ? 1 : 0);
   const bool partial = span.lo0 != span.lo1 || span.hi0 != span.hi1 || span.unplaced;
   if (threadIdx.x == 0) flag_bad = 0;
   if (p.n_split > 1 && !p.part) cluster_arrive();  // (waited for before the first push)
@@ -296,7 +324,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
     for (int hh = 0; hh < 2; ++hh) {
       const int r = r0 + 16 * mt + lane / 4 + 8 * hh;
       const bool on = r < r_end;
-      const int i = r / p.group, g = r - i * p.group;
+      const int i = p.by_group.div(r), g = r - i * p.group;
       const T *src = static_cast<const T *>(p.q) + b * p.qs[0] + (long long)(hk * p.group + g) * p.qs[1] + (long long)i * p.qs[2];
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) {
@@ -312,7 +340,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
       const int r = r0 + 16 * mt + lane / 4 + 8 * hh;
-      const int pos = len - p.Lq + r / p.group;
+      const int pos = len - p.Lq + p.by_group.div(r);
       lo[mt][hh] = hi[mt][hh] = 0;
       if (r < r_end && pos >= 0) window_bounds(p.rule, len, pos, lo[mt][hh], hi[mt][hh]);
     }
@@ -333,46 +361,54 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
   const T *kbase = static_cast<const T *>(p.k) + (kPaged ? 0 : b * p.ks[0]) + hk * p.ks[1];
   const T *vbase = static_cast<const T *>(p.v) + (kPaged ? 0 : b * p.vs[0]) + hk * p.vs[1];
 
-  // Page of this lane's key (lane % 16) of group g; -1: no key there.
-  auto page_of = [&](int g) -> int {
-    const int v = 16 * g + (lane & 15);
-    if (g >= g_hi || v >= span.n) return -1;
-    if (!kPaged) return 0;
-    const int pg = __ldg(p.block_table + (long long)b * p.max_pages + span.key(v) / p.page);
-    if (pg < 0 || pg >= p.n_pages) {
-      atomicExch(&g_cast_device_error, (int)CAST_ERR_INVALID_ARGUMENT);
-      return -1;
-    }
-    return pg;
+  // Where key lane % 16 of group g lies (nullptr: no key there).  A lane works
+  // out one key, a group ahead, and its row's copies take the pointer from it.
+  struct Place {
+    const T *k, *v;
   };
-  // Starts the copies of group g into stage st; returns a bit for each of the
-  // 16 keys that are there.
-  auto start = [&](int g, int st, int pg) -> uint32_t {
+  auto place_of = [&](int g) -> Place {
+    Place at{nullptr, nullptr};
     const int v = 16 * g + (lane & 15);
-    long long ko = 0, vo = 0;
-    if (pg >= 0) {
-      const int key = span.key(v);
-      if (kPaged) {
-        const int in = key % p.page;
-        ko = pg * p.ks[0] + in * p.ks[2];
-        vo = pg * p.vs[0] + in * p.vs[2];
-      } else {
-        ko = key * p.ks[2];
-        vo = key * p.vs[2];
+    if (g >= g_hi || v >= span.n) return at;
+    const int key = span.key(v);
+    long long ko, vo;
+    if (kPaged) {
+      const int pg_at = p.by_page.div(key), in = key - pg_at * p.page;
+      const int pg = __ldg(p.block_table + (long long)b * p.max_pages + pg_at);
+      if (pg < 0 || pg >= p.n_pages) {
+        atomicExch(&g_cast_device_error, (int)CAST_ERR_INVALID_ARGUMENT);
+        return at;
       }
+      ko = pg * p.ks[0] + in * p.ks[2];
+      vo = p.same_strides ? ko : pg * p.vs[0] + in * p.vs[2];
+    } else {
+      ko = key * p.ks[2];
+      vo = p.same_strides ? ko : key * p.vs[2];
     }
-    const uint32_t there = __ballot_sync(0xffffffffu, pg >= 0) & 0xFFFFu;
+    at.k = kbase + ko;
+    at.v = vbase + vo;
+    return at;
+  };
+  // Starts the copies of a group into stage st; returns a bit for each of the
+  // 16 keys that are there.
+  const ptrdiff_t v_from_k = reinterpret_cast<const char *>(vbase) - reinterpret_cast<const char *>(kbase);
+  auto start = [&](int st, const Place &at) -> uint32_t {
+    const uint32_t there = __ballot_sync(0xffffffffu, at.k != nullptr) & 0xFFFFu;
     const uint32_t dst = ring + st * 2 * S::group_bytes;
     constexpr int kRowsPer = 32 / kChunks;  // rows a pass of the warp covers
     const int c = lane % kChunks;
+    const unsigned long long mine = reinterpret_cast<unsigned long long>(at.k ? at.k : kbase);
+    const unsigned long long mine_v = reinterpret_cast<unsigned long long>(at.k ? at.v : vbase);
 #pragma unroll
     for (int i = 0; i < 16 / kRowsPer; ++i) {
       const int row = i * kRowsPer + lane / kChunks;
-      const long long kr = __shfl_sync(0xffffffffu, ko, row), vr = __shfl_sync(0xffffffffu, vo, row);
       const bool live = (there >> row) & 1u;
+      const char *kr = reinterpret_cast<const char *>(__shfl_sync(0xffffffffu, mine, row)) + 16 * c;
+      const char *vr = p.same_strides ? kr + v_from_k
+                                      : reinterpret_cast<const char *>(__shfl_sync(0xffffffffu, mine_v, row)) + 16 * c;
       const uint32_t off = row * S::row_bytes + ((c ^ (row & 7)) * 16);
-      cp_async16(dst + off, kbase + kr + 8 * c, live);
-      cp_async16(dst + S::group_bytes + off, vbase + vr + 8 * c, live);
+      cp_async16(dst + off, kr, live);
+      cp_async16(dst + S::group_bytes + off, vr, live);
     }
     return there;
   };
@@ -380,13 +416,12 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
   // groups g_lo + warp + kRowsWarps * t of this warp
   const int first = g_lo + warp;
   uint32_t there[kRowsStages];
-  int next_page = page_of(first);
+  Place next = place_of(first);
 #pragma unroll
   for (int st = 0; st < kRowsStages - 1; ++st) {
-    const int g = first + kRowsWarps * st;
-    const int pg = next_page;
-    next_page = page_of(g + kRowsWarps);
-    there[st] = start(g, st, pg);
+    const Place at = next;
+    next = place_of(first + kRowsWarps * (st + 1));
+    there[st] = start(st, at);
     cp_async_commit();
   }
   there[kRowsStages - 1] = 0;
@@ -398,10 +433,10 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
     cp_async_wait<kRowsStages - 2>();
     __syncwarp();
     {  // the stage read in the last step is free: start the group it takes
-      const int gn = g + kRowsWarps * (kRowsStages - 1), sn = (t + kRowsStages - 1) % kRowsStages;
-      const int pg = next_page;
-      next_page = page_of(gn + kRowsWarps);
-      const uint32_t bits = start(gn, sn, pg);
+      const int sn = (t + kRowsStages - 1) % kRowsStages;
+      const Place at = next;
+      next = place_of(g + kRowsWarps * kRowsStages);
+      const uint32_t bits = start(sn, at);
       cp_async_commit();
 #pragma unroll
       for (int x = 0; x < kRowsStages; ++x)
@@ -432,6 +467,11 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
         }
       }
     }
+    // Whether every row sees every key of the group (sinks and window never
+    // share one then).
+    const int k_first = span.key(16 * g), k_last = span.key(16 * g + 15);
+    const bool whole = mine == 0xFFFFu && !span.unplaced && k_last - k_first == 15 &&
+                       (k_last < min(span.sinks, span.hi0) || (k_first >= span.lo1 && k_last < span.hi0));
     // keys of this lane's four columns: 2 (lane % 4) + {0, 1, 8, 9}
     int key[4];
     uint32_t col_there = 0;
@@ -451,7 +491,8 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           float &v = s[mt][c >> 1][2 * hh + (c & 1)];
-          const bool on = ((col_there >> c) & 1u) && window_sees(key[c], lo[mt][hh], hi[mt][hh], span.sinks) && hi[mt][hh] > 0;
+          const bool on = whole || (((col_there >> c) & 1u) && window_sees(key[c], lo[mt][hh], hi[mt][hh], span.sinks) &&
+                                    hi[mt][hh] > 0);
           v = on ? v * p.scale_log2 : -INFINITY;
           x = fmaxf(x, v);
         }
@@ -484,7 +525,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
         }
       }
     }
-    if (partial) {
+    if (partial && !whole) {
       // A key that only some rows of the tile see: its value meets a zero
       // weight in the others, so an infinity or NaN there is taken out here
       // and given back to the rows that see it at the end.

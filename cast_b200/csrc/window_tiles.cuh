@@ -76,6 +76,7 @@ struct TilesParams {
   int groups_per_key;    // head groups that share a key head
   int rows, q_tiles;     // rows = pack * Lq of one head group
   int n_whole, parts;    // items [0, n_whole) whole, the later ones in `parts` parts each
+  FastDiv by_tiles, by_groups, by_keys;  // q_tiles, head_groups, groups_per_key
   int sinks8;            // sinks of a session long enough to have a gap, rounded up to 8
   int k_batch, k_head, v_batch, v_head;  // 0 where that dimension's stride is 0 (one box for all), else 1
   float scale_log2;
@@ -122,6 +123,15 @@ __device__ __forceinline__ void tma_load_5d(void *dst, const CUtensorMap *map, u
       "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(castdev::smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(castdev::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_store_5d(const CUtensorMap *map, const void *src, int c0, int c1, int c2, int c3,
+                                             int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5, %6}], [%1];" ::"l"(
+          reinterpret_cast<uint64_t>(map)),
+      "r"(castdev::smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
       : "memory");
 }
 
@@ -229,7 +239,8 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
     window_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_k_sink,
                         const __grid_constant__ CUtensorMap tm_v_sink, const __grid_constant__ CUtensorMap tm_k_rest,
-                        const __grid_constant__ CUtensorMap tm_v_rest, const __grid_constant__ TilesParams p) {
+                        const __grid_constant__ CUtensorMap tm_v_rest, const __grid_constant__ CUtensorMap tm_o,
+                        const __grid_constant__ TilesParams p) {
   using S = TilesSmem<D>;
   using X = TilesType<T>;
   constexpr int KT = S::keys;
@@ -256,10 +267,10 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
     x = p.n_whole + (x - p.n_whole) / p.parts;
     n_parts = p.parts;
   }
-  const int bhg = x / p.q_tiles;
+  const int bhg = p.by_tiles.div(x);
   const int qt = p.q_tiles - 1 - (x - bhg * p.q_tiles);  // later rows see more keys: first
-  const int b = bhg / p.head_groups, hg = bhg - b * p.head_groups;
-  const int hk = hg / p.groups_per_key;
+  const int b = p.by_groups.div(bhg), hg = bhg - b * p.head_groups;
+  const int hk = p.by_keys.div(hg);
   const int row0 = qt * 128, row_end = min(p.rows, row0 + 128);
   int len = p.kv_lens ? p.kv_lens[b] : p.lk;
   if (len < 0 || len > p.lk) {  // a session longer than its keys: nothing past them is read
@@ -271,33 +282,13 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
   const int s8 = span.s_n > 0 ? p.sinks8 : 0;
   const int n_places = span.n - span.s_n + s8;
   const int n_tiles = span.n > 0 ? (n_places + KT - 1) / KT : 0;
-  const int kt_lo = (int)((long long)part * n_tiles / n_parts);
-  const int n_kv = (int)((long long)(part + 1) * n_tiles / n_parts) - kt_lo;
+  int kt_lo = 0, n_kv = n_tiles;
+  if (n_parts > 1) {  // an equal share, the first parts one more
+    const int share = n_tiles / n_parts, more = n_tiles - share * n_parts;
+    kt_lo = part * share + min(part, more);
+    n_kv = share + (part < more ? 1 : 0);
+  }
   constexpr int kKWarp = 4, kMWarp = 5, kVWarp = 6;
-
-  if (warp == kKWarp && lane == 0) {
-    *err = 0;
-    *bad_flag = 0;
-    for (int i = 0; i < S::n_bars; ++i) castdev::mbar_init(&bar[i], 1);
-    for (int i = 0; i < 2; ++i) castdev::mbar_init(&p_full[i], 4);
-    castdev::fence_barrier_init();
-    castdev::tma_prefetch_desc(&tm_q);
-    castdev::tma_prefetch_desc(&tm_k);
-    castdev::tma_prefetch_desc(&tm_v);
-    if (n_kv > 0) {
-      castdev::mbar_arrive_expect_tx(q_full, S::q_tile);
-#pragma unroll
-      for (int h = 0; h < D / 64; ++h)
-        tma_load_5d(smem + h * 16384, &tm_q, q_full, 64 * h, 0, row0 >> p.pack_log2, hg, b);
-    }
-  }
-  if (warp == kMWarp) {
-    castdev::tmem_alloc(tmem_slot, 256);
-    castdev::tmem_relinquish();
-  }
-  __syncthreads();
-  castdev::tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
 
   // Starts the copies of the tile of KT places from place n0 on.
   auto start = [&](uint8_t *dst, uint64_t *full, int n0, const CUtensorMap *whole, const CUtensorMap *sink,
@@ -316,17 +307,61 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
     }
   };
 
+  // Whether some row does not see some key of the tile from place n0 on (what
+  // all rows see are one or two intervals of places).
+  auto ragged = [&](int n0) {
+    if (span.unplaced || n0 + KT > n_places) return true;
+    const int a = min(span.sinks, span.hi0), l = s8 + span.lo1 - span.base, h = s8 + span.hi0 - span.base;
+    return !(n0 + KT <= a || (n0 >= l && n0 + KT <= h) || (a >= l && n0 + KT <= h));
+  };
+  auto issue_k = [&](int j) {
+    castdev::mbar_arrive_expect_tx(&k_full[j & 1], S::tile);
+    start(smem + S::k_off + (j & 1) * S::tile, &k_full[j & 1], (kt_lo + j) * KT, &tm_k, &tm_k_sink, &tm_k_rest,
+          hk * p.k_head, b * p.k_batch);
+  };
+  auto issue_v = [&](int j) {
+    uint64_t *full = ragged((kt_lo + j) * KT) ? &v_raw[j & 1] : &v_full[j & 1];
+    castdev::mbar_arrive_expect_tx(full, S::tile);
+    start(smem + S::v_off + (j & 1) * S::tile, full, (kt_lo + j) * KT, &tm_v, &tm_v_sink, &tm_v_rest, hk * p.v_head,
+          b * p.v_batch);
+  };
+
+  if (warp == kKWarp && lane == 0) {
+    *err = 0;
+    *bad_flag = 0;
+    for (int i = 0; i < S::n_bars; ++i) castdev::mbar_init(&bar[i], 1);
+    for (int i = 0; i < 2; ++i) castdev::mbar_init(&p_full[i], 4);
+    castdev::fence_barrier_init();
+    castdev::tma_prefetch_desc(&tm_q);
+    castdev::tma_prefetch_desc(&tm_k);
+    castdev::tma_prefetch_desc(&tm_v);
+    if (n_kv > 0) {
+      castdev::mbar_arrive_expect_tx(q_full, S::q_tile);
+#pragma unroll
+      for (int h = 0; h < D / 64; ++h)
+        tma_load_5d(smem + h * 16384, &tm_q, q_full, 64 * h, 0, row0 >> p.pack_log2, hg, b);
+      for (int j = 0; j < min(n_kv, 2); ++j) {  // both rings, before the block meets
+        issue_k(j);
+        issue_v(j);
+      }
+    }
+  }
+  if (warp == kMWarp) {
+    castdev::tmem_alloc(tmem_slot, 256);
+    castdev::tmem_relinquish();
+  }
+  __syncthreads();
+  castdev::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
   if (warp >= 4) {
     regs_dec<kTilesRegsRest>();
     if (warp == kKWarp) {
       if (lane == 0 && n_kv > 0) {
-        int issued = 0;
-        for (int j = 0; j < n_kv; ++j) {
-          const int n0 = (kt_lo + j) * KT, ks = j & 1;
-          if (j >= 2 && !castdev::mbar_wait(&s_full[ks], ((j >> 1) - 1) & 1, err)) break;
-          castdev::mbar_arrive_expect_tx(&k_full[ks], S::tile);
-          start(smem + S::k_off + ks * S::tile, &k_full[ks], n0, &tm_k, &tm_k_sink, &tm_k_rest, hk * p.k_head,
-                b * p.k_batch);
+        int issued = min(n_kv, 2);
+        for (int j = 2; j < n_kv; ++j) {  // (the stage is free when S of step j - 2 is done)
+          if (!castdev::mbar_wait(&s_full[j & 1], ((j >> 1) - 1) & 1, err)) break;
+          issue_k(j);
           issued = j + 1;
         }
         castdev::mbar_wait_drain(q_full, 0, err);
@@ -339,12 +374,6 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
       // every row sees place n (sinks and the keys of all rows)
       auto all_see = [&](int n) {
         return !span.unplaced && (n < min(span.sinks, span.hi0) || (n >= s8 + span.lo1 - span.base && n < s8 + span.hi0 - span.base));
-      };
-      // (both ends of a run of KT places: visible ones are one or two intervals)
-      auto ragged = [&](int n0) {
-        if (span.unplaced || n0 + KT > n_places) return true;
-        const int a = min(span.sinks, span.hi0), l = s8 + span.lo1 - span.base, h = s8 + span.hi0 - span.base;
-        return !(n0 + KT <= a || (n0 >= l && n0 + KT <= h) || (a >= l && n0 + KT <= h));
       };
       auto go_over = [&](int j) -> bool {
         const int n0 = (kt_lo + j) * KT, vs = j & 1;
@@ -401,23 +430,15 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
         if (lane == 0) castdev::mbar_arrive(&v_full[vs]);
         return true;
       };
-      int issued = 0, looked = 0;  // tiles started; tiles gone over
+      int issued = min(n_kv, 2), looked = 0;  // tiles started; tiles gone over
       bool ok = true;
-      auto issue = [&](int j) {
-        const int n0 = (kt_lo + j) * KT, vs = j & 1;
-        uint64_t *full = ragged(n0) ? &v_raw[vs] : &v_full[vs];
-        if (lane == 0) {
-          castdev::mbar_arrive_expect_tx(full, S::tile);
-          start(smem + S::v_off + vs * S::tile, full, n0, &tm_v, &tm_v_sink, &tm_v_rest, hk * p.v_head, b * p.v_batch);
-        }
-        issued = j + 1;
-      };
-      if (n_kv > 1) issue(0);
       for (int j = 0; ok && j < n_kv; ++j) {
-        if (j >= 2) ok = __all_sync(0xffffffffu, castdev::mbar_wait(&pv_done[j & 1], ((j >> 1) - 1) & 1, err));
-        if (!ok) break;
-        const int next = j == 0 && n_kv > 1 ? 1 : j;  // the first two are started together
-        if (next >= issued) issue(next);
+        if (j >= 2) {  // (the stage is free when P V of step j - 2 is done)
+          ok = __all_sync(0xffffffffu, castdev::mbar_wait(&pv_done[j & 1], ((j >> 1) - 1) & 1, err));
+          if (!ok) break;
+          if (lane == 0) issue_v(j);
+          issued = j + 1;
+        }
         if (ragged((kt_lo + j) * KT)) ok = go_over(j);
         if (ok) looked = j + 1;
       }
@@ -564,7 +585,9 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
       if (n_parts == 1) {
         if (ok) {
           const float inv = l_run != 0.0f ? 1.0f / l_run : 0.0f;  // (a NaN sum stays one)
-          T *dst = static_cast<T *>(p.out) + b * p.os[0] + head * p.os[1] + token * p.os[2];
+          // Rows go to the Q tile's place in shared memory, swizzled as the
+          // map wants them (no product reads Q any more), and out by one copy,
+          // which leaves out rows past the last token.
 #pragma unroll 1
           for (int cc = 0; cc < D / 32; ++cc) {
             uint32_t o[32];
@@ -573,21 +596,27 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
             float y[32];
 #pragma unroll
             for (int c = 0; c < 32; ++c) y[c] = hi > 0 ? __uint_as_float(o[c]) * inv : 0.0f;
-            if (row_valid) {
-              if (__builtin_expect(bad, 0)) {
-                float z[32];
-                for (int c = 0; c < 32; ++c) z[c] = y[c];
-                tiles_give_back<T>(p, span, b, hk, lo, hi, 32 * cc, z);
-                for (int c = 0; c < 32; ++c) y[c] = z[c];
-              }
-              uint4 w[4];
-              uint32_t *wp = reinterpret_cast<uint32_t *>(w);
-#pragma unroll
-              for (int c = 0; c < 16; ++c) wp[c] = X::pack(y[2 * c], y[2 * c + 1]);
-#pragma unroll
-              for (int c = 0; c < 4; ++c) reinterpret_cast<uint4 *>(dst + 32 * cc)[c] = w[c];
+            if (__builtin_expect(bad, 0) && row_valid) {
+              float z[32];
+              for (int c = 0; c < 32; ++c) z[c] = y[c];
+              tiles_give_back<T>(p, span, b, hk, lo, hi, 32 * cc, z);
+              for (int c = 0; c < 32; ++c) y[c] = z[c];
             }
+            uint8_t *line = smem + (cc >> 1) * 16384 + lrow * 128;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              *reinterpret_cast<uint4 *>(line + (((4 * (cc & 1) + c) ^ (lrow & 7)) * 16)) =
+                  make_uint4(X::pack(y[8 * c], y[8 * c + 1]), X::pack(y[8 * c + 2], y[8 * c + 3]),
+                             X::pack(y[8 * c + 4], y[8 * c + 5]), X::pack(y[8 * c + 6], y[8 * c + 7]));
           }
+        }
+        castdev::fence_proxy_async_smem();
+        castdev::named_bar_sync(1, 128);
+        if (threadIdx.x == 0 && ok) {
+#pragma unroll
+          for (int h = 0; h < D / 64; ++h) tma_store_5d(&tm_o, smem + h * 16384, 64 * h, 0, row0 >> p.pack_log2, hg, b);
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         }
       } else if (ok) {
         // this part's O, maximum and sum: [tile][column][row], then [tile][m, l, flag][row]
