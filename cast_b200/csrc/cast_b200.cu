@@ -1324,24 +1324,25 @@ struct RowsPlan {
   size_t ws_bytes = 0;
 };
 
-// How the few-row kernel cuts a call.  Two of its CTAs fit on an SM and a CTA
-// keeps 48 KB of copies in flight, so the keys of a tile of rows are split
-// until there are two CTAs for each SM, or until a part has 128 keys (two
-// groups of 16 for each of its warps).  Up to eight parts are joined in a
-// cluster; more go through the workspace.
+// How the few-row kernel cuts a call.  Two of its CTAs fit on an SM, so the
+// keys of a tile of rows are split until there are two CTAs for each SM, or
+// until a part has 128 keys (little more than one step of its warps).  More
+// and smaller parts lose: 16 sessions x 8 key heads take 80.6 us in 2 parts
+// each, 85.4 in 4; 64 x 8 take 160 in 1, 173 in 2.  Up to eight parts are
+// joined in a cluster; more go through the workspace.
 static RowsPlan rows_plan(long long B, int Hk, int group, int Lq, int capacity, long long window,
                           long long sinks, int frame, int D, int n_sms) {
   RowsPlan r;
   const long long rows = (long long)group * Lq;
-  r.mt = rows <= 16 ? 1 : 2;
-  r.row_tiles = (int)((rows + 16 * r.mt - 1) / (16 * r.mt));
+  r.mt = rows <= 8 ? 0 : (rows <= 16 ? 1 : 2);
+  const int tile = r.mt == 0 ? 8 : 16 * r.mt;
+  r.row_tiles = (int)((rows + tile - 1) / tile);
   const long long items = B * Hk * r.row_tiles;
-  const long long tokens = std::min<long long>(Lq, 16 * r.mt / group + 2);
+  const long long tokens = std::min<long long>(Lq, tile / group + 2);
   const double span = std::min<double>(capacity, (double)(window + sinks + 1) * frame + (double)tokens);
   const long long most = std::max<long long>(1, (long long)(span / 128));
   const long long want = std::max<long long>(1, 2ll * n_sms / items);
   long long n = std::min(most, want);
-  { static const char *e = getenv("CAST_ROWS_SPLIT"); if (e) n = std::min<long long>(std::max<long long>(1,(long long)(span/16)), atoi(e)); }
   if (n <= castk::kRowsMaxCluster) {
     long long c = 1;
     while (2 * c <= n) c *= 2;
@@ -1349,7 +1350,7 @@ static RowsPlan rows_plan(long long B, int Hk, int group, int Lq, int capacity, 
     r.cluster = c > 1;
   } else {
     r.n_split = (int)n;
-    r.ws_bytes = (size_t)items * n * (16 * r.mt) * (D + 4) * sizeof(float);
+    r.ws_bytes = (size_t)items * n * tile * (D + 4) * sizeof(float);
   }
   return r;
 }
@@ -1386,16 +1387,17 @@ static int launch_rows(const castk::RowsParams &p, const RowsPlan &plan, cudaStr
   return CAST_OK;
 }
 
+template <typename T, int D, bool kPaged>
+static int launch_rows(const castk::RowsParams &p, const RowsPlan &plan, cudaStream_t s) {
+  if (plan.mt == 0) return launch_rows<T, D, 0, kPaged>(p, plan, s);
+  return plan.mt == 1 ? launch_rows<T, D, 1, kPaged>(p, plan, s) : launch_rows<T, D, 2, kPaged>(p, plan, s);
+}
+
 template <bool kPaged>
 static int launch_rows(const castk::RowsParams &p, const RowsPlan &plan, int dtype, int D, cudaStream_t s) {
-  using bf16 = __nv_bfloat16;
-  if (dtype == kBf16 && D == 128)
-    return plan.mt == 1 ? launch_rows<bf16, 128, 1, kPaged>(p, plan, s) : launch_rows<bf16, 128, 2, kPaged>(p, plan, s);
   if (dtype == kBf16)
-    return plan.mt == 1 ? launch_rows<bf16, 64, 1, kPaged>(p, plan, s) : launch_rows<bf16, 64, 2, kPaged>(p, plan, s);
-  if (D == 128)
-    return plan.mt == 1 ? launch_rows<__half, 128, 1, kPaged>(p, plan, s) : launch_rows<__half, 128, 2, kPaged>(p, plan, s);
-  return plan.mt == 1 ? launch_rows<__half, 64, 1, kPaged>(p, plan, s) : launch_rows<__half, 64, 2, kPaged>(p, plan, s);
+    return D == 128 ? launch_rows<__nv_bfloat16, 128, kPaged>(p, plan, s) : launch_rows<__nv_bfloat16, 64, kPaged>(p, plan, s);
+  return D == 128 ? launch_rows<__half, 128, kPaged>(p, plan, s) : launch_rows<__half, 64, kPaged>(p, plan, s);
 }
 
 static int window_dims_ok(int B, int Hq, int Hk, int Lq, int Lk, int D, long long window, long long sinks,

@@ -176,6 +176,13 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4
                : "r"(addr)
                : "memory");
 }
+// An 8 x 8 matrix of 16-bit values over the warp (row lane / 4, columns
+// 2 (lane % 4), + 1), transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t u) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(u));
+  return r;
+}
 // 16 bytes global -> shared, zeros where !live (nothing is read then).
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool live) {
   const int bytes = live ? 16 : 0;
@@ -191,8 +198,13 @@ __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // --------------------------------------------------------------- few rows
-constexpr int kRowsWarps = 4;
-constexpr int kRowsStages = 3;
+// Warps of a CTA and stages of each warp's ring.  A warp's step is a chain of
+// latencies (products, shuffles, exponentials), so warps count for more than
+// copies far ahead: six warps of two stages, two CTAs an SM (96 KB each), take
+// 80.6 us for 16 sessions x 8 key heads x 8208 keys of 128 (the copy rate);
+// four of three 81.5, four of two (three CTAs) 87.2, eight of two 87.6.
+constexpr int kRowsWarps = 6;
+constexpr int kRowsStages = 2;
 constexpr int kRowsMaxCluster = 8;
 
 struct RowsParams {
@@ -212,22 +224,25 @@ struct RowsParams {
   float scale_log2;
 };
 
-// One CTA: rows 16 MT of one (session, key head), part `split` of their
+// One CTA: a tile of rows of one (session, key head), part `split` of their
 // virtual keys.  Each of its warps takes every kRowsWarps-th group of 16 keys
 // through a ring of its own in shared memory (cp.async, no CTA barrier in the
-// loop): S = Q K^T and O += P V are m16n8k16 products whose rows are the query
-// heads that share the key head, so a key is read once for all of them.  The
-// warps' results are joined in shared memory, the CTAs' through distributed
-// shared memory of a cluster, or, for more parts than a cluster has, from
-// `part` by window_rows_join_kernel.  The order of every sum is fixed.
+// loop).  The products are m16n8k16 ones whose rows are the query heads that
+// share the key head, so a key is read once for all of them: S = Q K^T and
+// O += P V over 16 MT rows, or, for at most 8 rows (MT 0, most single tokens),
+// S^T = K Q^T and O^T += V^T P^T, half as many products.  The warps' results
+// are joined in shared memory, the CTAs' through distributed shared memory of
+// a cluster, or, for more parts than a cluster has, from `part` by
+// window_rows_join_kernel.  The order of every sum is fixed.
 template <typename T, int D, int MT, bool kPaged>
 struct RowsSmem {
   static constexpr int row_bytes = D * 2;
   static constexpr int group_bytes = 16 * row_bytes;               // 16 keys of K or V
   static constexpr int warp_bytes = kRowsStages * 2 * group_bytes;
   static constexpr int ring = kRowsWarps * warp_bytes;
-  static constexpr int join = kRowsWarps * 16 * MT * (D + 4) * 4;  // O, m, l of each warp
-  static constexpr int bytes = (ring > join ? ring : join) + 16 * MT * (D + 4) * 4;  // + the CTA's own
+  static constexpr int rows = MT == 0 ? 8 : 16 * MT;
+  static constexpr int join = kRowsWarps * rows * (D + 4) * 4;                  // O, m, l of each warp
+  static constexpr int bytes = (ring > join ? ring : join) + rows * (D + 4) * 4;  // + the CTA's box
 };
 
 // Where a value of a virtual key lies (nullptr: its page is not one).
@@ -292,7 +307,9 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
   using S = RowsSmem<T, D, MT, kPaged>;
   using H2 = Half2<T>;
   constexpr int kChunks = D / 8;  // 16-byte pieces of a row
-  constexpr int R = 16 * MT;
+  constexpr int R = S::rows;
+  constexpr bool kSwap = MT == 0;
+  constexpr int M = kSwap ? 1 : MT;
   extern __shared__ __align__(1024) uint8_t smem_rows[];
   __shared__ int flag_bad;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -317,11 +334,12 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
   __syncthreads();
 
   // ---- Q fragments: row r = lane / 4 (+ 8), columns 2 (lane % 4) (+ 8) of each 16
-  uint32_t qf[MT][D / 16][4];
+  // (kSwap: as the second operand, row lane / 4 alone)
+  uint32_t qf[M][D / 16][kSwap ? 2 : 4];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
+  for (int mt = 0; mt < M; ++mt) {
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
+    for (int hh = 0; hh < (kSwap ? 1 : 2); ++hh) {
       const int r = r0 + 16 * mt + lane / 4 + 8 * hh;
       const bool on = r < r_end;
       const int i = p.by_group.div(r), g = r - i * p.group;
@@ -329,28 +347,31 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) {
         qf[mt][s][hh] = on ? *reinterpret_cast<const uint32_t *>(src + 16 * s + 2 * (lane % 4)) : 0u;
-        qf[mt][s][2 + hh] = on ? *reinterpret_cast<const uint32_t *>(src + 16 * s + 8 + 2 * (lane % 4)) : 0u;
+        qf[mt][s][(kSwap ? 1 : 2) + hh] = on ? *reinterpret_cast<const uint32_t *>(src + 16 * s + 8 + 2 * (lane % 4)) : 0u;
       }
     }
   }
-  // what each of this lane's rows sees
-  int lo[MT][2], hi[MT][2];
+  // The two rows of each product tile whose scores this lane holds, and what they see.
+  auto own_row = [&](int mt, int hh) { return kSwap ? 2 * (lane % 4) + hh : 16 * mt + lane / 4 + 8 * hh; };
+  int lo[M][2], hi[M][2];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int mt = 0; mt < M; ++mt)
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
-      const int r = r0 + 16 * mt + lane / 4 + 8 * hh;
+      const int r = r0 + own_row(mt, hh);
       const int pos = len - p.Lq + p.by_group.div(r);
       lo[mt][hh] = hi[mt][hh] = 0;
       if (r < r_end && pos >= 0) window_bounds(p.rule, len, pos, lo[mt][hh], hi[mt][hh]);
     }
 
-  float o[MT][D / 8][4];
-  float m_run[MT][2], l_run[MT][2];
+  // O: [16 rows][8 columns] tiles, or (kSwap) [16 columns][8 rows] ones
+  constexpr int kOut = kSwap ? D / 16 : D / 8;
+  float o[M][kOut][4];
+  float m_run[M][2], l_run[M][2];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
+  for (int mt = 0; mt < M; ++mt) {
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j)
+    for (int j = 0; j < kOut; ++j)
 #pragma unroll
       for (int c = 0; c < 4; ++c) o[mt][j][c] = 0.0f;
     m_run[mt][0] = m_run[mt][1] = -INFINITY;
@@ -448,20 +469,30 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
       if (x == st) mine = there[x];
     const uint32_t ks = ring + st * 2 * S::group_bytes, vs = ks + S::group_bytes;
 
-    // S = Q K^T of 16 keys
-    float s[MT][2][4];
+    // S = Q K^T of 16 keys; s[mt][..][..]: this lane's two rows by four keys
+    float s[M][2][4];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int mt = 0; mt < M; ++mt)
 #pragma unroll
       for (int c = 0; c < 4; ++c) s[mt][0][c] = s[mt][1][c] = 0.0f;
-    {
+    if constexpr (kSwap) {  // S^T = K Q^T, two chains over the columns
+      const int row = (lane & 7) + (((lane >> 3) & 1) << 3), cc = lane >> 4;
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        uint32_t kf[4];
+        ldmatrix_x4(ks + row * S::row_bytes + (((2 * j + cc) ^ (row & 7)) * 16), kf);
+        H2::mma(s[0][j & 1], kf, qf[0][j][0], qf[0][j][1]);
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[0][0][c] += s[0][1][c];
+    } else {
       const int row = (lane & 7) + ((lane >> 4) << 3), cc = (lane >> 3) & 1;
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) {
         uint32_t kf[4];
         ldmatrix_x4(ks + row * S::row_bytes + (((2 * j + cc) ^ (row & 7)) * 16), kf);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int mt = 0; mt < M; ++mt) {
           H2::mma(s[mt][0], qf[mt][j], kf[0], kf[1]);
           H2::mma(s[mt][1], qf[mt][j], kf[2], kf[3]);
         }
@@ -472,33 +503,40 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
     const int k_first = span.key(16 * g), k_last = span.key(16 * g + 15);
     const bool whole = mine == 0xFFFFu && !span.unplaced && k_last - k_first == 15 &&
                        (k_last < min(span.sinks, span.hi0) || (k_first >= span.lo1 && k_last < span.hi0));
-    // keys of this lane's four columns: 2 (lane % 4) + {0, 1, 8, 9}
-    int key[4];
+    // This lane's keys: 2 (lane % 4) + {0, 1, 8, 9}, or (kSwap) lane / 4 + {0, 8}.
+    constexpr int kKeys = kSwap ? 2 : 4;
+    auto score = [&](int mt, int hh, int c) -> float & {
+      return kSwap ? s[0][0][2 * c + hh] : s[mt][c >> 1][2 * hh + (c & 1)];
+    };
+    int key[kKeys];
     uint32_t col_there = 0;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int col = 2 * (lane % 4) + (c & 1) + 8 * (c >> 1);
+    for (int c = 0; c < kKeys; ++c) {
+      const int col = kSwap ? lane / 4 + 8 * c : 2 * (lane % 4) + (c & 1) + 8 * (c >> 1);
       key[c] = span.key(16 * g + col);
       if ((mine >> col) & 1u) col_there |= 1u << c;
     }
-    uint32_t pf[MT][4];
+    uint32_t pf[M][4];  // (kSwap: [0][0..1])
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
+    for (int mt = 0; mt < M; ++mt) {
       float mx[2];
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
         float x = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float &v = s[mt][c >> 1][2 * hh + (c & 1)];
+        for (int c = 0; c < kKeys; ++c) {
+          float &v = score(mt, hh, c);
           const bool on = whole || (((col_there >> c) & 1u) && window_sees(key[c], lo[mt][hh], hi[mt][hh], span.sinks) &&
                                     hi[mt][hh] > 0);
           v = on ? v * p.scale_log2 : -INFINITY;
           x = fmaxf(x, v);
         }
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
         mx[hh] = x;
+      }
+#pragma unroll
+      for (int d = kSwap ? 4 : 1; d <= (kSwap ? 16 : 2); d *= 2) {
+        mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], d));
+        mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], d));
       }
       const bool move0 = mx[0] > m_run[mt][0] + H2::kSlack, move1 = mx[1] > m_run[mt][1] + H2::kSlack;
       if (__any_sync(0xffffffffu, move0 || move1)) {
@@ -507,22 +545,34 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
         m_run[mt][0] = n0, m_run[mt][1] = n1;
         l_run[mt][0] *= f0, l_run[mt][1] *= f1;
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) {
-          o[mt][j][0] *= f0, o[mt][j][1] *= f0;
-          o[mt][j][2] *= f1, o[mt][j][3] *= f1;
+        for (int j = 0; j < kOut; ++j) {
+          o[mt][j][0] *= f0, o[mt][j][1] *= kSwap ? f1 : f0;
+          o[mt][j][2] *= kSwap ? f0 : f1, o[mt][j][3] *= f1;
         }
       }
+      // (the sums take the weights that P V uses, so that these sum to one)
+      const float base0 = m_run[mt][0] == -INFINITY ? 0.0f : m_run[mt][0] - H2::kShift;
+      const float base1 = m_run[mt][1] == -INFINITY ? 0.0f : m_run[mt][1] - H2::kShift;
+      if constexpr (kSwap) {
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        const float base = m_run[mt][hh] == -INFINITY ? 0.0f : m_run[mt][hh] - H2::kShift;
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          const uint32_t u = H2::pack(fast_exp2(s[mt][nt][2 * hh] - base), fast_exp2(s[mt][nt][2 * hh + 1] - base));
-          pf[mt][2 * nt + hh] = u;
-          // the weights that P V uses, so that they sum to one
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t u = H2::pack(fast_exp2(score(0, 0, c) - base0), fast_exp2(score(0, 1, c) - base1));
+          pf[0][c] = transpose8(u);
           const float2 w = H2::unpack(u);
-          l_run[mt][hh] += w.x + w.y;
+          l_run[0][0] += w.x;
+          l_run[0][1] += w.y;
         }
+      } else {
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) {
+            const float base = hh == 0 ? base0 : base1;
+            const uint32_t u = H2::pack(fast_exp2(s[mt][nt][2 * hh] - base), fast_exp2(s[mt][nt][2 * hh + 1] - base));
+            pf[mt][2 * nt + hh] = u;
+            const float2 w = H2::unpack(u);
+            l_run[mt][hh] += w.x + w.y;
+          }
       }
     }
     if (partial && !whole) {
@@ -549,14 +599,22 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
       __syncwarp();
     }
     // O += P V
-    {
+    if constexpr (kSwap) {  // O^T += V^T P^T
+      const int row = (lane & 7) + ((lane >> 4) << 3), cc = (lane >> 3) & 1;
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        uint32_t vf[4];
+        ldmatrix_x4_trans(vs + row * S::row_bytes + (((2 * j + cc) ^ (row & 7)) * 16), vf);
+        H2::mma(o[0][j], vf, pf[0][0], pf[0][1]);
+      }
+    } else {
       const int row = (lane & 7) + (((lane >> 3) & 1) << 3), cc = lane >> 4;
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) {
         uint32_t vf[4];
         ldmatrix_x4_trans(vs + row * S::row_bytes + (((2 * j + cc) ^ (row & 7)) * 16), vf);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int mt = 0; mt < M; ++mt) {
           H2::mma(o[mt][2 * j], pf[mt], vf[0], vf[1]);
           H2::mma(o[mt][2 * j + 1], pf[mt], vf[2], vf[3]);
         }
@@ -574,26 +632,34 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
   float *js = reinterpret_cast<float *>(smem_rows);
   float *box = reinterpret_cast<float *>(smem_rows + (S::ring > S::join ? S::ring : S::join));
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int mt = 0; mt < M; ++mt)
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
       float l = l_run[mt][hh];
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
-      const int r = 16 * mt + lane / 4 + 8 * hh;
+#pragma unroll
+      for (int d = kSwap ? 4 : 1; d <= (kSwap ? 16 : 2); d *= 2) l += __shfl_xor_sync(0xffffffffu, l, d);
+      const int r = own_row(mt, hh);
       if (r >= n_rows) continue;
       float *row = js + (warp * R + r) * kRow;
+      if constexpr (kSwap) {
 #pragma unroll
-      for (int j = 0; j < D / 8; ++j)
-        *reinterpret_cast<float2 *>(row + 8 * j + 2 * (lane % 4)) = make_float2(o[mt][j][2 * hh], o[mt][j][2 * hh + 1]);
-      if (lane % 4 == 0) {
+        for (int j = 0; j < D / 16; ++j) {
+          row[16 * j + lane / 4] = o[0][j][hh];
+          row[16 * j + lane / 4 + 8] = o[0][j][2 + hh];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j)
+          *reinterpret_cast<float2 *>(row + 8 * j + 2 * (lane % 4)) = make_float2(o[mt][j][2 * hh], o[mt][j][2 * hh + 1]);
+      }
+      if (kSwap ? lane < 4 : lane % 4 == 0) {
         row[D] = m_run[mt][hh];
         row[D + 1] = l;
       }
     }
   __syncthreads();
   // Row r of every CTA of the cluster goes to CTA r % n_split, place
-  // (r / n_split) n_split + split of its box (16 MT rows in all), which
+  // (r / n_split) n_split + split of its box (R rows in all), which
   // joins them: one barrier between the pushes and the joins, and nobody's
   // memory is touched after it.
   namespace cg = cooperative_groups;
@@ -637,7 +703,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
 constexpr int kJoinShare = 4;
 template <typename T, int D, int MT, bool kPaged>
 __global__ void __launch_bounds__(128) window_rows_join_kernel(const __grid_constant__ RowsParams p) {
-  constexpr int R = 16 * MT;
+  constexpr int R = RowsSmem<T, D, MT, kPaged>::rows;
   const int item = blockIdx.x / kJoinShare;
   const int rt = item % p.row_tiles, bh = item / p.row_tiles;
   const int b = bh / p.Hk, hk = bh - b * p.Hk;
