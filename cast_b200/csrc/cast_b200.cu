@@ -1381,7 +1381,7 @@ static int launch_rows(const castk::RowsParams &p, const RowsPlan &plan, cudaStr
   }
   CAST_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p));
   if (p.part) {
-    castk::window_rows_join_kernel<T, D, MT, kPaged><<<(unsigned)(items * castk::kJoinShare), 128, 0, s>>>(p);
+    castk::window_rows_join_kernel<T, D, MT, kPaged><<<(unsigned)(items * S::rows), castk::kRowsJoin * D / 4, 0, s>>>(p);
     CAST_CUDA_TRY(cudaGetLastError());
   }
   return CAST_OK;
@@ -1416,7 +1416,7 @@ static int window_dims_ok(int B, int Hq, int Hk, int Lq, int Lk, int D, long lon
 
 static int rows_call(castk::RowsParams &p, const RowsPlan &plan, bool paged, int dtype, int D, void *workspace,
                      size_t workspace_bytes, cudaStream_t s) {
-  if ((long long)p.B * p.Hk * plan.row_tiles * std::max(plan.n_split, castk::kJoinShare) >= (1ll << 31))
+  if ((long long)p.B * p.Hk * plan.row_tiles * std::max(plan.n_split, 32) >= (1ll << 31))
     return fail(CAST_ERR_UNSUPPORTED, "size outside the kernels' grid");
   p.row_tiles = plan.row_tiles;
   p.n_split = plan.n_split;
@@ -1472,8 +1472,10 @@ struct TilesPlan {
 // How the many-row kernel cuts a call: an item is a query tile of one head
 // group, and two CTAs run on an SM.  The items of the last, incomplete wave
 // (or of the last two) are cut along their keys into equal parts where that
-// ends sooner, counted in steps of 128 keys: an item costs its keys and about
-// 4 steps to start and end, a part 2.5 more to leave and join its result.
+// ends sooner, counted in steps of 128 keys (1.5 us with two CTAs on the SM):
+// an item costs its keys and about 4 steps to start and end, a part one more
+// to leave its result, and the second launch that joins them 3 and a little
+// for each part's 64 KB.
 static TilesPlan tiles_plan(int B, int Hq, int Hk, int Lq, int Lk, long long window, long long sinks, int frame,
                             int D, int n_sms) {
   TilesPlan t;
@@ -1494,7 +1496,7 @@ static TilesPlan tiles_plan(int B, int Hq, int Hk, int Lq, int Lk, long long win
     if (cut == 0) continue;
     for (int parts = 2; parts <= 128 && c / parts >= 2.0; ++parts) {
       const double rounds = std::ceil((double)cut * parts / slots);
-      const double cost = (waves - q) * (c + 4.0) + rounds * (c / parts + 6.5) + 0.05 * parts;
+      const double cost = (waves - q) * (c + 4.0) + rounds * (c / parts + 5.0) + 3.0 + 0.02 * cut * parts;
       if (cost < 0.97 * best) {
         best = cost;
         t.parts = parts;
@@ -1615,7 +1617,11 @@ static int launch_tiles(const castk::RowsParams &r, const TilesPlan &plan, int d
                                                                             tm_k[2], tm_v[2], tm_o, p);
   CAST_CUDA_TRY(cudaGetLastError());
   if (cut > 0) {
-    castk::window_tiles_join_kernel<T, D><<<cut * (D / castk::kJoinCols), 128 * castk::kJoinGroups, 0, s>>>(p);
+    // (eight groups of threads where each has parts to take, else two)
+    if (plan.parts >= 12)
+      castk::window_tiles_join_kernel<T, D, 8><<<cut * (D / castk::kJoinCols), 128 * 8, 0, s>>>(p);
+    else
+      castk::window_tiles_join_kernel<T, D, 2><<<cut * (D / castk::kJoinCols), 128 * 2, 0, s>>>(p);
     CAST_CUDA_TRY(cudaGetLastError());
   }
   return CAST_OK;

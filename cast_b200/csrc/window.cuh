@@ -254,6 +254,35 @@ __device__ __forceinline__ const T *rows_value(const RowsParams &p, int b, int h
   return pg < 0 || pg >= p.n_pages ? nullptr : v + pg * p.vs[0] + (key % p.page) * p.vs[2];
 }
 
+// Gives columns c .. c + 3 of a token's row the infinities and NaN of the
+// values that it sees and not every row of its tile does.
+template <typename T, bool kPaged>
+__device__ __noinline__ void rows_give_back(const RowsParams &p, const WindowSpan &span, int b, int hk, int token, int c,
+                                            float (&a)[4]) {
+  const int pos = span.len - p.Lq + token;
+  if (pos < 0) return;
+  int lo, hi;
+  window_bounds(p.rule, span.len, pos, lo, hi);
+  for (int v = 0; v < span.n; ++v) {
+    const int key = span.key(v);
+    if (!span.some(key) || !window_sees(key, lo, hi, span.sinks)) continue;
+    const T *src = rows_value<T, kPaged>(p, b, hk, key);
+    if (!src) continue;
+    for (int i = 0; i < 4; ++i) {
+      const float y = (float)src[c + i];
+      if (!isfinite(y)) a[i] += y;
+    }
+  }
+}
+
+// Writes columns c .. c + 3 of row r (token r / group, head r % group).
+template <typename T>
+__device__ __forceinline__ void rows_store(const RowsParams &p, int b, int hk, int r, int c, const float (&a)[4]) {
+  const int token = p.by_group.div(r), head = hk * p.group + r - token * p.group;
+  T *dst = static_cast<T *>(p.out) + b * p.os[0] + (long long)head * p.os[1] + (long long)token * p.os[2] + c;
+  *reinterpret_cast<uint2 *>(dst) = make_uint2(Half2<T>::pack(a[0], a[1]), Half2<T>::pack(a[2], a[3]));
+}
+
 // Joins the parts' (O, m, l) of rows first, first + step, ... of a tile's
 // n_rows, normalises and writes them; part(r, j) is the j-th part's row: O, m,
 // l and whether the part took an infinity or NaN out of a value that only some
@@ -281,24 +310,12 @@ __device__ __forceinline__ void window_write(const RowsParams &p, const WindowSp
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // (a NaN sum stays one)
 #pragma unroll
     for (int i = 0; i < 4; ++i) a[i] *= inv;
-    const int token = (r0 + r) / p.group, head = hk * p.group + (r0 + r) % p.group;
-    if (bad != 0.0f) {
-      int lo = 0, hi = 0;
-      const int pos = span.len - p.Lq + token;
-      if (pos >= 0) window_bounds(p.rule, span.len, pos, lo, hi);
-      for (int v = 0; v < span.n; ++v) {
-        const int key = span.key(v);
-        if (!span.some(key) || hi == 0 || !window_sees(key, lo, hi, span.sinks)) continue;
-        const T *src = rows_value<T, kPaged>(p, b, hk, key);
-        if (!src) continue;
-        for (int i = 0; i < 4; ++i) {
-          const float y = (float)src[c + i];
-          if (!isfinite(y)) a[i] += y;
-        }
-      }
+    if (__builtin_expect(bad != 0.0f, 0)) {
+      float z[4] = {a[0], a[1], a[2], a[3]};
+      rows_give_back<T, kPaged>(p, span, b, hk, p.by_group.div(r0 + r), c, z);
+      for (int i = 0; i < 4; ++i) a[i] = z[i];
     }
-    T *dst = static_cast<T *>(p.out) + b * p.os[0] + (long long)head * p.os[1] + (long long)token * p.os[2] + c;
-    *reinterpret_cast<uint2 *>(dst) = make_uint2(Half2<T>::pack(a[0], a[1]), Half2<T>::pack(a[2], a[3]));
+    rows_store<T>(p, b, hk, r0 + r, c, a);
   }
 }
 
@@ -698,22 +715,68 @@ __global__ void __launch_bounds__(kRowsWarps * 32) window_rows_kernel(const __gr
                                  (int)threadIdx.x, (int)blockDim.x);
 }
 
-// Joins the parts that window_rows_kernel left in p.part: kJoinShare CTAs for
-// each tile of rows.
-constexpr int kJoinShare = 4;
+// Joins the parts that window_rows_kernel left in p.part: one CTA for a row
+// of a tile.  Its threads take the parts' maxima and sums side by side, then
+// every kRowsJoin-th part's O, so that no load waits for another (a thread
+// walking the parts one after the other took 20 us for 37 parts).
+constexpr int kRowsJoin = 8;
 template <typename T, int D, int MT, bool kPaged>
-__global__ void __launch_bounds__(128) window_rows_join_kernel(const __grid_constant__ RowsParams p) {
-  constexpr int R = RowsSmem<T, D, MT, kPaged>::rows;
-  const int item = blockIdx.x / kJoinShare;
-  const int rt = item % p.row_tiles, bh = item / p.row_tiles;
-  const int b = bh / p.Hk, hk = bh - b * p.Hk;
+__global__ void __launch_bounds__(kRowsJoin * D / 4) window_rows_join_kernel(const __grid_constant__ RowsParams p) {
+  constexpr int R = RowsSmem<T, D, MT, kPaged>::rows, kRow = D + 4, kThreads = kRowsJoin * D / 4;
+  __shared__ float4 acc_s[kRowsJoin][D / 4];
+  __shared__ float red_s[2][kThreads / 32];
+  const int item = blockIdx.x / R, r = blockIdx.x % R;
+  const int bh = p.by_tiles.div(item), rt = item - bh * p.row_tiles;
+  const int b = p.by_hk.div(bh), hk = bh - b * p.Hk;
   const int r0 = rt * R, r_end = min(p.rows, r0 + R);
-  const int len = min(max(p.kv_lens ? p.kv_lens[b] : p.lk, 0), p.lk);
-  const WindowSpan span = window_span(p.rule, len, p.Lq, r0 / p.group, (r_end - 1) / p.group);
-  const float *base = p.part + (long long)item * p.n_split * (R * (D + 4));
-  window_write<T, D, MT, kPaged>(p, span, b, hk, r0, r_end - r0, blockIdx.x % kJoinShare, kJoinShare,
-                                 [&](int r, int j) { return base + ((long long)j * R + r) * (D + 4); },
-                                 (int)threadIdx.x, (int)blockDim.x);
+  if (r0 + r >= r_end) return;  // (whole CTAs)
+  const float *base = p.part + (long long)item * p.n_split * (R * kRow) + r * kRow;
+  auto part = [&](int j) { return base + (long long)j * (R * kRow); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the parts' maximum
+  float m = -INFINITY;
+  for (int j = threadIdx.x; j < p.n_split; j += kThreads) m = fmaxf(m, part(j)[D]);
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  if (lane == 0) red_s[0][warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) m = fmaxf(m, red_s[0][w]);
+  // sums and O
+  const int g = threadIdx.x / (D / 4), c = threadIdx.x % (D / 4);
+  float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float l = 0.0f;
+  bool bad = false;
+#pragma unroll 4
+  for (int j = g; j < p.n_split; j += kRowsJoin) {
+    const float4 tail = *reinterpret_cast<const float4 *>(part(j) + D);
+    const float4 v = *reinterpret_cast<const float4 *>(part(j) + 4 * c);
+    const float f = tail.x == -INFINITY ? 0.0f : fast_exp2(tail.x - m);
+    l = fmaf(tail.y, f, l);
+    a.x = fmaf(v.x, f, a.x), a.y = fmaf(v.y, f, a.y), a.z = fmaf(v.z, f, a.z), a.w = fmaf(v.w, f, a.w);
+    bad = bad || __float_as_int(tail.z) != 0;
+  }
+  acc_s[g][c] = a;
+  if (c == 0) red_s[1][g] = l;  // (kRowsJoin of them fit: a warp each or two)
+  const bool any_bad = __syncthreads_or(bad);
+  if (g != 0) return;
+  float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  l = 0.0f;
+#pragma unroll
+  for (int j = 0; j < kRowsJoin; ++j) {
+    const float4 v = acc_s[j][c];
+    y[0] += v.x, y[1] += v.y, y[2] += v.z, y[3] += v.w;
+    l += red_s[1][j];
+  }
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // (a NaN sum stays one)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] *= inv;
+  if (any_bad) {
+    const int len = min(max(p.kv_lens ? p.kv_lens[b] : p.lk, 0), p.lk);
+    const WindowSpan span = window_span(p.rule, len, p.Lq, p.by_group.div(r0), p.by_group.div(r_end - 1));
+    rows_give_back<T, kPaged>(p, span, b, hk, p.by_group.div(r0 + r), 4 * c, y);
+  }
+  rows_store<T>(p, b, hk, r0 + r, 4 * c, y);
 }
 
 }  // namespace castk

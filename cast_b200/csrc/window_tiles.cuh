@@ -650,42 +650,51 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
   }
 }
 
-// Joins the parts of the cut items: one CTA for eight columns of a query
-// tile; thread (row, g) takes every kJoinGroups-th part.
-constexpr int kJoinGroups = 4, kJoinCols = 8;
-template <typename T, int D>
+// Joins the parts of the cut items: one CTA for eight columns of a query tile;
+// thread (row, g) takes every kJoinGroups-th part, several loads at a time.
+constexpr int kJoinCols = 8;
+template <typename T, int D, int kJoinGroups>
 __global__ void __launch_bounds__(128 * kJoinGroups) window_tiles_join_kernel(const __grid_constant__ TilesParams p) {
   __shared__ float acc_s[kJoinGroups][kJoinCols + 1][128];
+  __shared__ float max_s[kJoinGroups][128];
   constexpr int cuts = D / kJoinCols;
+  constexpr long long kPart = tiles_part_floats<D>();
   const int cut = blockIdx.x % cuts, item = blockIdx.x / cuts;
   const int row_in = threadIdx.x & 127, g = threadIdx.x >> 7;
   const int x = p.n_whole + item;
-  const int bhg = x / p.q_tiles, qt = p.q_tiles - 1 - (x - bhg * p.q_tiles);
-  const int b = bhg / p.head_groups, hg = bhg - b * p.head_groups;
+  const int bhg = p.by_tiles.div(x), qt = p.q_tiles - 1 - (x - bhg * p.q_tiles);
+  const int b = p.by_groups.div(bhg), hg = bhg - b * p.head_groups;
   const int row0 = qt * 128, row_end = min(p.rows, row0 + 128);
   const int row = row0 + row_in;
   const bool on = row < p.rows;
-  const float *base = p.part + (long long)item * p.parts * tiles_part_floats<D>();
+  const float *base = p.part + (long long)item * p.parts * kPart;
   const float *tails = base + 128 * D + row_in;
+  const int parts = on ? p.parts : 0;
   float m = -INFINITY;
-  bool bad = false;
-  if (on)
-    for (int j = 0; j < p.parts; ++j) m = fmaxf(m, tails[j * tiles_part_floats<D>()]);
+#pragma unroll 8
+  for (int j = g; j < parts; j += kJoinGroups) m = fmaxf(m, __ldg(tails + j * kPart));
+  max_s[g][row_in] = m;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kJoinGroups; ++j) m = fmaxf(m, max_s[j][row_in]);
   float l = 0.0f, a[kJoinCols];
 #pragma unroll
   for (int c = 0; c < kJoinCols; ++c) a[c] = 0.0f;
-  if (on) {
-#pragma unroll 4
-    for (int j = g; j < p.parts; j += kJoinGroups) {
-      const float *tail = tails + j * tiles_part_floats<D>();
-      const float mj = tail[0];
-      bad = bad || __float_as_int(tail[256]) != 0;
-      if (mj == -INFINITY) continue;  // nothing seen: its O may not be written
-      const float f = fast_exp2(mj - m);
-      const float *o = base + j * tiles_part_floats<D>() + cut * kJoinCols * 128 + row_in;
-      l = fmaf(tail[128], f, l);
+  bool bad = false;
+#pragma unroll 3
+  for (int j = g; j < parts; j += kJoinGroups) {
+    const float *tail = tails + j * kPart;
+    const float *o = base + j * kPart + cut * kJoinCols * 128 + row_in;
+    const float mj = __ldg(tail), lj = __ldg(tail + 128), flag = __ldg(tail + 256);
+    float v[kJoinCols];
 #pragma unroll
-      for (int c = 0; c < kJoinCols; ++c) a[c] = fmaf(o[c * 128], f, a[c]);
+    for (int c = 0; c < kJoinCols; ++c) v[c] = __ldg(o + c * 128);
+    bad = bad || __float_as_int(flag) != 0;
+    if (mj != -INFINITY) {  // (where nothing was seen, O may hold anything)
+      const float f = fast_exp2(mj - m);
+      l = fmaf(lj, f, l);
+#pragma unroll
+      for (int c = 0; c < kJoinCols; ++c) a[c] = fmaf(v[c], f, a[c]);
     }
   }
 #pragma unroll
@@ -715,7 +724,7 @@ __global__ void __launch_bounds__(128 * kJoinGroups) window_tiles_join_kernel(co
     if (pos >= 0) window_bounds(p.rule, len, pos, lo, hi);
     float z[kJoinCols];
     for (int c = 0; c < kJoinCols; ++c) z[c] = y[c];
-    tiles_give_back<T>(p, span, b, hg / p.groups_per_key, lo, hi, cut * kJoinCols, z);
+    tiles_give_back<T>(p, span, b, p.by_keys.div(hg), lo, hi, cut * kJoinCols, z);
     for (int c = 0; c < kJoinCols; ++c) y[c] = z[c];
   }
   T *dst = static_cast<T *>(p.out) + b * p.os[0] + head * p.os[1] + token * p.os[2] + cut * kJoinCols;
