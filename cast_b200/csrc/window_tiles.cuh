@@ -143,6 +143,13 @@ __device__ __forceinline__ uint32_t interval_mask(int lo, int hi, int n0) {
   return below_b & ~below_a;
 }
 
+// Waits for the loads into v; ties v to the wait, so that nothing reads it before.
+__device__ __forceinline__ void tmem_wait_ld64(uint32_t (&v)[64]) {
+  castdev::tmem_wait_ld();
+#pragma unroll
+  for (int i = 0; i < 64; ++i) asm volatile("" : "+r"(v[i]));
+}
+
 // One 64-key step's P = 2^(S c2 - base) in pairs in v[0..31]; returns their sum
 // as rounded.  (Taking an eighth to a half of the exponentials to the FMA pipe
 // with a polynomial of degree 3 was slower: 321 to 340 us against 313 for 24
@@ -512,47 +519,45 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
 #pragma unroll
         for (int c = 0; c < 32; ++c) v[c] = 0u;
       } else {
-        castdev::tmem_ld32(sb, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-        castdev::tmem_ld32(sb + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
-        castdev::tmem_wait_ld();
-        bool slow = __any_sync(0xffffffffu, m_run == -INFINITY);
-        if (!slow) {
-          sum = full_step ? tiles_probs<T, false>(v, seen, c2, m_run - X::kShift)
-                          : tiles_probs<T, true>(v, seen, c2, m_run - X::kShift);
-          slow = __any_sync(0xffffffffu, !(sum <= X::kSumLimit));
-          if (slow) {
-            castdev::tmem_ld32(sb, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-            castdev::tmem_ld32(sb + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
-            castdev::tmem_wait_ld();
-          }
-        }
-        if (__builtin_expect(slow, 0)) {
-          const float m_step = full_step ? row_max<false, false>(v, seen, c2) : row_max<false, true>(v, seen, c2);
-          float o_scale = 1.0f;
-          if (m_step > m_run + X::kSlack || m_run == -INFINITY) {
-            const float m_new = fmaxf(m_run, m_step);
-            o_scale = (m_run == -INFINITY) ? (m_new == -INFINITY ? 1.0f : 0.0f) : fast_exp2(m_run - m_new);
-            l_run *= o_scale;
-            m_run = m_new;
-          }
-          if (h > 0 && __any_sync(0xffffffffu, o_scale != 1.0f)) {
-            const int hp = h - 1;
-            ok = __all_sync(0xffffffffu, castdev::mbar_wait(&pv_done[hp & 1], (hp >> 1) & 1, err));
-            if (!ok) break;
-            castdev::tc_fence_after();
+        // One pass against the running maximum; where that is not set yet, or a
+        // sum passes its limit, the maximum is found and the pass made again
+        // (the same code: the loop has to stay in the instruction cache).
+        bool find = __any_sync(0xffffffffu, m_run == -INFINITY);
+        for (;;) {
+          castdev::tmem_ld32(sb, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+          castdev::tmem_ld32(sb + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+          tmem_wait_ld64(v);
+          if (__builtin_expect(find, 0)) {
+            const float m_step = row_max<false, true>(v, seen, c2);
+            float o_scale = 1.0f;
+            if (m_step > m_run + X::kSlack || m_run == -INFINITY) {
+              const float m_new = fmaxf(m_run, m_step);
+              o_scale = (m_run == -INFINITY) ? (m_new == -INFINITY ? 1.0f : 0.0f) : fast_exp2(m_run - m_new);
+              l_run *= o_scale;
+              m_run = m_new;
+            }
+            if (h > 0 && __any_sync(0xffffffffu, o_scale != 1.0f)) {
+              const int hp = h - 1;
+              ok = __all_sync(0xffffffffu, castdev::mbar_wait(&pv_done[hp & 1], (hp >> 1) & 1, err));
+              if (!ok) break;
+              castdev::tc_fence_after();
 #pragma unroll 1
-            for (int cc = 0; cc < D / 32; ++cc) {
-              uint32_t o[32];
-              castdev::tmem_ld32(o_addr + 32 * cc, o);
-              castdev::tmem_wait_ld();
+              for (int cc = 0; cc < D / 32; ++cc) {
+                uint32_t o[32];
+                castdev::tmem_ld32(o_addr + 32 * cc, o);
+                castdev::tmem_wait_ld();
 #pragma unroll
-              for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * o_scale);
-              castdev::tmem_st32(o_addr + 32 * cc, o);
+                for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * o_scale);
+                castdev::tmem_st32(o_addr + 32 * cc, o);
+              }
             }
           }
           const float base = (m_run == -INFINITY) ? 0.0f : m_run - X::kShift;
           sum = full_step ? tiles_probs<T, false>(v, seen, c2, base) : tiles_probs<T, true>(v, seen, c2, base);
+          if (find || !__any_sync(0xffffffffu, !(sum <= X::kSumLimit))) break;
+          find = true;
         }
+        if (!ok) break;
       }
       castdev::tmem_st32(sb, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
       l_run += sum;
@@ -616,7 +621,7 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
 #pragma unroll
           for (int h = 0; h < D / 64; ++h) tma_store_5d(&tm_o, smem + h * 16384, 64 * h, 0, row0 >> p.pack_log2, hg, b);
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-          asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+          asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         }
       } else if (ok) {
         // this part's O, maximum and sum: [tile][column][row], then [tile][m, l, flag][row]
