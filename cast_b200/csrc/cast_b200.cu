@@ -1479,7 +1479,7 @@ struct TilesPlan {
 static TilesPlan tiles_plan(int B, int Hq, int Hk, int Lq, int Lk, long long window, long long sinks, int frame,
                             int D, int n_sms) {
   TilesPlan t;
-  const int group = Hq / Hk, slots = 2 * n_sms;
+  const int group = Hq / Hk, slots = (D == 128 ? castk::TilesSmem<128>::ctas : castk::TilesSmem<64>::ctas) * n_sms;
   while (t.pack < 128 && group % (2 * t.pack) == 0) t.pack *= 2, ++t.pack_log2;
   t.head_groups = Hq / t.pack;
   const long long rows = (long long)t.pack * Lq;
@@ -1610,7 +1610,7 @@ static int launch_tiles(const castk::RowsParams &r, const TilesPlan &plan, int d
   });
   CAST_CUDA_TRY(err);
   // the softmax warps' larger share comes out of what the block was launched with
-  if (regs * castk::kTilesThreads < 128 * (castk::kTilesRegsSoft + castk::kTilesRegsRest))
+  if (regs * castk::kTilesThreads < 128 * (castk::TilesSmem<D>::regs_soft + castk::TilesSmem<D>::regs_rest))
     return fail(CAST_ERR_UNSUPPORTED, "window kernel built with %d registers a thread", regs);
   const int cut = plan.n_items - plan.n_whole;
   kernel<<<plan.n_whole + cut * plan.parts, castk::kTilesThreads, smem, s>>>(tm_q, tm_k[0], tm_v[0], tm_k[1], tm_v[1],

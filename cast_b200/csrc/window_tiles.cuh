@@ -31,27 +31,35 @@
 namespace castk {
 
 constexpr int kTilesThreads = 256;
-// Registers of a thread of the softmax warps and of the others:
-// 128 (200 + 56) = 256 * 128, the block's share of the SM at launch.
-constexpr int kTilesRegsSoft = 200, kTilesRegsRest = 56;
 constexpr int kTilesPartCols = 4;  // m, l, flag (and nothing) of a part's rows beside its O
 
+// What depends on the head vectors' length.  128: TMEM holds O (128 columns)
+// and two S buffers for two CTAs, so that S of the next step is there while the
+// softmax works.  64: O takes half, and four CTAs with one S buffer each keep
+// the exponentials busier than two with two (twice the softmax warps).
 template <int D>
 struct TilesSmem {
+  static constexpr int ctas = D == 128 ? 2 : 4;    // on an SM
+  static constexpr int bufs = D == 128 ? 2 : 1;    // S buffers
+  static constexpr int chunk = D == 128 ? 64 : 32; // scores a thread holds at a time
+  // Registers of a thread of the softmax warps and of the others; their sum
+  // times 128 is the block's share of the SM at launch, 65536 / ctas.
+  static constexpr int regs_soft = D == 128 ? 200 : 88, regs_rest = D == 128 ? 56 : 40;
+  static constexpr int tmem_cols = D == 128 ? 256 : 128, s_col = D;  // O in columns [0, D)
   static constexpr int keys = 64;  // of one K or V tile: one step
   static constexpr int q_tile = 128 * D * 2;
   static constexpr int tile = keys * D * 2;
   static constexpr int half = keys * 128;  // 64 columns of a tile
-  // Two stages each: K of step h is free when S of step h is done (s_full) and
-  // V when P V is (pv_done), so neither ring has barriers of its own for that.
   static constexpr int stages = 2;
   static constexpr int k_off = q_tile;
   static constexpr int v_off = k_off + stages * tile;
   static constexpr int bars = v_off + stages * tile;
-  // q_full, then [2] each: k_full, v_full, v_raw, s_full, p_full, pv_done; drain
-  static constexpr int n_bars = 1 + 6 * 2 + 1;
+  // q_full, then [2] each: k_full, v_full, v_raw, s_full, p_full, pv_done, k_free, v_free; drain
+  static constexpr int n_bars = 1 + 8 * 2 + 1;
   static constexpr int tmem_slot = bars + 8 * n_bars;
   static constexpr int alloc = tmem_slot + 16;
+  static __device__ __forceinline__ int buf(int h) { return bufs == 2 ? h & 1 : 0; }
+  static __device__ __forceinline__ uint32_t phase(int h) { return bufs == 2 ? (h >> 1) & 1 : h & 1; }
 };
 
 template <int N>
@@ -143,48 +151,75 @@ __device__ __forceinline__ uint32_t interval_mask(int lo, int hi, int n0) {
   return below_b & ~below_a;
 }
 
-// Waits for the loads into v; ties v to the wait, so that nothing reads it before.
-__device__ __forceinline__ void tmem_wait_ld64(uint32_t (&v)[64]) {
+// N columns from TMEM into x, there when this returns (x is tied to the wait,
+// so that nothing reads it before).
+template <int N>
+__device__ __forceinline__ void tmem_get(uint32_t addr, uint32_t (&x)[N]) {
+  if constexpr (N == 16) {
+    castdev::tmem_ld16(addr, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 32) castdev::tmem_ld32(addr + i, *reinterpret_cast<uint32_t(*)[32]>(&x[i]));
+  }
   castdev::tmem_wait_ld();
 #pragma unroll
-  for (int i = 0; i < 64; ++i) asm volatile("" : "+r"(v[i]));
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(x[i]));
+}
+__device__ __forceinline__ void tmem_put(uint32_t addr, const uint32_t (&r)[32]) { castdev::tmem_st32(addr, r); }
+__device__ __forceinline__ void tmem_put(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
 }
 
-// One 64-key step's P = 2^(S c2 - base) in pairs in v[0..31]; returns their sum
-// as rounded.  (Taking an eighth to a half of the exponentials to the FMA pipe
-// with a polynomial of degree 3 was slower: 321 to 340 us against 313 for 24
-// heads of 3520 queries over 7920 keys; it takes ten issue slots for each.)
-template <typename T, bool kMasked>
-__device__ __forceinline__ float tiles_probs(uint32_t (&v)[64], const uint32_t (&seen)[2], float c2, float base) {
+// P = 2^(x c2 - base) of N scores in pairs; returns their sum as rounded.
+// (Taking an eighth to a half of the exponentials to the FMA pipe with a
+// polynomial of degree 3 was slower: 321 to 340 us against 313 for 24 heads of
+// 3520 queries over 7920 keys; it takes ten issue slots for each.)
+template <typename T, bool kMasked, int N>
+__device__ __forceinline__ float tiles_probs(const uint32_t (&x)[N], uint32_t (&pk)[N / 2], const uint32_t (&seen)[N / 32],
+                                             float c2, float base) {
   using X = TilesType<T>;
   const uint64_t c2x2 = f2_pack(c2, c2), nbx2 = f2_pack(-base, -base);
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int c = 0; c < 32; ++c) {
+  for (int c = 0; c < N / 2; ++c) {
     float x0, x1;
-    f2_unpack(f2_fma(f2_pack(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])), c2x2, nbx2), x0, x1);
+    f2_unpack(f2_fma(f2_pack(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])), c2x2, nbx2), x0, x1);
     float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
     if (kMasked) {
       const uint32_t w = seen[c / 16];
       e0 = ((w >> ((2 * c) % 32)) & 1u) ? e0 : 0.0f;
       e1 = ((w >> ((2 * c + 1) % 32)) & 1u) ? e1 : 0.0f;
     }
-    const uint32_t pk = X::pack(e0, e1);
-    acc[2 * (c & 3)] = X::add_lo(pk, acc[2 * (c & 3)]);
-    acc[2 * (c & 3) + 1] = X::add_hi(pk, acc[2 * (c & 3) + 1]);
-    v[c] = pk;
+    pk[c] = X::pack(e0, e1);
+    acc[2 * (c & 3)] = X::add_lo(pk[c], acc[2 * (c & 3)]);
+    acc[2 * (c & 3) + 1] = X::add_hi(pk[c], acc[2 * (c & 3) + 1]);
   }
   return ((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7]));
 }
 
-// Issues the products of one query tile over n 64-key steps.  S of step h + 2
-// goes into the buffer that P of step h came from, right after P V of step h.
-// What can be waited for ahead (V of this step, K of the one after the next)
-// is, so that only P stands between the softmax and the tensor core.
+// Maximum of the scores that are seen, times c2; -inf where none is.
+__device__ __forceinline__ float tiles_max(const uint32_t (&x)[32], uint32_t seen, float c2) {
+  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < 32; ++c) m[c & 3] = fmaxf(m[c & 3], ((seen >> c) & 1u) ? __uint_as_float(x[c]) : -INFINITY);
+  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * c2;
+}
+
+// Issues the products of one query tile over n 64-key steps.  The S that takes
+// the buffer of P of step h (step h + bufs) comes right after P V of step h.
+// What can be waited for ahead is, so that only P stands between the softmax
+// and the tensor core.  A stage of the K ring is free when its S is done and
+// one of the V ring when its P V is: with two S buffers s_full and pv_done say
+// so, with one (whose phase may have moved on twice) barriers of their own.
 template <typename T, int D>
 __device__ __forceinline__ bool tiles_issuer(uint32_t tmem, uint32_t sbase, int n, uint64_t *q_full, uint64_t *k_full,
-                                           uint64_t *v_full, uint64_t *s_full, uint64_t *p_full, uint64_t *pv_done,
-                                           int *err) {
+                                             uint64_t *v_full, uint64_t *s_full, uint64_t *p_full, uint64_t *pv_done,
+                                             uint64_t *k_free, uint64_t *v_free, int *err) {
   using S = TilesSmem<D>;
   constexpr uint32_t fmt = TilesType<T>::fmt;
   constexpr uint32_t idesc_s = castdev::make_idesc(1, fmt, fmt, 0, 0, 128, 64);
@@ -192,33 +227,35 @@ __device__ __forceinline__ bool tiles_issuer(uint32_t tmem, uint32_t sbase, int 
   const DescW qd = desc_words(sbase, 16);
   const DescW kd = desc_words(sbase + S::k_off, 16);
   const DescW vd = desc_words(sbase + S::v_off, S::half);
-  const uint32_t s_col = tmem + 128;
-  auto issue_s = [&](int buf) {
-    const uint32_t d = s_col + buf * 64, ko = buf * S::tile;
+  const uint32_t s_col = tmem + S::s_col;
+  auto issue_s = [&](int h) {
+    const uint32_t d = s_col + S::buf(h) * 64, ko = (h & 1) * S::tile;
 #pragma unroll
     for (int s = 0; s < D / 16; ++s)
       castdev::mma_f16_ss(d, qd.at((s >> 2) * 16384 + (s & 3) * 32), kd.at(ko + (s >> 2) * S::half + (s & 3) * 32),
                           idesc_s, s > 0);
-    castdev::tc_commit(&s_full[buf]);
+    castdev::tc_commit(&s_full[S::buf(h)]);
+    if (S::bufs == 1) castdev::tc_commit(&k_free[h & 1]);
   };
   if (!castdev::mbar_wait(q_full, 0, err)) return false;
-  for (int h = 0; h < min(n, 2); ++h) {
+  for (int h = 0; h < min(n, S::bufs); ++h) {
     if (!castdev::mbar_wait(&k_full[h], 0, err)) return false;
     castdev::tc_fence_after();
     issue_s(h);
   }
   for (int h = 0; h < n; ++h) {
-    const int buf = h & 1, phase = (h >> 1) & 1;
-    const bool more = h + 2 < n;
-    if (!castdev::mbar_wait(&v_full[buf], phase, err)) return false;
-    if (more && !castdev::mbar_wait(&k_full[buf], phase ^ 1, err)) return false;
-    if (!castdev::mbar_wait(&p_full[buf], phase, err)) return false;
+    const int stage = h & 1, next = h + S::bufs;
+    const bool more = next < n;
+    if (!castdev::mbar_wait(&v_full[stage], (h >> 1) & 1, err)) return false;
+    if (more && !castdev::mbar_wait(&k_full[next & 1], (next >> 1) & 1, err)) return false;
+    if (!castdev::mbar_wait(&p_full[S::buf(h)], S::phase(h), err)) return false;
     castdev::tc_fence_after();
-    const uint32_t vo = buf * S::tile, pa = s_col + buf * 64;
+    const uint32_t vo = stage * S::tile, pa = s_col + S::buf(h) * 64;
 #pragma unroll
     for (int s = 0; s < 4; ++s) castdev::mma_f16_ts(tmem, pa + 8 * s, vd.at(vo + 2048 * s), idesc_pv, (h | s) != 0);
-    castdev::tc_commit(&pv_done[buf]);
-    if (more) issue_s(buf);
+    castdev::tc_commit(&pv_done[S::buf(h)]);
+    if (S::bufs == 1) castdev::tc_commit(&v_free[stage]);
+    if (more) issue_s(next);
   }
   return true;
 }
@@ -242,7 +279,7 @@ __device__ __noinline__ void tiles_give_back(const TilesParams &p, const WindowS
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kTilesThreads, 2)
+__global__ void __launch_bounds__(kTilesThreads, TilesSmem<D>::ctas)
     window_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_k_sink,
                         const __grid_constant__ CUtensorMap tm_v_sink, const __grid_constant__ CUtensorMap tm_k_rest,
@@ -261,7 +298,9 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
   uint64_t *s_full = v_raw + 2;
   uint64_t *p_full = s_full + 2;
   uint64_t *pv_done = p_full + 2;
-  uint64_t *mma_drain = pv_done + 2;
+  uint64_t *k_free = S::bufs == 2 ? s_full : pv_done + 2;   // see tiles_issuer
+  uint64_t *v_free = S::bufs == 2 ? pv_done : pv_done + 4;
+  uint64_t *mma_drain = pv_done + 6;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + S::tmem_slot);
   volatile uint32_t *bad_flag = tmem_slot + 1;  // an infinity or NaN was taken out of a V tile
   int *err = reinterpret_cast<int *>(tmem_slot + 2);
@@ -339,22 +378,16 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
     for (int i = 0; i < S::n_bars; ++i) castdev::mbar_init(&bar[i], 1);
     for (int i = 0; i < 2; ++i) castdev::mbar_init(&p_full[i], 4);
     castdev::fence_barrier_init();
-    castdev::tma_prefetch_desc(&tm_q);
-    castdev::tma_prefetch_desc(&tm_k);
-    castdev::tma_prefetch_desc(&tm_v);
-    if (n_kv > 0) {
+    if (n_kv > 0) {  // what the first product needs, before the block meets
       castdev::mbar_arrive_expect_tx(q_full, S::q_tile);
 #pragma unroll
       for (int h = 0; h < D / 64; ++h)
         tma_load_5d(smem + h * 16384, &tm_q, q_full, 64 * h, 0, row0 >> p.pack_log2, hg, b);
-      for (int j = 0; j < min(n_kv, 2); ++j) {  // both rings, before the block meets
-        issue_k(j);
-        issue_v(j);
-      }
+      issue_k(0);
     }
   }
   if (warp == kMWarp) {
-    castdev::tmem_alloc(tmem_slot, 256);
+    castdev::tmem_alloc(tmem_slot, S::tmem_cols);
     castdev::tmem_relinquish();
   }
   __syncthreads();
@@ -362,12 +395,12 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
   const uint32_t tmem = *tmem_slot;
 
   if (warp >= 4) {
-    regs_dec<kTilesRegsRest>();
+    regs_dec<S::regs_rest>();
     if (warp == kKWarp) {
       if (lane == 0 && n_kv > 0) {
-        int issued = min(n_kv, 2);
-        for (int j = 2; j < n_kv; ++j) {  // (the stage is free when S of step j - 2 is done)
-          if (!castdev::mbar_wait(&s_full[j & 1], ((j >> 1) - 1) & 1, err)) break;
+        int issued = 1;
+        for (int j = 1; j < n_kv; ++j) {  // (the stage is free when S of step j - 2 is done)
+          if (j >= 2 && !castdev::mbar_wait(&k_free[j & 1], ((j >> 1) - 1) & 1, err)) break;
           issue_k(j);
           issued = j + 1;
         }
@@ -439,9 +472,11 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
       };
       int issued = min(n_kv, 2), looked = 0;  // tiles started; tiles gone over
       bool ok = true;
+      if (lane == 0)
+        for (int j = 0; j < issued; ++j) issue_v(j);
       for (int j = 0; ok && j < n_kv; ++j) {
         if (j >= 2) {  // (the stage is free when P V of step j - 2 is done)
-          ok = __all_sync(0xffffffffu, castdev::mbar_wait(&pv_done[j & 1], ((j >> 1) - 1) & 1, err));
+          ok = __all_sync(0xffffffffu, castdev::mbar_wait(&v_free[j & 1], ((j >> 1) - 1) & 1, err));
           if (!ok) break;
           if (lane == 0) issue_v(j);
           issued = j + 1;
@@ -461,18 +496,18 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
         }
     } else if (warp == kMWarp) {
       if (lane == 0 && n_kv > 0) {
-        tiles_issuer<T, D>(tmem, castdev::smem_u32(smem), n_kv, q_full, k_full, v_full, s_full, p_full, pv_done, err);
+        tiles_issuer<T, D>(tmem, castdev::smem_u32(smem), n_kv, q_full, k_full, v_full, s_full, p_full, pv_done, k_free, v_free, err);
         castdev::tc_commit(mma_drain);
         castdev::mbar_wait_drain(mma_drain, 0, err);
       }
     }
   } else {
     // ------------------------------------------------------------ softmax
-    regs_inc<kTilesRegsSoft>();
+    regs_inc<S::regs_soft>();
     const int lrow = warp * 32 + lane;
     const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
     const uint32_t o_addr = tmem + lane_off;
-    const uint32_t s_addr = tmem + lane_off + 128;
+    const uint32_t s_addr = tmem + lane_off + S::s_col;
     const int my_steps = n_kv;
     const int row = row0 + lrow;
     const bool row_valid = row < p.rows;
@@ -499,7 +534,6 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
     bool ok = true;
     const float c2 = p.scale_log2;
     for (int h = 0; h < my_steps; ++h) {
-      const int half = h & 1;
       const int n0 = kt_lo * KT + h * 64;
       const bool full_step = n0 + 64 <= w_near_lo || (n0 >= w_from_hi && n0 + 64 <= w_to_lo);
       const bool empty_step = n0 >= w_near_hi && (n0 + 64 <= w_from_lo || n0 >= w_to_hi);
@@ -509,62 +543,99 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
         for (int w = 0; w < 2; ++w)
           seen[w] = interval_mask(0, near, n0 + 32 * w) | interval_mask(from, to, n0 + 32 * w);
       }
-      ok = __all_sync(0xffffffffu, castdev::mbar_wait(&s_full[half], (h >> 1) & 1, err));
+      ok = __all_sync(0xffffffffu, castdev::mbar_wait(&s_full[S::buf(h)], S::phase(h), err));
       if (!ok) break;
       castdev::tc_fence_after();
-      const uint32_t sb = s_addr + 64 * half;
-      uint32_t v[64];
+      const uint32_t sb = s_addr + 64 * S::buf(h);
       float sum = 0.0f;
-      if (empty_step) {
-#pragma unroll
-        for (int c = 0; c < 32; ++c) v[c] = 0u;
-      } else {
-        // One pass against the running maximum; where that is not set yet, or a
-        // sum passes its limit, the maximum is found and the pass made again
-        // (the same code: the loop has to stay in the instruction cache).
-        bool find = __any_sync(0xffffffffu, m_run == -INFINITY);
-        for (;;) {
-          castdev::tmem_ld32(sb, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-          castdev::tmem_ld32(sb + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
-          tmem_wait_ld64(v);
-          if (__builtin_expect(find, 0)) {
-            const float m_step = row_max<false, true>(v, seen, c2);
-            float o_scale = 1.0f;
-            if (m_step > m_run + X::kSlack || m_run == -INFINITY) {
-              const float m_new = fmaxf(m_run, m_step);
-              o_scale = (m_run == -INFINITY) ? (m_new == -INFINITY ? 1.0f : 0.0f) : fast_exp2(m_run - m_new);
-              l_run *= o_scale;
-              m_run = m_new;
-            }
-            if (h > 0 && __any_sync(0xffffffffu, o_scale != 1.0f)) {
-              const int hp = h - 1;
-              ok = __all_sync(0xffffffffu, castdev::mbar_wait(&pv_done[hp & 1], (hp >> 1) & 1, err));
-              if (!ok) break;
-              castdev::tc_fence_after();
+      // Raises the running maximum to a row's mx where that is above it by more
+      // than the slack, and scales what is relative to it: l, O and the sum of
+      // this step.  The maximum is a whole number, so all of that, P included,
+      // is scaled by powers of two.  Returns the scale (1: not raised).
+      auto raise = [&](float mx) -> float {
+        float f = 1.0f;
+        if (mx > m_run + X::kSlack || m_run == -INFINITY) {
+          const float m_new = fmaxf(m_run, ceilf(mx));
+          f = (m_run == -INFINITY) ? (m_new == -INFINITY ? 1.0f : 0.0f) : fast_exp2(m_run - m_new);
+          l_run *= f;
+          sum *= f;
+          m_run = m_new;
+        }
+        if (h > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
+          ok = __all_sync(0xffffffffu, castdev::mbar_wait(&pv_done[S::buf(h - 1)], S::phase(h - 1), err));
+          if (ok) {
+            castdev::tc_fence_after();
 #pragma unroll 1
-              for (int cc = 0; cc < D / 32; ++cc) {
-                uint32_t o[32];
-                castdev::tmem_ld32(o_addr + 32 * cc, o);
-                castdev::tmem_wait_ld();
+            for (int cc = 0; cc < D / 32; ++cc) {
+              uint32_t o[32];
+              tmem_get(o_addr + 32 * cc, o);
 #pragma unroll
-                for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * o_scale);
-                castdev::tmem_st32(o_addr + 32 * cc, o);
-              }
+              for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
+              tmem_put(o_addr + 32 * cc, o);
             }
           }
-          const float base = (m_run == -INFINITY) ? 0.0f : m_run - X::kShift;
-          sum = full_step ? tiles_probs<T, false>(v, seen, c2, base) : tiles_probs<T, true>(v, seen, c2, base);
-          if (find || !__any_sync(0xffffffffu, !(sum <= X::kSumLimit))) break;
-          find = true;
+        }
+        return f;
+      };
+      auto find = [&](uint32_t addr, int words, const uint32_t *w) -> float {  // maximum of 32 * words scores in TMEM
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int q = 0; q < words; ++q) {
+          uint32_t x[32];
+          tmem_get(addr + 32 * q, x);
+          mx = fmaxf(mx, tiles_max(x, q ? w[1] : w[0], c2));
+        }
+        return mx;
+      };
+      if (empty_step) {
+        const uint32_t zero[16] = {};
+        tmem_put(sb, zero);
+        tmem_put(sb + 16, zero);
+      } else {
+        if (__builtin_expect(__any_sync(0xffffffffu, m_run == -INFINITY), 0)) raise(find(sb, 2, seen));
+        // A chunk of columns at a time.  P of the first chunk goes over scores
+        // that have been read.
+#pragma unroll 1
+        for (int q = 0; q < 64 / S::chunk; ++q) {
+          uint32_t x[S::chunk], pk[S::chunk / 2], mine[S::chunk / 32];
+          if constexpr (S::chunk == 64) {
+            mine[0] = seen[0], mine[1] = seen[1];
+          } else {
+            mine[0] = q ? seen[1] : seen[0];
+          }
+          float part;
+          for (bool again = false;;) {
+            tmem_get(sb + S::chunk * q, x);
+            const float base = (m_run == -INFINITY) ? 0.0f : m_run - X::kShift;
+            part = full_step ? tiles_probs<T, false, S::chunk>(x, pk, mine, c2, base)
+                             : tiles_probs<T, true, S::chunk>(x, pk, mine, c2, base);
+            if (again || !__any_sync(0xffffffffu, !(part <= X::kSumLimit))) break;
+            // some weights are too large against a maximum that is behind: it
+            // is found, and the pass made again
+            const float f = raise(find(sb + S::chunk * q, S::chunk / 32, mine));
+            if (S::chunk == 32 && q == 1) {  // the first chunk's P, already stored
+              uint32_t w[16];
+              castdev::tmem_wait_st();
+              tmem_get(sb, w);
+#pragma unroll
+              for (int c = 0; c < 16; ++c) {
+                const float2 y = Half2<T>::unpack(w[c]);
+                w[c] = X::pack(y.x * f, y.y * f);
+              }
+              tmem_put(sb, w);
+            }
+            again = true;
+          }
+          tmem_put(sb + S::chunk / 2 * q, pk);
+          sum += part;
         }
         if (!ok) break;
       }
-      castdev::tmem_st32(sb, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
       l_run += sum;
       castdev::tmem_wait_st();
       castdev::tc_fence_before();
       __syncwarp();
-      if (lane == 0) castdev::mbar_arrive(&p_full[half]);
+      if (lane == 0) castdev::mbar_arrive(&p_full[S::buf(h)]);
     }
     if (hi == 0) {  // a row that sees nothing is nothing (and its maximum is none)
       m_run = -INFINITY;
@@ -573,7 +644,7 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
     // ------------------------------------------------------------ epilogue
     if (ok && my_steps > 0) {
       const int hl = my_steps - 1;
-      ok = __all_sync(0xffffffffu, castdev::mbar_wait(&pv_done[hl & 1], (hl >> 1) & 1, err));
+      ok = __all_sync(0xffffffffu, castdev::mbar_wait(&pv_done[S::buf(hl)], S::phase(hl), err));
       castdev::tc_fence_after();
     }
     {
@@ -651,7 +722,7 @@ __global__ void __launch_bounds__(kTilesThreads, 2)
   __syncthreads();
   if (warp == kMWarp) {
     castdev::tc_fence_after();
-    castdev::tmem_dealloc(tmem, 256);
+    castdev::tmem_dealloc(tmem, S::tmem_cols);
   }
 }
 
