@@ -1160,7 +1160,7 @@ struct RotaryPositions {
 
 // Checks shared by both entry points and the parameters they share.
 static int rotary_params(castk::RotaryParams &p, const RotaryPositions &at, int B, int L, int heads,
-                         int D, int R, int flags) {
+                         int D, int R, int flags, bool norm, bool even) {
   if (B <= 0 || L <= 0 || heads <= 0) return fail(CAST_ERR_INVALID_ARGUMENT, "non-positive size");
   if (L > (1 << 30) || B > (1 << 30)) return fail(CAST_ERR_UNSUPPORTED, "%d x %d tokens in one call", B, L);
   if (D <= 0 || D % 8 || D > 256)
@@ -1202,30 +1202,58 @@ static int rotary_params(castk::RotaryParams &p, const RotaryPositions &at, int 
   p.R = R;
   p.inv_d = 1.0f / (float)D;
   p.inverse = (flags >> 1) & 1;
-  p.lanes = 8;
-  while (p.lanes < D / 8) p.lanes *= 2;
+  // A lane of one piece of eight columns or of two, and how many heads of a
+  // token it takes.  With the norm, two pieces halve what a head costs beside
+  // its values (reduction, root, addresses), and a lane takes eight heads or
+  // more, so that position and table row are paid once for them: 16 + 16 heads
+  // of 128 in 53.1 us (12500 tokens) against 59.4 with one piece, 32 + 8 with
+  // pages in 69.6 against 91.6.  Where one batch of three one-piece heads a
+  // lane is all of q, and all of k, one piece over as many lanes as there are
+  // is better: 24 + 24 heads in 48.7 us against 56.2.  Without the norm one piece is
+  // (66 against 74 us for 31680 tokens of 24 heads), and it has to be where the
+  // half layout's pairs are not half a head apart.
+  p.pieces = norm && D % 16 == 0 && (!half || R == D || R == 0) && !even ? 2 : 1;
+  p.lanes = p.pieces == 2 ? 4 : 8;
+  while (p.lanes * p.pieces * 8 < D) p.lanes *= 2;
   const int groups = castk::kRotaryThreads / p.lanes;
   p.slots_per_token = 1, p.slots_log2 = 0;
   while (p.slots_per_token < groups && p.slots_per_token < heads) p.slots_per_token *= 2, ++p.slots_log2;
+  auto ctas = [&](int slots, int run) { return (long long)B * ceil_div(L, groups / slots * run); };
+  while (!(norm && even) && p.slots_per_token > 1 && heads / p.slots_per_token < 8 &&
+         ctas(p.slots_per_token / 2, 1) >= 148 * 7)
+    p.slots_per_token /= 2, --p.slots_log2;
   // A CTA takes the tokens its lanes have room for, and up to kRotaryRun times
   // as many one after the other while the grid still fills the device.
   const int at_once = groups >> p.slots_log2;
   int run = 1;
-  while (run < castk::kRotaryRun && (long long)B * (L / (at_once * run * 2)) >= 148 * 16) run *= 2;
+  while (run < castk::kRotaryRun && ctas(p.slots_per_token, 2 * run) >= 148 * 16) run *= 2;
   p.tokens_per_cta = at_once * run;
   return CAST_OK;
 }
 
-template <typename InT, typename OutT, bool kNorm, bool kHalf>
-static int launch_rotary(const castk::RotaryParams &p, cudaStream_t s) {
+template <typename InT, typename OutT, bool kNorm, bool kHalf, int kC, int kLanes>
+static void launch_rotary_lanes(const castk::RotaryParams &p, cudaStream_t s) {
   const int by = std::min(p.B, 32768);
   const dim3 grid((unsigned)ceil_div(p.L, p.tokens_per_cta), (unsigned)by, (unsigned)ceil_div(p.B, by));
-  if (p.lanes == 8)
-    castk::rotary_kernel<InT, OutT, kNorm, kHalf, 8><<<grid, castk::kRotaryThreads, 0, s>>>(p);
-  else if (p.lanes == 16)
-    castk::rotary_kernel<InT, OutT, kNorm, kHalf, 16><<<grid, castk::kRotaryThreads, 0, s>>>(p);
-  else
-    castk::rotary_kernel<InT, OutT, kNorm, kHalf, 32><<<grid, castk::kRotaryThreads, 0, s>>>(p);
+  castk::rotary_kernel<InT, OutT, kNorm, kHalf, kC, kLanes><<<grid, castk::kRotaryThreads, 0, s>>>(p);
+}
+
+template <typename InT, typename OutT, bool kNorm, bool kHalf>
+static int launch_rotary(const castk::RotaryParams &p, cudaStream_t s) {
+  if (p.pieces == 2) {
+    if (p.lanes == 4)
+      launch_rotary_lanes<InT, OutT, kNorm, kHalf, 2, 4>(p, s);
+    else if (p.lanes == 8)
+      launch_rotary_lanes<InT, OutT, kNorm, kHalf, 2, 8>(p, s);
+    else
+      launch_rotary_lanes<InT, OutT, kNorm, kHalf, 2, 16>(p, s);
+  } else if (p.lanes == 8) {
+    launch_rotary_lanes<InT, OutT, kNorm, kHalf, 1, 8>(p, s);
+  } else if (p.lanes == 16) {
+    launch_rotary_lanes<InT, OutT, kNorm, kHalf, 1, 16>(p, s);
+  } else {
+    launch_rotary_lanes<InT, OutT, kNorm, kHalf, 1, 32>(p, s);
+  }
   CAST_CUDA_TRY(cudaGetLastError());
   return CAST_OK;
 }
@@ -1264,7 +1292,7 @@ extern "C" int cast_rope(const void *x, int dtype, const float *table, int table
   if (!dtype_ok(dtype)) return fail(CAST_ERR_INVALID_ARGUMENT, "dtype %d (0 = bf16, 1 = fp32, 2 = fp16)", dtype);
   castk::RotaryParams p;
   int st = rotary_params(p, {table, table_rows, positions, positions_64, pos_batch_stride, first_position, axes},
-                         B, L, H, D, R, flags);
+                         B, L, H, D, R, flags, false, false);
   if (st) return st;
   if (!aligned16(x) || !aligned16(out) || !strides_ok(strides, 6, dtype))
     return fail(CAST_ERR_ALIGNMENT, "x and out must start, and their strides step, on 16-byte boundaries");
@@ -1293,9 +1321,12 @@ extern "C" int cast_qk_norm_rope(const void *q, const void *k, const void *v, in
     return fail(CAST_ERR_INVALID_ARGUMENT, "%d query and %d key heads", Hq, Hk);
   if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(CAST_ERR_INVALID_ARGUMENT, "eps must be finite, 0 or more");
   if (slots && (n_pages <= 0 || page <= 0)) return fail(CAST_ERR_INVALID_ARGUMENT, "non-positive cache size");
+  // three heads of one piece a lane, in one batch (see rotary_params)
+  const int wide = 3 * castk::kRotaryThreads / (D <= 64 ? 8 : (D <= 128 ? 16 : 32));
+  const bool filled = Hq == wide && Hk == wide && !v;
   castk::RotaryParams p;
   int st = rotary_params(p, {table, table_rows, positions, positions_64, pos_batch_stride, first_position, axes},
-                         B, L, Hq + (v ? 2 : 1) * Hk, D, R, flags);
+                         B, L, Hq + (v ? 2 : 1) * Hk, D, R, flags, q_weight || k_weight, filled);
   if (st) return st;
   if (!aligned16(q) || !aligned16(k) || (v && !aligned16(v)) || !aligned16(q_out) || !aligned16(k_out) ||
       (v_out && !aligned16(v_out)) || (q_weight && !aligned16(q_weight)) || (k_weight && !aligned16(k_weight)) ||

@@ -11,13 +11,15 @@
 // position has lost the turn's fraction.  Norm, rotation and sums are float32;
 // the result is rounded to the output type once.
 //
-// Bound: HBM.  Every value is read and written once, in 16-byte pieces of
-// eight values (two for float32), one lane a piece, so a head is a group of
-// 8, 16 or 32 lanes of one warp: its sum of squares is a shuffle reduction and
-// the half layout's partner values are a shuffle away, with no shared memory.
+// Bound: HBM, if instructions do not come first.  Every value is read and
+// written once, in 16-byte pieces of eight values (two for float32), and a head
+// is a group of 4 to 32 lanes of one warp, so its sum of squares is a shuffle
+// reduction.  A lane has two pieces, half a head apart, where it can (the pairs
+// of the half layout are then its own), else one, and a partner's values are a
+// shuffle away.  No shared memory.
 // A lane keeps the same eight columns for every head of its token, so the
 // table row is read once per token and lane and its (c, s) stay in registers;
-// kRotaryBatch heads are loaded before the first is worked on.
+// a few heads are loaded before the first is worked on.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -35,13 +37,12 @@ __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
 }
 
 constexpr int kRotaryThreads = 128;
-#ifndef ROT_BATCH
-#define ROT_BATCH 3
-#define ROT_RUN 4
-#define ROT_MINB 8
-#endif
-constexpr int kRotaryBatch = ROT_BATCH;  // heads in flight per lane
-constexpr int kRotaryRun = ROT_RUN;    // tokens a lane takes one after the other
+constexpr int kRotaryRun = 4;  // tokens a lane takes one after the other
+// Heads in flight per lane of one piece or two, and CTAs on an SM: registers
+// for more of either cost more than they give (one piece: 4 heads and 6 CTAs
+// are level; two pieces: 3 heads and 6 CTAs take 94 us where 2 and 7 take 69).
+constexpr int rotary_batch(int pieces) { return pieces == 2 ? 2 : 3; }
+constexpr int rotary_ctas(int pieces) { return pieces == 2 ? 7 : 8; }
 
 // One tensor of a call: q, k and (copied only) v.
 struct RotaryTensor {
@@ -63,7 +64,7 @@ struct RotaryParams {
   int table_rows, pos64, slots64, n_axes, axis_end0, axis_end1;
   int page;
   int B, L, D, R;
-  int lanes;                        // of one head: 8, 16 or 32
+  int pieces, lanes;                // of eight values to a lane (1 or 2); lanes of one head
   int slots_per_token, slots_log2;  // heads of one token at once, a power of two
   int tokens_per_cta;
   int inverse, weight_f32, weight_per_head;
@@ -131,104 +132,138 @@ __device__ __forceinline__ long long load_index(const void *p, int is64, long lo
               : (long long)__ldg(static_cast<const int32_t *>(p) + i);
 }
 
-// One tensor's heads of one token: this lane's eight columns of the heads
-// h0, h0 + step, ... below t.heads.  `turn`: rotate (q and k); `at`: the
-// destination row of head 0, nullptr: nothing is written.
-template <typename InT, typename OutT, bool kNorm, bool kHalf, int kLanes>
+// A lane's columns of a head: kC pieces of eight, 8 c and, with two, D / 2 + 8 c
+// (which then holds the other values of its pairs in the half layout).
+template <typename InT, typename OutT, bool kNorm, bool kHalf, int kC, int kLanes>
 struct RotaryLane {
-  static constexpr int kPairs = kHalf ? 8 : 4;  // table entries of a lane's eight columns
+  static constexpr int kBatch = rotary_batch(kC);
+  static constexpr int kPairs = kHalf ? 8 : 4 * kC;  // table entries of a lane's columns
   float cs[kPairs], sn[kPairs];
-  bool live, turns;
+  bool live, turns[kC];
   bool blank;  // this token's position is unknown: its q and k are zeros
-  int c, h0, step, partner;
+  int c, h0, step, partner, second;  // second: columns from the first piece to the second
 
   template <bool kBlank>
   __device__ __forceinline__ void load(const RotaryParams &p, const RotaryTensor &t, const InT *row, int hb,
-                                       Eight<InT> (&raw)[kRotaryBatch]) const {
+                                       Eight<InT> (&raw)[kBatch][kC]) const {
     const InT *src = row + (long long)(hb + h0) * t.ss[2];
 #pragma unroll
-    for (int u = 0; u < kRotaryBatch; ++u) {
-      if (live && hb + u * step + h0 < t.heads) raw[u].load(src);
+    for (int u = 0; u < kBatch; ++u) {
+      if (live && hb + u * step + h0 < t.heads) {
+#pragma unroll
+        for (int j = 0; j < kC; ++j) raw[u][j].load(src + j * second);
+      }
       src += step * t.ss[2];
     }
-    if (kBlank && blank) {
+    if (kBlank && blank) clear(raw);
+  }
+  __device__ __forceinline__ void clear(Eight<InT> (&raw)[kBatch][kC]) const {
 #pragma unroll
-      for (int u = 0; u < kRotaryBatch; ++u) raw[u] = Eight<InT>{};
-    }
+    for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+      for (int j = 0; j < kC; ++j) raw[u][j] = Eight<InT>{};
   }
 
+  // One tensor's heads of one token, h0, h0 + step, ... below t.heads.  kTurn:
+  // norm and rotate (q and k); at: the destination of head 0, nullptr: nothing
+  // is written.
   template <bool kTurn>
   __device__ __forceinline__ void run(const RotaryParams &p, const RotaryTensor &t, const InT *row, OutT *at,
-                                      long long at_step, Eight<InT> (&raw)[kRotaryBatch]) const {
-    uint64_t w[4];  // the weight's eight values, in pairs
+                                      long long at_step, Eight<InT> (&raw)[kBatch][kC]) const {
+    uint64_t w[4 * kC];  // the weight's values, in pairs
     auto weight = [&](int h) {
       const long long wo = (p.weight_per_head ? (long long)h * p.D : 0) + 8 * c;
-      float f[8];
-      if (p.weight_f32) {
-        Eight<float> e;
-        e.load(static_cast<const float *>(t.weight) + wo);
-        e.values(f);
-      } else {
-        Eight<InT> e;
-        e.load(static_cast<const InT *>(t.weight) + wo);
-        e.values(f);
-      }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = f2_pack(f[2 * i], f[2 * i + 1]);
+      for (int j = 0; j < kC; ++j) {
+        float f[8];
+        if (p.weight_f32) {
+          Eight<float> e;
+          e.load(static_cast<const float *>(t.weight) + wo + j * second);
+          e.values(f);
+        } else {
+          Eight<InT> e;
+          e.load(static_cast<const InT *>(t.weight) + wo + j * second);
+          e.values(f);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[4 * j + i] = f2_pack(f[2 * i], f[2 * i + 1]);
+      }
     };
     const bool normed = kNorm && kTurn && t.weight != nullptr;
     if (normed && live && !p.weight_per_head) weight(0);
-    for (int hb = 0; hb < t.heads; hb += step * kRotaryBatch) {  // same trip count in the whole CTA
+    for (int hb = 0; hb < t.heads; hb += step * kBatch) {  // same trip count in the whole CTA
       if (hb > 0) load<kTurn>(p, t, row, hb, raw);
       OutT *dst = at + (long long)(hb + h0) * at_step;
 #pragma unroll
-      for (int u = 0; u < kRotaryBatch; ++u, dst += step * at_step) {
-        if (hb + u * step >= t.heads) break;  // uniform
+      for (int u = 0; u < kBatch; ++u, dst += step * at_step) {
         const int h = hb + u * step + h0;
         const bool on = live && h < t.heads;
-        float x[8];  // (lanes without a head compute what they hold and write nothing)
-        raw[u].values(x);
-        if (normed) {
-          uint64_t x2[4], sum2 = 0;
+        float x[kC][8];  // (lanes without a head compute what they hold and write nothing)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            x2[i] = f2_pack(x[2 * i], x[2 * i + 1]);
-            sum2 = f2_fma(x2[i], x2[i], sum2);
-          }
+        for (int j = 0; j < kC; ++j) raw[u][j].values(x[j]);
+        if (normed) {
+          uint64_t sum2 = 0;
+#pragma unroll
+          for (int j = 0; j < kC; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint64_t v = f2_pack(x[j][2 * i], x[j][2 * i + 1]);
+              sum2 = f2_fma(v, v, sum2);
+            }
           float lo, hi;
           f2_unpack(sum2, lo, hi);
           float sum = lo + hi;
 #pragma unroll
           for (int s = kLanes / 2; s >= 1; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-          const float r = rsqrtf(fmaf(sum, p.inv_d, p.eps));
+          const float r = blank ? 0.0f : rsqrtf(fmaf(sum, p.inv_d, p.eps));
           const uint64_t r2 = f2_pack(r, r);
           if (p.weight_per_head && on) weight(h);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) f2_unpack(f2_mul(f2_mul(x2[i], r2), w[i]), x[2 * i], x[2 * i + 1]);
+          for (int j = 0; j < kC; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              f2_unpack(f2_mul(f2_mul(f2_pack(x[j][2 * i], x[j][2 * i + 1]), r2), w[4 * j + i]), x[j][2 * i], x[j][2 * i + 1]);
         }
-        if (kTurn && kHalf) {
+        if constexpr (kTurn && kHalf && kC == 2) {
+          if (turns[0]) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float a = x[0][i], q = x[1][i];
+              x[0][i] = fmaf(a, cs[i], -(q * sn[i]));
+              x[1][i] = fmaf(a, sn[i], q * cs[i]);
+            }
+          }
+        } else if constexpr (kTurn && kHalf) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float o = __shfl_sync(0xffffffffu, x[i], partner);
-            if (turns) x[i] = fmaf(x[i], cs[i], o * sn[i]);
+            const float o = __shfl_sync(0xffffffffu, x[0][i], partner);
+            if (turns[0]) x[0][i] = fmaf(x[0][i], cs[i], o * sn[i]);
           }
-        } else if (kTurn && turns) {
+        } else if constexpr (kTurn) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float a = x[2 * i], q = x[2 * i + 1];
-            x[2 * i] = fmaf(a, cs[i], -(q * sn[i]));
-            x[2 * i + 1] = fmaf(a, sn[i], q * cs[i]);
+          for (int j = 0; j < kC; ++j) {
+            if (turns[j]) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float a = x[j][2 * i], q = x[j][2 * i + 1];
+                x[j][2 * i] = fmaf(a, cs[4 * j + i], -(q * sn[4 * j + i]));
+                x[j][2 * i + 1] = fmaf(a, sn[4 * j + i], q * cs[4 * j + i]);
+              }
+            }
           }
         }
-        if (on && at) store8(dst, x);
+        if (on && at) {
+#pragma unroll
+          for (int j = 0; j < kC; ++j) store8(dst + j * second, x[j]);
+        }
       }
     }
   }
 };
 
-template <typename InT, typename OutT, bool kNorm, bool kHalf, int kLanes>
-__global__ void __launch_bounds__(kRotaryThreads, ROT_MINB) rotary_kernel(const __grid_constant__ RotaryParams p) {
-  RotaryLane<InT, OutT, kNorm, kHalf, kLanes> f;
+template <typename InT, typename OutT, bool kNorm, bool kHalf, int kC, int kLanes>
+__global__ void __launch_bounds__(kRotaryThreads, rotary_ctas(kC)) rotary_kernel(const __grid_constant__ RotaryParams p) {
+  RotaryLane<InT, OutT, kNorm, kHalf, kC, kLanes> f;
   constexpr int kPairs = f.kPairs;
   int *err = &g_cast_device_error;
   f.c = threadIdx.x & (kLanes - 1);
@@ -238,9 +273,11 @@ __global__ void __launch_bounds__(kRotaryThreads, ROT_MINB) rotary_kernel(const 
   const int b = blockIdx.y + blockIdx.z * gridDim.y;
   if (b >= p.B) return;  // (whole CTAs)
   const int half_pairs = p.R >> 1, half_chunks = p.R >> 4;
-  const int pair0 = kHalf ? (c < half_chunks ? 8 * c : 8 * (c - half_chunks)) : 4 * c;
-  const bool flip = (p.inverse != 0) != (kHalf && c < half_chunks);
-  f.partner = kHalf ? (((threadIdx.x & 31) - c + (c < half_chunks ? c + half_chunks : c - half_chunks)) & 31) : 0;
+  f.second = p.D >> 1;
+  // first pair of each piece (two pieces in the half layout have the same pairs)
+  const int pair0 = kHalf ? (kC == 2 || c < half_chunks ? 8 * c : 8 * (c - half_chunks)) : 4 * c;
+  const bool flip = (p.inverse != 0) != (kHalf && kC == 1 && c < half_chunks);
+  f.partner = kHalf && kC == 1 ? (((threadIdx.x & 31) - c + (c < half_chunks ? c + half_chunks : c - half_chunks)) & 31) : 0;
 
   const InT *src[3];
   OutT *dst[3];
@@ -249,14 +286,19 @@ __global__ void __launch_bounds__(kRotaryThreads, ROT_MINB) rotary_kernel(const 
     src[i] = static_cast<const InT *>(p.t[i].src) + b * p.t[i].ss[0] + 8 * c;
     dst[i] = static_cast<OutT *>(p.t[i].dst) + b * p.t[i].ds[0] + 8 * c;
   }
-  Eight<InT> raw[kRotaryBatch] = {};  // zeros where a lane has no column: they enter a head's sum
+  Eight<InT> raw[rotary_batch(kC)][kC] = {};  // zeros where a lane has no column: they enter a head's sum
   const int l_end = min(p.L, (int)(blockIdx.x + 1) * p.tokens_per_cta);
   for (int l = blockIdx.x * p.tokens_per_cta + (group >> p.slots_log2);; l += (kRotaryThreads / kLanes) >> p.slots_log2) {
     // the lanes of a warp may have different tokens: it leaves together
     if (!__any_sync(0xffffffffu, l < l_end)) break;
     const bool live_token = l < l_end;
-    f.live = live_token && 8 * c < p.D;
-    f.turns = f.live && 8 * c < p.R;
+    f.live = live_token && 8 * kC * c < p.D;
+    bool any_turns = false;
+#pragma unroll
+    for (int j = 0; j < kC; ++j) {
+      f.turns[j] = f.live && (kHalf && kC == 2 ? p.R > 0 : 8 * c + j * f.second < p.R);
+      any_turns = any_turns || f.turns[j];
+    }
 
     // on its way while the position and then its table row are fetched
     f.blank = false;
@@ -291,27 +333,31 @@ __global__ void __launch_bounds__(kRotaryThreads, ROT_MINB) rotary_kernel(const 
           pos[0] = pos[1] = pos[2] = 0;
           if (c == 0 && f.h0 == 0) atomicExch(err, (int)CAST_ERR_INVALID_ARGUMENT);
           f.blank = true;
-#pragma unroll
-          for (int u = 0; u < kRotaryBatch; ++u) raw[u] = Eight<InT>{};
+          f.clear(raw);
         }
       }
-      if (f.turns) {
-        const float2 *tab = reinterpret_cast<const float2 *>(p.table) + pair0;
-        if (p.n_axes == 1) {
-          const float4 *row = reinterpret_cast<const float4 *>(tab + pos[0] * half_pairs);
+      if (any_turns) {
+        constexpr int kPieces = kHalf ? 1 : kC, kEach = kHalf ? 8 : 4;  // runs of pairs
 #pragma unroll
-          for (int i = 0; i < kPairs / 2; ++i) {
-            const float4 w = __ldg(row + i);
-            f.cs[2 * i] = w.x, f.sn[2 * i] = w.y, f.cs[2 * i + 1] = w.z, f.sn[2 * i + 1] = w.w;
-          }
-        } else {
-          const float2 *row[3];
+        for (int j = 0; j < kPieces; ++j) {
+          const int first = pair0 + j * (f.second >> 1);
+          if (kPieces > 1 && !f.turns[j]) continue;
+          const float2 *tab = reinterpret_cast<const float2 *>(p.table) + first;
+          if (p.n_axes == 1) {
+            const float4 *row = reinterpret_cast<const float4 *>(tab + pos[0] * half_pairs);
 #pragma unroll
-          for (int a = 0; a < 3; ++a) row[a] = tab + pos[a] * half_pairs;
+            for (int i = 0; i < kEach / 2; ++i) {
+              const float4 w = __ldg(row + i);
+              f.cs[kEach * j + 2 * i] = w.x, f.sn[kEach * j + 2 * i] = w.y;
+              f.cs[kEach * j + 2 * i + 1] = w.z, f.sn[kEach * j + 2 * i + 1] = w.w;
+            }
+          } else {
 #pragma unroll
-          for (int i = 0; i < kPairs; ++i) {
-            const float2 w = __ldg((pair0 + i < p.axis_end0 ? row[0] : pair0 + i < p.axis_end1 ? row[1] : row[2]) + i);
-            f.cs[i] = w.x, f.sn[i] = w.y;
+            for (int i = 0; i < kEach; ++i) {
+              const int r = first + i < p.axis_end0 ? pos[0] : first + i < p.axis_end1 ? pos[1] : pos[2];
+              const float2 w = __ldg(tab + r * half_pairs + i);
+              f.cs[kEach * j + i] = w.x, f.sn[kEach * j + i] = w.y;
+            }
           }
         }
         // (kHalf: the second value of a pair takes y_b = z_b c + z_a s, the first y_a = z_a c - z_b s)
