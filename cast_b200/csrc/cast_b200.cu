@@ -1349,6 +1349,18 @@ extern "C" int cast_qk_norm_rope(const void *q, const void *k, const void *v, in
 // ===========================================================================
 // sliding-window attention with sinks
 // ===========================================================================
+// Raises a kernel's dynamic shared memory limit on the current device, once
+// for each device (`done`: a bit for each).
+static int allow_smem(const void *kernel, int bytes, std::atomic<unsigned long long> &done) {
+  int dev = 0;
+  CAST_CUDA_TRY(cudaGetDevice(&dev));
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (bit && (done.load(std::memory_order_acquire) & bit)) return CAST_OK;
+  CAST_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit, std::memory_order_release);
+  return CAST_OK;
+}
+
 struct RowsPlan {
   int mt = 1, row_tiles = 1, n_split = 1;
   bool cluster = false;  // joined in a cluster (else through the workspace, or nothing to join)
@@ -1390,12 +1402,9 @@ template <typename T, int D, int MT, bool kPaged>
 static int launch_rows(const castk::RowsParams &p, const RowsPlan &plan, cudaStream_t s) {
   using S = castk::RowsSmem<T, D, MT, kPaged>;
   auto kernel = castk::window_rows_kernel<T, D, MT, kPaged>;
-  static std::once_flag once;
-  static cudaError_t err = cudaSuccess;
-  std::call_once(once, [&] {
-    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes);
-  });
-  CAST_CUDA_TRY(err);
+  static std::atomic<unsigned long long> done{0};
+  const int st = allow_smem(reinterpret_cast<const void *>(kernel), S::bytes, done);
+  if (st) return st;
   const long long items = (long long)p.B * p.Hk * p.row_tiles;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(items * p.n_split));
@@ -1630,13 +1639,14 @@ static int launch_tiles(const castk::RowsParams &r, const TilesPlan &plan, int d
   }
   auto kernel = castk::window_tiles_kernel<T, D>;
   constexpr int smem = castk::TilesSmem<D>::alloc;
-  static std::once_flag once;
+  static std::atomic<unsigned long long> done{0};
+  if ((st = allow_smem(reinterpret_cast<const void *>(kernel), smem, done))) return st;
+  static std::once_flag once;  // (the same code on every device)
   static cudaError_t err = cudaSuccess;
   static int regs = 0;
   std::call_once(once, [&] {
-    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     cudaFuncAttributes fa;
-    if (err == cudaSuccess) err = cudaFuncGetAttributes(&fa, kernel);
+    err = cudaFuncGetAttributes(&fa, kernel);
     if (err == cudaSuccess) regs = fa.numRegs;
   });
   CAST_CUDA_TRY(err);

@@ -724,7 +724,7 @@ template <typename T, int D, int MT, bool kPaged>
 __global__ void __launch_bounds__(kRowsJoin * D / 4) window_rows_join_kernel(const __grid_constant__ RowsParams p) {
   constexpr int R = RowsSmem<T, D, MT, kPaged>::rows, kRow = D + 4, kThreads = kRowsJoin * D / 4;
   __shared__ float4 acc_s[kRowsJoin][D / 4];
-  __shared__ float red_s[2][kThreads / 32];
+  __shared__ float max_s[kThreads / 32], sum_s[kRowsJoin];
   const int item = blockIdx.x / R, r = blockIdx.x % R;
   const int bh = p.by_tiles.div(item), rt = item - bh * p.row_tiles;
   const int b = p.by_hk.div(bh), hk = bh - b * p.Hk;
@@ -738,10 +738,10 @@ __global__ void __launch_bounds__(kRowsJoin * D / 4) window_rows_join_kernel(con
   for (int j = threadIdx.x; j < p.n_split; j += kThreads) m = fmaxf(m, part(j)[D]);
 #pragma unroll
   for (int d = 16; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  if (lane == 0) red_s[0][warp] = m;
+  if (lane == 0) max_s[warp] = m;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) m = fmaxf(m, red_s[0][w]);
+  for (int w = 0; w < kThreads / 32; ++w) m = fmaxf(m, max_s[w]);
   // sums and O
   const int g = threadIdx.x / (D / 4), c = threadIdx.x % (D / 4);
   float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -757,7 +757,7 @@ __global__ void __launch_bounds__(kRowsJoin * D / 4) window_rows_join_kernel(con
     bad = bad || __float_as_int(tail.z) != 0;
   }
   acc_s[g][c] = a;
-  if (c == 0) red_s[1][g] = l;  // (kRowsJoin of them fit: a warp each or two)
+  if (c == 0) sum_s[g] = l;
   const bool any_bad = __syncthreads_or(bad);
   if (g != 0) return;
   float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -766,7 +766,7 @@ __global__ void __launch_bounds__(kRowsJoin * D / 4) window_rows_join_kernel(con
   for (int j = 0; j < kRowsJoin; ++j) {
     const float4 v = acc_s[j][c];
     y[0] += v.x, y[1] += v.y, y[2] += v.z, y[3] += v.w;
-    l += red_s[1][j];
+    l += sum_s[j];
   }
   const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // (a NaN sum stays one)
 #pragma unroll

@@ -261,3 +261,34 @@ def test_rotary_on_another_stream_and_in_a_graph(cuda):
     still.copy_(x)
     g.replay()
     assert torch.equal(y, want) and torch.equal(gq, wq) and torch.equal(gk, wk)
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("b,l,hq,hk,d,r", [(1, 2100, 24, 24, 128, 128), (3, 700, 8, 2, 128, 128), (1, 5000, 3, 1, 64, 32),
+                                           (2, 1500, 16, 16, 64, 64), (1, 4097, 1, 1, 48, 48), (1, 1300, 5, 2, 256, 256),
+                                           (1, 3001, 4, 4, 24, 16 * 1), (1, 9, 2, 1, 40, 32)])
+def test_many_tokens_and_every_lane_layout(cuda, interleaved, b, l, hq, hk, d, r):
+    """The layouts that the launch picks from: one or two pieces a lane, few or many heads a lane, runs of tokens."""
+    f = rotary.rope_frequencies(r)
+    table = rotary.rope_table(f, l + 3)
+    q, k = _x(b, l, hq, d, dtype=torch.bfloat16), _x(b, l, hk, d, dtype=torch.bfloat16, seed=1)
+    w = 1 + _x(d, dtype=torch.float32, seed=2) / 8
+    theta = ora.angles(torch.arange(3, l + 3, device="cuda").expand(b, l), f)
+    for y, x in zip(rotary.qk_norm_rope(q, k, w, w, table, start=3, interleaved=interleaved), (q, k)):
+        z = ora.norm(x, w, 1e-6)
+        _close(y.transpose(1, 2), ora.turn(z, theta, interleaved), ora.pair_size(z, r, interleaved), 20)
+    want = ora.turn(q.double(), theta, interleaved)
+    _close(rotary.rope(q, table, start=3, interleaved=interleaved), want, ora.pair_size(q.double(), r, interleaved), 4)
+    _quiet()
+
+
+def test_unknown_positions_under_the_norm(cuda):
+    table = rotary.rope_table(rotary.rope_frequencies(128), 10)
+    x = _x(1, 4, 8, 128, dtype=torch.bfloat16)
+    w = torch.ones(128, dtype=torch.bfloat16, device="cuda")
+    pos = torch.tensor([3, 10, -1, 9], device="cuda")
+    for eps in (1e-6, 0.0):
+        for y in rotary.qk_norm_rope(x, x[:, :, :2], w, w, table, pos, eps=eps):
+            assert (y[0, :, 1:3] == 0).all() and (y[0, :, 0] != 0).any() and (y[0, :, 3] != 0).any()
+        with pytest.raises(CastError):
+            _quiet()

@@ -314,3 +314,83 @@ def test_a_session_token_by_token(cuda):
     # the chunk's attention over dense keys gives what the pages gave
     dense = window.window_attention(q, k, v, window=win, sinks=sinks)
     _check(dense, q, k, v, None, window=win, sinks=sinks)
+
+
+@pytest.mark.parametrize("d,dtype,lq,hq,hk", [(64, FP16, 1, 2, 1), (64, BF16, 3, 4, 1), (64, BF16, 5, 6, 1),
+                                              (128, FP16, 16, 2, 1)])
+def test_many_parts_of_few_rows(cuda, d, dtype, lq, hq, hk):
+    """More parts than a cluster has, joined by a second launch; 8, 16 and 32 rows a tile."""
+    q, k, v = _data(1, hq, hk, d, lq, 30011, dtype, seed=d + lq)
+    v[0, 0, 30010, 3] = float("inf")  # seen by the last query alone
+    v[0, 0, 5, 2] = float("nan")      # seen by none: behind the window
+    got = window.window_attention(q, k, v, window=30000, sinks=2)
+    _check(got, q, k, v, None, window=30000, sinks=2)
+    kp, vp, table = _pages(k, v, 64)
+    n = torch.tensor([30011], dtype=torch.int32, device="cuda")
+    _check(window.paged_window_attention(q, kp, vp, table, n, window=30000, sinks=2), q, k, v, None, window=30000, sinks=2)
+    _quiet()
+
+
+@pytest.mark.parametrize("d,dtype,hq,hk,lq,lk,lens", [
+    (64, BF16, 4, 2, 90, 9000, None),          # few items: many parts
+    (128, FP16, 2, 1, 100, 9000, [9000, 40]),  # a session with fewer tiles than parts
+    (128, BF16, 24, 24, 1700, 2600, None),     # a last wave in few parts
+    (64, FP16, 24, 24, 3300, 3300, None)])
+def test_parts_of_tiles(cuda, d, dtype, hq, hk, lq, lk, lens):
+    b = 1 if lens is None else len(lens)
+    q, k, v = _data(b, hq, hk, d, lq, lk, dtype, seed=lk)
+    last = lk if lens is None else lens[0]
+    v[0, 0, last - 1, 3] = float("inf")     # seen by the last query alone
+    v[0, 0, last - lq + 1, 5] = float("nan")  # not by the first one
+    n = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    got = window.window_attention(q, k, v, window=None, kv_lens=n)
+    _check(got, q, k, v, lens, window=None, heads=sorted({0, hq // hk - 1, hq - 1}))
+    _quiet()
+
+
+def test_a_maximum_that_rises_all_the_way(cuda):
+    """Every step's scores are far above the last one's: sums, O and weights
+    already stored are scaled again and again."""
+    for dtype in (BF16, FP16):
+        for d in (64, 128):
+            q, k, v = _data(1, 2, 1, d, 130, 700, dtype, seed=d)
+            q.fill_(1.0)
+            ramp = torch.arange(700, device="cuda").float()[:, None] * (200.0 / 700 / d ** 0.5)
+            k[0, 0] = ramp.to(dtype).expand(700, d)
+            for lq in (1, 20, 130):
+                got = window.window_attention(q[:, :, :lq], k, v, window=650, sinks=3)
+                _check(got, q[:, :, :lq], k, v, None, window=650, sinks=3)
+
+
+@pytest.mark.parametrize("lq", [1, 4, 96])
+def test_offsets_past_32_bits(cuda, lq):
+    """Keys of the last head lie more than 2^31 elements (4 GB) in."""
+    hk, lk, d, win = 3, 6 << 20, 128, 300
+    k = torch.empty(1, hk, lk, d, dtype=BF16, device="cuda")
+    v = torch.empty(1, hk, lk, d, dtype=BF16, device="cuda")
+    assert k.numel() > 1 << 31
+    q, kt, vt = _data(1, hk, hk, d, lq, win + lq, BF16, seed=lq)
+    k[:, :, -(win + lq):], v[:, :, -(win + lq):] = kt, vt
+    got = window.window_attention(q, k, v, window=win)
+    _check(got, q, kt, vt, None, window=win)
+    if lq < 96:  # the same memory as a paged cache
+        kp, vp = k.view(-1, hk, 64, d), v.view(-1, hk, 64, d)
+        pages = -(-(win + lq) // 64)
+        for j in range(pages):
+            kp[-1 - j, :, :min(64, win + lq - 64 * j)] = kt[0, :, 64 * j:64 * j + 64]
+            vp[-1 - j, :, :min(64, win + lq - 64 * j)] = vt[0, :, 64 * j:64 * j + 64]
+        table = (kp.shape[0] - 1 - torch.arange(pages, device="cuda")).to(torch.int32)[None]
+        n = torch.tensor([win + lq], dtype=torch.int32, device="cuda")
+        _check(window.paged_window_attention(q, kp, vp, table, n, window=win), q, kt, vt, None, window=win)
+    _quiet()
+
+
+def test_strides_that_tensor_maps_cannot_hold(cuda):
+    """One key for all positions (a stride of 0 along the tokens)."""
+    q, k, v = _data(1, 2, 1, 64, 70, 1, BF16)
+    got = window.window_attention(q, k.expand(1, 1, 200, 64), v.expand(1, 1, 200, 64), window=50)
+    _check(got, q, k.expand(1, 1, 200, 64), v.expand(1, 1, 200, 64), None, window=50)
+    # and of 0 along batch and heads of q: queries that all heads share
+    one = q[:, :1].expand(1, 4, 70, 64)
+    k, v = (t.contiguous() for t in _data(1, 4, 4, 64, 70, 200, BF16)[1:])
+    _check(window.window_attention(one, k, v, window=50), one, k, v, None, window=50)
