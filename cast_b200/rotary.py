@@ -241,8 +241,8 @@ def rope(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor | None = 
         axes = tuple(axes)
     try:
         key = (x.dtype, x.shape, x.stride(), x.device, table.dtype, table.shape, table.stride(), table.device,
-               None if positions is None else _sig(positions), None if out is None else _sig(out), interleaved, axes,
-               inverse, start)
+               None if positions is None else (positions.dtype, positions.shape, positions.stride(), positions.device),
+               None if out is None else _sig(out), interleaved, axes, inverse, start)
         plan = _rope_plans.get(key)
     except AttributeError:
         key = plan = None  # (not a tensor: the checks say so)
@@ -352,7 +352,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
                None if table is None else (table.dtype, table.shape, table.stride(), table.device),
                None if positions is None else (positions.dtype, positions.shape, positions.stride(), positions.device),
                None if out is None else (_sig(qo), _sig(ko)),
-               None if cache is v is slots is None else (_sig(v), _sig(kp), _sig(vp), _sig(slots)),
+               None if cache is v is slots is None else
+               (v.dtype, v.shape, v.stride(), v.device, kp.dtype, kp.shape, kp.stride(), kp.device, vp.dtype, vp.shape,
+                vp.stride(), vp.device, slots.dtype, slots.shape, slots.stride(), slots.device),
                interleaved, axes, start, out_dtype)
         plan = _norm_plans.get(key)
     except AttributeError:
@@ -361,8 +363,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
         plan = _keep(_norm_plans, key, _norm_plan(q, k, q_weight, k_weight, table, positions, interleaved, axes, start,
                                                   out_dtype, qo, ko, v, cache, slots))
     empty, index, out_dtype, q_shape, k_shape, types, weights, rows, rest, places = plan
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or any(
-            t is not None and t.requires_grad for t in (q_weight, k_weight, table, v, kp, vp))):
+    if torch.is_grad_enabled() and (
+            q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)
+            or (k_weight is not None and k_weight.requires_grad) or (table is not None and table.requires_grad)
+            or (cache is not None and (v.requires_grad or kp.requires_grad or vp.requires_grad))):
         _no_gradient()
     if qo is None:
         qo = q.new_empty(q_shape) if out_dtype is q.dtype else q.new_empty(q_shape, dtype=out_dtype)

@@ -106,7 +106,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     """
     try:
         key = (q.dtype, q.shape, q.stride(), q.device, k.dtype, k.shape, k.stride(), k.device, v.dtype, v.shape,
-               v.stride(), v.device, None if kv_lens is None else _sig(kv_lens), None if out is None else _sig(out),
+               v.stride(), v.device,
+               None if kv_lens is None else (kv_lens.dtype, kv_lens.shape, kv_lens.stride(), kv_lens.device),
+               None if out is None else _sig(out),
                window, sinks, frame_tokens)
         plan = _plans.get(key)
     except AttributeError:
@@ -175,7 +177,8 @@ def paged_window_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     try:
         key = (q.dtype, q.shape, q.stride(), q.device, k_pages.dtype, k_pages.shape, k_pages.stride(), k_pages.device,
                v_pages.dtype, v_pages.shape, v_pages.stride(), v_pages.device, block_table.dtype, block_table.shape,
-               block_table.stride(), block_table.device, _sig(kv_lens),
+               block_table.stride(), block_table.device, kv_lens.dtype, kv_lens.shape, kv_lens.stride(),
+               kv_lens.device,
                None if out is None else _sig(out), window, sinks, frame_tokens)
         plan = _paged_plans.get(key)
     except AttributeError:
