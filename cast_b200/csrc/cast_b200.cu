@@ -1208,10 +1208,12 @@ static int rotary_params(castk::RotaryParams &p, const RotaryPositions &at, int 
   // more, so that position and table row are paid once for them: 16 + 16 heads
   // of 128 in 53.1 us (12500 tokens) against 59.4 with one piece, 32 + 8 with
   // pages in 69.6 against 91.6.  Where one batch of three one-piece heads a
-  // lane is all of q, and all of k, one piece over as many lanes as there are
-  // is better: 24 + 24 heads in 48.7 us against 56.2.  Without the norm one piece is
-  // (66 against 74 us for 31680 tokens of 24 heads), and it has to be where the
-  // half layout's pairs are not half a head apart.
+  // lane is all of q, and all of k, and pairs lie side by side, one piece over
+  // as many lanes as there are is better: 24 + 24 heads of 128 in 48.7 us against
+  // 56.2, float32 76.8 against 99.3, 12 + 12 of 256 94.3 against 99.3 (half
+  // layout: 63.4 against 55.5, two batches: level).  Without the norm one piece
+  // is (66 against 74 us for 31680 tokens of 24 heads), and it has to be where
+  // the half layout's pairs are not half a head apart.
   p.pieces = norm && D % 16 == 0 && (!half || R == D || R == 0) && !even ? 2 : 1;
   p.lanes = p.pieces == 2 ? 4 : 8;
   while (p.lanes * p.pieces * 8 < D) p.lanes *= 2;
@@ -1323,7 +1325,7 @@ extern "C" int cast_qk_norm_rope(const void *q, const void *k, const void *v, in
   if (slots && (n_pages <= 0 || page <= 0)) return fail(CAST_ERR_INVALID_ARGUMENT, "non-positive cache size");
   // three heads of one piece a lane, in one batch (see rotary_params)
   const int wide = 3 * castk::kRotaryThreads / (D <= 64 ? 8 : (D <= 128 ? 16 : 32));
-  const bool filled = Hq == wide && Hk == wide && !v;
+  const bool filled = Hq == wide && Hk == wide && !v && (flags & 1);
   castk::RotaryParams p;
   int st = rotary_params(p, {table, table_rows, positions, positions_64, pos_batch_stride, first_position, axes},
                          B, L, Hq + (v ? 2 : 1) * Hk, D, R, flags, q_weight || k_weight, filled);
