@@ -17,9 +17,15 @@
 // reduction.  A lane has two pieces, half a head apart, where it can (the pairs
 // of the half layout are then its own), else one, and a partner's values are a
 // shuffle away.  No shared memory.
-// A lane keeps the same eight columns for every head of its token, so the
-// table row is read once per token and lane and its (c, s) stay in registers;
-// a few heads are loaded before the first is worked on.
+// A lane keeps the same columns for every head of its token, so the table row
+// is read once per token and lane and its (c, s) stay in registers; a few heads
+// are loaded before the first is worked on.
+//
+// Measured (B200, graph over rotating inputs): rotation alone, 31680 tokens of
+// 24 heads of 128 bf16, 65.9 us = 5.9 TB/s, 0.90 of the measured copy; with
+// the norm, 3520 tokens of 24 + 24 heads, 22.7 us = 3.8 TB/s: about 200
+// instructions a head and 16 lanes, where the rotation alone takes 150 (half of
+// it position and table row).
 #pragma once
 
 #include <cuda_fp16.h>
