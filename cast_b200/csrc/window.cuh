@@ -70,7 +70,7 @@ struct WindowSpan {
   __device__ __forceinline__ int key(int v) const { return v < s_n ? v : base + (v - s_n); }
   // whether a key of the list is hidden from some row of the tile
   __device__ __forceinline__ bool some(int key) const {
-    return unplaced || (key >= sinks && (key < lo1 || key >= hi0));
+    return unplaced || key >= hi0 || (key >= sinks && key < lo1);
   }
 };
 

@@ -394,3 +394,18 @@ def test_strides_that_tensor_maps_cannot_hold(cuda):
     one = q[:, :1].expand(1, 4, 70, 64)
     k, v = (t.contiguous() for t in _data(1, 4, 4, 64, 70, 200, BF16)[1:])
     _check(window.window_attention(one, k, v, window=50), one, k, v, None, window=50)
+
+
+@pytest.mark.parametrize("lq", [8, 30, 140, 300])
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_first_token_that_the_first_queries_do_not_see(cuda, lq, d):
+    """Sinks ahead of the first queries of a prompt: hidden from these alone."""
+    q, k, v = _data(1, 2, 1, d, lq, lq, BF16, seed=lq)
+    v[0, 0, 5, 1], v[0, 0, 6, 2] = float("inf"), float("nan")
+    for win in (2, 4, None):
+        got = window.window_attention(q, k, v, window=win, sinks=20)
+        _check(got, q, k, v, None, window=win, sinks=20)
+        kp, vp, table = _pages(k, v, 16)
+        n = torch.tensor([lq], dtype=torch.int32, device="cuda")
+        _check(window.paged_window_attention(q, kp, vp, table, n, window=win, sinks=20), q, k, v, None, window=win, sinks=20)
+    _quiet()
