@@ -40,7 +40,8 @@ def _rule(window, sinks, frame_tokens):
     window = _FOREVER if window is None else int(window)
     if window < 1 or sinks < 0 or frame_tokens < 1:
         raise ValueError("window must be at least 1 (or None), sinks at least 0, frame_tokens at least 1")
-    return min(window, _FOREVER), min(int(sinks), _FOREVER), int(frame_tokens)
+    # (no session has 2^30 keys: a longer frame is one that holds them all)
+    return min(window, _FOREVER), min(int(sinks), _FOREVER), min(int(frame_tokens), 1 << 30)
 
 
 def _workspace_bytes(name: str, device: torch.device, *shape) -> int:

@@ -292,3 +292,19 @@ def test_unknown_positions_under_the_norm(cuda):
             assert (y[0, :, 1:3] == 0).all() and (y[0, :, 0] != 0).any() and (y[0, :, 3] != 0).any()
         with pytest.raises(CastError):
             _quiet()
+
+
+def test_single_precision_into_half_precision_pages(cuda):
+    table = rotary.rope_table(rotary.rope_frequencies(64), 16)
+    q, k, v = (_x(2, 5, h, 64, dtype=torch.float32, seed=h) for h in (4, 2, 2))
+    v = v * 1.001
+    w = torch.ones(64, device="cuda")
+    kp = torch.zeros(3, 2, 8, 64, dtype=torch.bfloat16, device="cuda")
+    vp = torch.zeros_like(kp)
+    slots = torch.arange(10, device="cuda").view(2, 5) + 7
+    rotary.qk_norm_rope(q, k, w, w, table, v=v, cache=(kp, vp), slots=slots, out_dtype=torch.bfloat16)
+    want = rotary.qk_norm_rope(q, k, w, w, table, out_dtype=torch.bfloat16)[1]
+    s = slots.view(-1)
+    assert torch.equal(kp[s // 8, :, s % 8], want.transpose(1, 2).reshape(10, 2, 64))
+    assert torch.equal(vp[s // 8, :, s % 8], v.bfloat16().reshape(10, 2, 64))
+    _quiet()

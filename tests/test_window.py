@@ -56,6 +56,11 @@ def test_rule_refused(kw):
         window._rule(kw["window"], kw.get("sinks", 0), kw.get("frame_tokens", 1))
 
 
+def test_rule_takes_any_size():
+    assert window._rule(None, 0, 1)[0] >= 1 << 31
+    assert window._rule(1 << 70, 1 << 70, 1 << 70) == (1 << 40, 1 << 40, 1 << 30)
+
+
 def _call(lib, **kw):
     a = dict(q=4096, k=4096, v=4096, dtype=0, lens=None, B=1, Hq=4, Hk=2, Lq=8, Lk=16, D=128,
              strides=[4096, 1024, 128] * 4, window=8, sinks=0, frame=1, scale=0.1, out=4096)

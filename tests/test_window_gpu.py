@@ -409,3 +409,13 @@ def test_a_first_token_that_the_first_queries_do_not_see(cuda, lq, d):
         n = torch.tensor([lq], dtype=torch.int32, device="cuda")
         _check(window.paged_window_attention(q, kp, vp, table, n, window=win, sinks=20), q, k, v, None, window=win, sinks=20)
     _quiet()
+
+
+@pytest.mark.parametrize("lq", [1, 50])
+def test_sizes_that_mean_everything(cuda, lq):
+    q, k, v = _data(1, 2, 1, 64, lq, 90, BF16)
+    seen = window.window_attention(q, k, v, window=1, frame_tokens=1 << 45)  # one frame: all see all
+    assert torch.equal(seen, window.window_attention(q, k, v, window=1, frame_tokens=90))
+    _check(seen, q, k, v, None, window=1, frame=90)
+    assert torch.equal(window.window_attention(q, k, v, window=1 << 60, sinks=1 << 60),
+                       window.window_attention(q, k, v, window=None))
