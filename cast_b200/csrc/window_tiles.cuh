@@ -754,36 +754,46 @@ __global__ void __launch_bounds__(128 * kJoinGroups) window_tiles_join_kernel(co
   const float *base = p.part + (long long)item * p.parts * kPart;
   const float *tails = base + 128 * D + row_in;
   const int parts = on ? p.parts : 0;
-  float m = -INFINITY;
-#pragma unroll 8
-  for (int j = g; j < parts; j += kJoinGroups) m = fmaxf(m, __ldg(tails + j * kPart));
-  max_s[g][row_in] = m;
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < kJoinGroups; ++j) m = fmaxf(m, max_s[j][row_in]);
-  float l = 0.0f, a[kJoinCols];
+  float m = -INFINITY, l = 0.0f, a[kJoinCols];
 #pragma unroll
   for (int c = 0; c < kJoinCols; ++c) a[c] = 0.0f;
   bool bad = false;
-#pragma unroll 3
-  for (int j = g; j < parts; j += kJoinGroups) {
-    const float *tail = tails + j * kPart;
-    const float *o = base + j * kPart + cut * kJoinCols * 128 + row_in;
-    const float mj = __ldg(tail), lj = __ldg(tail + 128), flag = __ldg(tail + 256);
-    float v[kJoinCols];
+  constexpr int kAtOnce = 3;  // parts whose loads are under way together
+  for (int j0 = g; j0 < parts; j0 += kAtOnce * kJoinGroups) {
+    float mj[kAtOnce], lj[kAtOnce], flag[kAtOnce], v[kAtOnce][kJoinCols];
+    float top = m;
 #pragma unroll
-    for (int c = 0; c < kJoinCols; ++c) v[c] = __ldg(o + c * 128);
-    bad = bad || __float_as_int(flag) != 0;
-    if (mj != -INFINITY) {  // (where nothing was seen, O may hold anything)
-      const float f = fast_exp2(mj - m);
-      l = fmaf(lj, f, l);
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int j = min(j0 + u * kJoinGroups, parts - 1);
+      const float *tail = tails + j * kPart, *o = base + j * kPart + cut * kJoinCols * 128 + row_in;
+      mj[u] = j0 + u * kJoinGroups < parts ? __ldg(tail) : -INFINITY;
+      lj[u] = __ldg(tail + 128), flag[u] = __ldg(tail + 256);
 #pragma unroll
-      for (int c = 0; c < kJoinCols; ++c) a[c] = fmaf(v[c], f, a[c]);
+      for (int c = 0; c < kJoinCols; ++c) v[u][c] = __ldg(o + c * 128);
+    }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      top = fmaxf(top, mj[u]);
+      bad = bad || __float_as_int(flag[u]) != 0;
+    }
+    const float f0 = m == -INFINITY ? 0.0f : fast_exp2(m - top);
+    m = top;
+    l *= f0;
+#pragma unroll
+    for (int c = 0; c < kJoinCols; ++c) a[c] *= f0;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      if (mj[u] == -INFINITY) continue;  // nothing was seen: O may hold anything
+      const float f = fast_exp2(mj[u] - m);
+      l = fmaf(lj[u], f, l);
+#pragma unroll
+      for (int c = 0; c < kJoinCols; ++c) a[c] = fmaf(v[u][c], f, a[c]);
     }
   }
 #pragma unroll
   for (int c = 0; c < kJoinCols; ++c) acc_s[g][c][row_in] = a[c];
   acc_s[g][kJoinCols][row_in] = l;
+  max_s[g][row_in] = m;
   const bool any_bad = __syncthreads_or(bad);
   if (g != 0 || !on) return;
   float y[kJoinCols];
@@ -791,10 +801,13 @@ __global__ void __launch_bounds__(128 * kJoinGroups) window_tiles_join_kernel(co
 #pragma unroll
   for (int c = 0; c < kJoinCols; ++c) y[c] = 0.0f;
 #pragma unroll
-  for (int j = 0; j < kJoinGroups; ++j) {
-    l += acc_s[j][kJoinCols][row_in];
+  for (int j = 0; j < kJoinGroups; ++j) m = fmaxf(m, max_s[j][row_in]);
 #pragma unroll
-    for (int c = 0; c < kJoinCols; ++c) y[c] += acc_s[j][c][row_in];
+  for (int j = 0; j < kJoinGroups; ++j) {
+    const float mj = max_s[j][row_in], f = mj == -INFINITY ? 0.0f : fast_exp2(mj - m);
+    l = fmaf(acc_s[j][kJoinCols][row_in], f, l);
+#pragma unroll
+    for (int c = 0; c < kJoinCols; ++c) y[c] = fmaf(acc_s[j][c][row_in], f, y[c]);
   }
   const float inv = l != 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
