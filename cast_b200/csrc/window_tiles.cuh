@@ -581,6 +581,8 @@ __global__ void __launch_bounds__(kTilesThreads, TilesSmem<D>::ctas)
               for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
               tmem_put(o_addr + 32 * cc, o);
             }
+            // (the second chunk of a step may raise the maximum again and read O)
+            castdev::tmem_wait_st();
           }
         }
         return f;

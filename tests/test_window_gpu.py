@@ -419,3 +419,24 @@ def test_sizes_that_mean_everything(cuda, lq):
     _check(seen, q, k, v, None, window=1, frame=90)
     assert torch.equal(window.window_attention(q, k, v, window=1 << 60, sinks=1 << 60),
                        window.window_attention(q, k, v, window=None))
+
+
+@pytest.mark.parametrize("dtype,rise,fall", [(BF16, 18, 10), (FP16, 10, 3)])
+@pytest.mark.parametrize("lq", [40, 128, 200])
+def test_a_maximum_that_rises_twice_within_a_step(cuda, dtype, rise, fall, lq):
+    """Scores `rise` powers of two above the last ones every 32 keys: a step of
+    64 keys scales O in both its halves.  Values fall by `fall` powers of two at
+    the same places: an O that missed one of the two scales in the last step
+    holds 2^(2 fall - rise) of the result too much, 2^2 and 2^-4 of it, where
+    the type's rounding is 2^-8 and 2^-11."""
+    d, lk = 64, 256
+    q, k, v = _data(1, 2, 1, d, lq, lk, dtype, seed=rise + lq)
+    chunk = torch.arange(lk, device="cuda") // 32
+    q.fill_(1.0)
+    k.copy_(chunk.to(dtype)[:, None].expand(lk, d))
+    v.mul_((2.0 ** (fall * (3.0 - chunk))).to(dtype)[:, None])
+    scale = rise * 0.6931471805599453 / d  # q.k scale: rise ln 2 a chunk
+    for win, sinks in ((None, 0), (150, 40)):
+        got = window.window_attention(q, k, v, window=win, sinks=sinks, sm_scale=scale)
+        _check(got, q, k, v, None, window=win, sinks=sinks, scale=scale)
+    _quiet()
