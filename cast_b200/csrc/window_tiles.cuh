@@ -785,7 +785,12 @@ __global__ void __launch_bounds__(128 * kJoinGroups) window_tiles_join_kernel(co
     for (int c = 0; c < kJoinCols; ++c) a[c] *= f0;
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) {
-      if (mj[u] == -INFINITY) continue;  // nothing was seen: O may hold anything
+      // Nothing was seen (O may hold anything), or nothing but NaN scores: these
+      // leave no maximum and a NaN sum, which makes the row NaN.
+      if (mj[u] == -INFINITY) {
+        if (isnan(lj[u])) l = lj[u];
+        continue;
+      }
       const float f = fast_exp2(mj[u] - m);
       l = fmaf(lj[u], f, l);
 #pragma unroll

@@ -440,3 +440,31 @@ def test_a_maximum_that_rises_twice_within_a_step(cuda, dtype, rise, fall, lq):
         got = window.window_attention(q, k, v, window=win, sinks=sinks, sm_scale=scale)
         _check(got, q, k, v, None, window=win, sinks=sinks, scale=scale)
     _quiet()
+
+
+@pytest.mark.parametrize("d,dtype,hq,hk,lq,lk,lens", [
+    (64, BF16, 4, 2, 90, 9000, None), (64, FP16, 3, 1, 150, 6000, [6000, 900]),
+    (128, BF16, 2, 1, 100, 9000, [9000, 40]), (128, BF16, 24, 24, 1700, 2600, None)])
+def test_scores_that_are_nan_in_items_cut_into_parts(cuda, d, dtype, hq, hk, lq, lk, lens):
+    """A NaN in a query, and keys that make all scores of a part NaN, reach every
+    row that sees them and no other, however its keys are cut."""
+    b = 1 if lens is None else len(lens)
+    q, k, v = _data(b, hq, hk, d, lq, lk, dtype, seed=lk + d)
+    n = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    some = sorted({0, hq // hk - 1, hq - 1})
+    with torch.cuda.device(q.device):
+        assert _lib.load().cast_window_attention_workspace_bytes(b, hq, hk, lq, lk, d, lk, 0, 1) > 0  # (cut)
+    q[0, :, 3, 5], q[0, hq - 1, lq - 1] = float("nan"), float("nan")
+    for win in (None, lk - lq // 2):
+        got = window.window_attention(q, k, v, window=win, kv_lens=n)
+        assert torch.isnan(got[0, :, 3]).all() and torch.isfinite(got[0, 0, 4:10]).all()
+        _check(got, q, k, v, lens, window=win, heads=some)
+    # the last keys: seen by the last rows alone; and with a window, a long run that the last rows do not see
+    q = _data(b, hq, hk, d, lq, lk, dtype, seed=lk + d)[0]
+    end = lk if lens is None else lens[0]
+    k[0, :, end - 7:end] = float("nan")
+    k[0, 0, 2:end - lq // 2 - 100] = float("nan")
+    for win in (None, 100 + lq // 4):
+        got = window.window_attention(q, k, v, window=win, kv_lens=n, sinks=1)
+        _check(got, q, k, v, lens, window=win, sinks=1, heads=some)
+    _quiet()
