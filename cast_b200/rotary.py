@@ -145,8 +145,10 @@ def rope_frequencies(rotary_dim: int, *, base: float = 10000.0, axes=None, scali
             def pair_of(turns):  # the (fractional) pair that turns so often over the learned length
                 return n * math.log(length / (turns * 2 * math.pi)) / math.log(base)
 
-            lo = min(max(math.floor(pair_of(fast)), 0), max(n - 1, 0))
-            hi = min(max(math.ceil(pair_of(slow)), 0), max(n - 1, 0))
+            # (places run to the head's 2 n values, past the last pair: there the ramp of a
+            # long learned length ends, and no pair is divided by the whole factor)
+            lo = max(math.floor(pair_of(fast)), 0)
+            hi = min(math.ceil(pair_of(slow)), max(2 * n - 1, 0))
             blend = ((i - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)  # 0: kept, 1: divided
             f = f * (1.0 - blend) + f / factor * blend
         out.append(f)

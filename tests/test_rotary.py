@@ -142,3 +142,34 @@ def _norm(lib, **kw):
 def test_qk_norm_rope_refused(lib, kw, status, text):
     assert _norm(lib, **kw) == status
     assert text in lib.cast_last_error_message()
+
+
+@pytest.mark.parametrize("r,base,factor,length,fast,slow", [
+    (128, 10000.0, 8.0, 131072, 32.0, 1.0),   # the slowest pair turns 2.4 times over the learned length
+    (64, 500.0, 4.0, 32768, 32.0, 1.0),       # 8 times or so
+    (128, 10000.0, 8.0, 4096, 32.0, 1.0),
+    (64, 10000.0, 16.0, 10 ** 7, 8.0, 2.0),   # every pair turns often: all are kept
+    (128, 1000000.0, 4.0, 32768, 32.0, 1.0)])
+def test_blended_frequencies_pair_by_pair(r, base, factor, length, fast, slow):
+    """Each pair by itself: kept above `fast` turns over the learned length,
+    divided below `slow`, and between them linear in the pair's index, from the
+    last whole index of the first kind to the first one of the second (the
+    head's last value at most)."""
+    got = rotary.rope_frequencies(r, base=base, scaling=("yarn", factor, length, fast, slow))
+    # base^(-2j/r) length / (2 pi) = turns
+    place = [r / 2 * math.log(length / (2 * math.pi * t), base) for t in (fast, slow)]
+    first, last = math.floor(place[0]), min(math.ceil(place[1]), r - 1)
+    assert first >= 0
+    for j in range(r // 2):
+        step = base ** (-2 * j / r)
+        turns = step * length / (2 * math.pi)
+        if turns >= fast:
+            want = step
+        elif turns <= slow:
+            want = step / factor
+        else:
+            share = min(max((j - first) / (last - first), 0.0), 1.0)
+            want = step * (1 - share) + step / factor * share
+        assert got[j].item() == pytest.approx(want, rel=1e-12), (j, turns)
+        if turns > slow and j < last:
+            assert got[j].item() > step / factor  # never divided by the whole factor
