@@ -128,9 +128,14 @@ def rope_frequencies(rotary_dim: int, *, base: float = 10000.0, axes=None, scali
     parts = [rotary_dim // 2] if axes is None else [int(n) for n in axes]
     if sum(parts) != rotary_dim // 2 or min(parts) < 0:
         raise ValueError(f"axes {axes} must add up to {rotary_dim // 2} pairs")
-    kind, factor = (None, 1.0) if scaling is None else (scaling[0], float(scaling[1]))
-    if kind not in (None, "linear", "ntk", "yarn") or not factor > 0.0:
+    kind, factor, rest = (None, 1.0, ()) if scaling is None else (scaling[0], float(scaling[1]), tuple(scaling[2:]))
+    if kind not in (None, "linear", "ntk", "yarn") or not factor > 0.0 \
+            or (kind == "yarn" and len(rest) in (0, 2)):
         raise ValueError(f"scaling {scaling!r}: ('linear' | 'ntk', factor) or ('yarn', factor, length[, fast, slow])")
+    if kind == "yarn":
+        length, fast, slow = map(float, (*rest, 32.0, 1.0) if len(rest) == 1 else rest[:3])
+        if not (0.0 < length < math.inf and 0.0 < slow <= fast < math.inf):
+            raise ValueError(f"scaling {scaling!r}: length and slow must be positive, fast not below slow")
     out = []
     for n in parts:
         i = torch.arange(n, dtype=torch.float64)
@@ -139,9 +144,6 @@ def rope_frequencies(rotary_dim: int, *, base: float = 10000.0, axes=None, scali
         if kind == "linear":
             f = f / factor
         elif kind == "yarn":
-            length = float(scaling[2])
-            fast, slow = (float(scaling[3]), float(scaling[4])) if len(scaling) > 3 else (32.0, 1.0)
-
             def pair_of(turns):  # the (fractional) pair that turns so often over the learned length
                 return n * math.log(length / (turns * 2 * math.pi)) / math.log(base)
 
@@ -150,6 +152,8 @@ def rope_frequencies(rotary_dim: int, *, base: float = 10000.0, axes=None, scali
             lo = max(math.floor(pair_of(fast)), 0)
             hi = min(math.ceil(pair_of(slow)), max(2 * n - 1, 0))
             blend = ((i - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)  # 0: kept, 1: divided
+            if pair_of(slow) <= 0:  # a length that no pair turns over so often
+                blend = torch.ones_like(i)
             f = f * (1.0 - blend) + f / factor * blend
         out.append(f)
     return torch.cat(out)

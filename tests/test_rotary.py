@@ -173,3 +173,18 @@ def test_blended_frequencies_pair_by_pair(r, base, factor, length, fast, slow):
         assert got[j].item() == pytest.approx(want, rel=1e-12), (j, turns)
         if turns > slow and j < last:
             assert got[j].item() > step / factor  # never divided by the whole factor
+
+
+@pytest.mark.parametrize("scaling", [("yarn", 4.0), ("yarn", 4.0, 4096, 32.0), ("yarn", 4.0, 0), ("yarn", 4.0, -5.0),
+                                     ("yarn", 4.0, 4096, 1.0, 32.0), ("yarn", 4.0, 4096, 32.0, 0.0),
+                                     ("yarn", 4.0, float("inf")), ("ntk", float("nan"))])
+def test_scalings_refused(scaling):
+    with pytest.raises(ValueError, match="scaling"):
+        rotary.rope_frequencies(64, scaling=scaling)
+
+
+def test_blended_frequencies_of_a_length_that_no_pair_turns_over():
+    f = rotary.rope_frequencies(64)
+    for length in (1, 6):  # the fastest pair turns once over 6.3 positions
+        assert torch.allclose(rotary.rope_frequencies(64, scaling=("yarn", 4.0, length)), f / 4, rtol=1e-14)
+    assert rotary.rope_frequencies(64, scaling=("yarn", 4.0, 7))[0] == f[0]
