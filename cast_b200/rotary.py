@@ -68,7 +68,8 @@ def _strides(t: torch.Tensor, order) -> list[int]:
 
 # Checked calls, by all that their checks look at (types, shapes, strides,
 # devices, options; no tensor, address or value): a call like an earlier one
-# is launched without checking it again.
+# is launched without checking it again.  Options enter as the numbers they
+# are at the call: a tensor would be found again after its value has changed.
 _PLANS_KEPT = 4096
 _fn: dict[str, object] = {}
 
@@ -243,8 +244,8 @@ def rope(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor | None = 
     allowed.  A position that is no row of the table gives zeros and sets the
     device error word (:func:`cast_b200._lib.check_device`).
     """
-    if axes is not None:
-        axes = tuple(axes)
+    axes = None if axes is None else tuple(map(int, axes))
+    interleaved, inverse, start = bool(interleaved), bool(inverse), int(start)
     try:
         key = (x.dtype, x.shape, x.stride(), x.device, table.dtype, table.shape, table.stride(), table.device,
                None if positions is None else (positions.dtype, positions.shape, positions.stride(), positions.device),
@@ -347,8 +348,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     written; one past the end is not written and sets the device error word.
     Slots must differ from one another.
     """
-    if axes is not None:
-        axes = tuple(axes)
+    axes = None if axes is None else tuple(map(int, axes))
+    interleaved, start = bool(interleaved), int(start)
     qo, ko = (None, None) if out is None else out
     kp, vp = (None, None) if cache is None else cache
     try:

@@ -36,12 +36,17 @@ _plans: dict = {}
 _paged_plans: dict = {}
 
 
+def _options(window, sinks, frame_tokens):
+    """The options as the numbers they are now (they may be given as tensors)."""
+    return None if window is None else int(window), int(sinks), int(frame_tokens)
+
+
 def _rule(window, sinks, frame_tokens):
-    window = _FOREVER if window is None else int(window)
+    window = _FOREVER if window is None else window
     if window < 1 or sinks < 0 or frame_tokens < 1:
         raise ValueError("window must be at least 1 (or None), sinks at least 0, frame_tokens at least 1")
     # (no session has 2^30 keys: a longer frame is one that holds them all)
-    return min(window, _FOREVER), min(int(sinks), _FOREVER), min(int(frame_tokens), 1 << 30)
+    return min(window, _FOREVER), min(sinks, _FOREVER), min(frame_tokens, 1 << 30)
 
 
 def _workspace_bytes(name: str, device: torch.device, *shape) -> int:
@@ -105,6 +110,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     that sees nothing gives zeros.  A length outside ``[0, Lk]`` is clipped
     and sets the device error word.
     """
+    window, sinks, frame_tokens = _options(window, sinks, frame_tokens)
     try:
         key = (q.dtype, q.shape, q.stride(), q.device, k.dtype, k.shape, k.stride(), k.device, v.dtype, v.shape,
                v.stride(), v.device,
@@ -175,6 +181,7 @@ def paged_window_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     device error word, as a length outside ``[0, max_pages * page]`` does.
     Sessions may share pages (a common prefix).
     """
+    window, sinks, frame_tokens = _options(window, sinks, frame_tokens)
     try:
         key = (q.dtype, q.shape, q.stride(), q.device, k_pages.dtype, k_pages.shape, k_pages.stride(), k_pages.device,
                v_pages.dtype, v_pages.shape, v_pages.stride(), v_pages.device, block_table.dtype, block_table.shape,

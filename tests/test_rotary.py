@@ -188,3 +188,32 @@ def test_blended_frequencies_of_a_length_that_no_pair_turns_over():
     for length in (1, 6):  # the fastest pair turns once over 6.3 positions
         assert torch.allclose(rotary.rope_frequencies(64, scaling=("yarn", 4.0, length)), f / 4, rtol=1e-14)
     assert rotary.rope_frequencies(64, scaling=("yarn", 4.0, 7))[0] == f[0]
+
+
+def test_options_are_read_at_every_call(monkeypatch):
+    """An option given as a tensor that changes in place between two calls."""
+    seen = []
+
+    def rope(x, table, positions, interleaved, axes, inverse, start, out):
+        seen.append((interleaved, axes, inverse, start))
+        return True, 0, 0, 0, ()
+
+    def norm(q, k, qw, kw, table, positions, interleaved, axes, start, out_dtype, *rest):
+        seen.append((interleaved, axes, start))
+        return True, 0, q.dtype, (1,), (1,), (), (), 0, (), ()
+
+    monkeypatch.setattr(rotary, "_rope_plan", rope)
+    monkeypatch.setattr(rotary, "_norm_plan", norm)
+    monkeypatch.setattr(rotary, "_rope_plans", {})
+    monkeypatch.setattr(rotary, "_norm_plans", {})
+    x, table = torch.zeros(1, 2, 2, 16), torch.zeros(9, 8, 2)
+    start, inter, inv, axes = torch.tensor(1), torch.tensor(True), torch.tensor(False), torch.tensor([4, 2, 2])
+    for change in (lambda: None, lambda: start.add_(1), lambda: inter.logical_not_(), lambda: inv.logical_not_(),
+                   lambda: axes.copy_(torch.tensor([2, 2, 4]))):
+        change()
+        rotary.rope(x, table, interleaved=inter, inverse=inv, axes=axes, start=start)
+        rotary.qk_norm_rope(x, x, None, None, table, interleaved=inter, axes=axes, start=start)
+    a, b = (4, 2, 2), (2, 2, 4)
+    assert [s for s in seen if len(s) == 4] == [(True, a, False, 1), (True, a, False, 2), (False, a, False, 2),
+                                                (False, a, True, 2), (False, b, True, 2)]
+    assert [s for s in seen if len(s) == 3] == [(True, a, 1), (True, a, 2), (False, a, 2), (False, b, 2)]

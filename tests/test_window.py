@@ -118,3 +118,32 @@ def test_python_refuses_what_is_no_tensor():
         window.window_attention([1], None, None, window=4)
     with pytest.raises(ValueError, match="CUDA"):
         window.paged_window_attention(None, None, None, None, None, window=4)
+
+
+def test_options_are_read_at_every_call(monkeypatch):
+    """An option given as a tensor that changes in place between two calls."""
+    seen = []
+
+    def plan(q, k, v, win, sinks, frame, *rest):
+        seen.append((win, sinks, frame))
+        return True, False, 0, 0, 0.0, (), ()
+
+    def paged(q, k, v, table, lens, win, sinks, frame, *rest):
+        seen.append((win, sinks, frame))
+        return True, False, 0, 0, 0.0, (), (), ()
+
+    monkeypatch.setattr(window, "_window_plan", plan)
+    monkeypatch.setattr(window, "_paged_plan", paged)
+    monkeypatch.setattr(window, "_plans", {})
+    monkeypatch.setattr(window, "_paged_plans", {})
+    x, n = torch.zeros(1, 2, 4, 64), torch.zeros(1, dtype=torch.int32)
+    for call in (lambda *a: window.window_attention(x, x, x, window=a[0], sinks=a[1], frame_tokens=a[2]),
+                 lambda *a: window.paged_window_attention(x, x, x, n[None], n, window=a[0], sinks=a[1], frame_tokens=a[2])):
+        opts = [torch.tensor(9), torch.tensor(2), torch.tensor(3)]
+        seen.clear()
+        call(*opts)
+        for o in opts:
+            o.add_(1)
+            call(*opts)
+        assert seen == [(9, 2, 3), (10, 2, 3), (10, 3, 3), (10, 3, 4)]
+        assert all(type(v) is int for s in seen for v in s)
