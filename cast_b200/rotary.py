@@ -25,6 +25,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -85,8 +86,17 @@ def _keep(plans: dict, key, plan):
     return plan
 
 
-def _no_gradient():
-    raise ValueError("an input needs a gradient, which this operator has not (use torch.no_grad())")
+def _refuse_gradients(*tensors) -> None:
+    """No input may need a gradient, of reverse or of forward mode (a tangent
+    passes ``torch.no_grad``), and none may be asked of an output given."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("an input or out needs a gradient, which this operator has not (use torch.no_grad())")
+    if forward_ad._current_level >= 0:  # (tensors have tangents within a dual level alone)
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError("an input or out has a tangent (forward-mode gradient), which this operator has not")
 
 
 def _launch(index: int, name: str, *args) -> None:
@@ -256,8 +266,7 @@ def rope(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor | None = 
     if plan is None:
         plan = _keep(_rope_plans, key, _rope_plan(x, table, positions, interleaved, axes, inverse, start, out))
     empty, index, dtype, rows, rest = plan
-    if torch.is_grad_enabled() and (x.requires_grad or table.requires_grad):
-        _no_gradient()
+    _refuse_gradients(x, table, out)
     if out is None:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
     if not empty:
@@ -370,11 +379,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
         plan = _keep(_norm_plans, key, _norm_plan(q, k, q_weight, k_weight, table, positions, interleaved, axes, start,
                                                   out_dtype, qo, ko, v, cache, slots))
     empty, index, out_dtype, q_shape, k_shape, types, weights, rows, rest, places = plan
-    if torch.is_grad_enabled() and (
-            q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)
-            or (k_weight is not None and k_weight.requires_grad) or (table is not None and table.requires_grad)
-            or (cache is not None and (v.requires_grad or kp.requires_grad or vp.requires_grad))):
-        _no_gradient()
+    _refuse_gradients(q, k, q_weight, k_weight, table, v, kp, vp, qo, ko)
     if qo is None:
         qo = q.new_empty(q_shape) if out_dtype is q.dtype else q.new_empty(q_shape, dtype=out_dtype)
     if cache is None and ko is None:

@@ -27,7 +27,7 @@ import math
 import torch
 
 from . import _lib
-from .rotary import DTYPES, _check, _check_out, _keep, _launch, _no_gradient, _sig, _strides
+from .rotary import DTYPES, _check, _check_out, _keep, _launch, _refuse_gradients, _sig, _strides
 
 _TYPES = (torch.bfloat16, torch.float16)
 _Twelve = ctypes.c_longlong * 12
@@ -123,8 +123,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     if plan is None:
         plan = _keep(_plans, key, _window_plan(q, k, v, window, sinks, frame_tokens, kv_lens, out))
     empty, blind, index, nbytes, scale, dtype, rest = plan
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        _no_gradient()
+    _refuse_gradients(q, k, v, out)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if empty:
@@ -195,8 +194,7 @@ def paged_window_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
         plan = _keep(_paged_plans, key, _paged_plan(q, k_pages, v_pages, block_table, kv_lens, window, sinks,
                                                     frame_tokens, out))
     empty, blind, index, nbytes, scale, dtype, pages, rest = plan
-    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
-        _no_gradient()
+    _refuse_gradients(q, k_pages, v_pages, out)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if empty:

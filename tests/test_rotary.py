@@ -5,6 +5,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from cast_b200 import _lib, rotary
 from oracle import rotary as ora
@@ -217,3 +218,16 @@ def test_options_are_read_at_every_call(monkeypatch):
     assert [s for s in seen if len(s) == 4] == [(True, a, False, 1), (True, a, False, 2), (False, a, False, 2),
                                                 (False, a, True, 2), (False, b, True, 2)]
     assert [s for s in seen if len(s) == 3] == [(True, a, 1), (True, a, 2), (False, a, 2), (False, b, 2)]
+
+
+def test_gradients_of_both_modes_refused():
+    x, y = torch.zeros(3), torch.zeros(3, requires_grad=True)
+    rotary._refuse_gradients(x, None)
+    with pytest.raises(ValueError, match="gradient"):
+        rotary._refuse_gradients(x, None, y)
+    with torch.no_grad():
+        rotary._refuse_gradients(x, None, y)
+        with forward_ad.dual_level():
+            rotary._refuse_gradients(x, None)
+            with pytest.raises(ValueError, match="tangent"):  # no_grad does not end forward mode
+                rotary._refuse_gradients(None, forward_ad.make_dual(x, torch.ones(3)))

@@ -308,3 +308,39 @@ def test_single_precision_into_half_precision_pages(cuda):
     assert torch.equal(kp[s // 8, :, s % 8], want.transpose(1, 2).reshape(10, 2, 64))
     assert torch.equal(vp[s // 8, :, s % 8], v.bfloat16().reshape(10, 2, 64))
     _quiet()
+
+
+def test_inputs_with_tangents_and_outs_with_gradients_refused(cuda):
+    from torch.autograd import forward_ad
+
+    from cast_b200 import window
+
+    table = rotary.rope_table(rotary.rope_frequencies(64), 10)
+    x = _x(1, 4, 3, 64, dtype=torch.bfloat16)
+    w = torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    n = torch.tensor([3], dtype=torch.int32, device="cuda")
+    pages = torch.zeros(1, dtype=torch.int32, device="cuda")[None]
+
+    def calls(y, out=None):
+        yield lambda: rotary.rope(y, table, out=out)
+        yield lambda: rotary.qk_norm_rope(x, y, w, w, table, out=None if out is None else (None, out.transpose(1, 2)))
+        yield lambda: window.window_attention(x, x, y, window=2, out=out)
+        yield lambda: window.paged_window_attention(x, x, y, pages, n, window=2, out=out)
+
+    for call in calls(x):
+        call()  # as it is (and kept as checked)
+    with forward_ad.dual_level(), torch.no_grad():
+        for call in calls(forward_ad.make_dual(x, torch.ones_like(x))):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+        for call in calls(x):
+            call()
+    for call in calls(x, out=torch.zeros_like(x, requires_grad=True)):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+    with torch.no_grad():
+        for call in calls(x, out=torch.zeros_like(x, requires_grad=True)):
+            call()
+    with pytest.raises(ValueError, match="gradient"):
+        rotary.qk_norm_rope(x, x, w.clone().requires_grad_(), w, table)
+    _quiet()
