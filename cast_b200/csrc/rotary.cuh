@@ -146,10 +146,8 @@ struct RotaryLane {
   static constexpr int kPairs = kHalf ? 8 : 4 * kC;  // table entries of a lane's columns
   float cs[kPairs], sn[kPairs];
   bool live, turns[kC];
-  bool blank;  // this token's position is unknown: its q and k are zeros
   int c, h0, step, partner, second;  // second: columns from the first piece to the second
 
-  template <bool kBlank>
   __device__ __forceinline__ void load(const RotaryParams &p, const RotaryTensor &t, const InT *row, int hb,
                                        Eight<InT> (&raw)[kBatch][kC]) const {
     const InT *src = row + (long long)(hb + h0) * t.ss[2];
@@ -161,13 +159,14 @@ struct RotaryLane {
       }
       src += step * t.ss[2];
     }
-    if (kBlank && blank) clear(raw);
   }
-  __device__ __forceinline__ void clear(Eight<InT> (&raw)[kBatch][kC]) const {
+  // Zeros in place of a tensor's heads.
+  __device__ __forceinline__ void zeros(const RotaryTensor &t, OutT *at, long long at_step) const {
+    const float x[8] = {};
+#pragma unroll 1
+    for (int h = h0; live && h < t.heads; h += step)
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u)
-#pragma unroll
-      for (int j = 0; j < kC; ++j) raw[u][j] = Eight<InT>{};
+      for (int j = 0; j < kC; ++j) store8(at + h * at_step + j * second, x);
   }
 
   // One tensor's heads of one token, h0, h0 + step, ... below t.heads.  kTurn:
@@ -198,7 +197,7 @@ struct RotaryLane {
     const bool normed = kNorm && kTurn && t.weight != nullptr;
     if (normed && live && !p.weight_per_head) weight(0);
     for (int hb = 0; hb < t.heads; hb += step * kBatch) {  // same trip count in the whole CTA
-      if (hb > 0) load<kTurn>(p, t, row, hb, raw);
+      if (hb > 0) load(p, t, row, hb, raw);
       OutT *dst = at + (long long)(hb + h0) * at_step;
 #pragma unroll
       for (int u = 0; u < kBatch; ++u, dst += step * at_step) {
@@ -221,7 +220,7 @@ struct RotaryLane {
           float sum = lo + hi;
 #pragma unroll
           for (int s = kLanes / 2; s >= 1; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-          const float r = blank ? 0.0f : rsqrtf(fmaf(sum, p.inv_d, p.eps));
+          const float r = rsqrtf(fmaf(sum, p.inv_d, p.eps));
           const uint64_t r2 = f2_pack(r, r);
           if (p.weight_per_head && on) weight(h);
 #pragma unroll
@@ -307,8 +306,7 @@ __global__ void __launch_bounds__(kRotaryThreads, rotary_ctas(kC)) rotary_kernel
     }
 
     // on its way while the position and then its table row are fetched
-    f.blank = false;
-    f.template load<false>(p, p.t[0], src[0] + l * p.t[0].ss[1], 0, raw);
+    f.load(p, p.t[0], src[0] + l * p.t[0].ss[1], 0, raw);
 
     // ---- this lane's (cos, sin): none where its columns are not rotated
     if (p.R > 0) {
@@ -335,11 +333,12 @@ __global__ void __launch_bounds__(kRotaryThreads, rotary_ctas(kC)) rotary_kernel
         }
       }
       if (__any_sync(0xffffffffu, !known)) {
-        if (!known) {  // zeros, and said so
+        if (!known) {  // zeros, and said so; what this token's q and k come to is left unwritten
           pos[0] = pos[1] = pos[2] = 0;
           if (c == 0 && f.h0 == 0) atomicExch(err, (int)CAST_ERR_INVALID_ARGUMENT);
-          f.blank = true;
-          f.clear(raw);
+          f.zeros(p.t[0], dst[0] + l * p.t[0].ds[1], p.t[0].ds[2]);
+          if (!p.slots) f.zeros(p.t[1], dst[1] + l * p.t[1].ds[1], p.t[1].ds[2]);
+          f.live = false;
         }
       }
       if (any_turns) {
@@ -376,7 +375,7 @@ __global__ void __launch_bounds__(kRotaryThreads, rotary_ctas(kC)) rotary_kernel
     f.template run<true>(p, p.t[0], src[0] + l * p.t[0].ss[1], dst[0] + l * p.t[0].ds[1], p.t[0].ds[2], raw);
     if (p.t[1].heads == 0) continue;  // uniform
 
-    f.template load<true>(p, p.t[1], src[1] + l * p.t[1].ss[1], 0, raw);
+    f.load(p, p.t[1], src[1] + l * p.t[1].ss[1], 0, raw);
     if (!p.slots) {
       f.template run<true>(p, p.t[1], src[1] + l * p.t[1].ss[1], dst[1] + l * p.t[1].ds[1], p.t[1].ds[2], raw);
       continue;
@@ -393,8 +392,15 @@ __global__ void __launch_bounds__(kRotaryThreads, rotary_ctas(kC)) rotary_kernel
       }
     }
     const long long head = (long long)p.page * p.D;
+    const bool column = live_token && 8 * kC * c < p.D;
+    if (column && !f.live) {
+      f.live = true;
+      if (place >= 0) f.zeros(p.t[1], dst[1] + place, head);
+      f.live = false;
+    }
     f.template run<true>(p, p.t[1], src[1] + l * p.t[1].ss[1], place < 0 ? nullptr : dst[1] + place, head, raw);
-    f.template load<false>(p, p.t[2], src[2] + l * p.t[2].ss[1], 0, raw);
+    f.live = column;  // (the value is copied whatever the position)
+    f.load(p, p.t[2], src[2] + l * p.t[2].ss[1], 0, raw);
     f.template run<false>(p, p.t[2], src[2] + l * p.t[2].ss[1], place < 0 ? nullptr : dst[2] + place, head, raw);
   }
 }

@@ -344,3 +344,32 @@ def test_inputs_with_tangents_and_outs_with_gradients_refused(cuda):
     with pytest.raises(ValueError, match="gradient"):
         rotary.qk_norm_rope(x, x, w.clone().requires_grad_(), w, table)
     _quiet()
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("d,r,l,h", [(128, 128, 4, 5), (128, 64, 4, 3), (64, 64, 300, 7), (256, 256, 4, 2), (80, 48, 9, 3)])
+def test_unknown_positions_are_zeros_whatever_weights_and_table_hold(cuda, interleaved, d, r, l, h):
+    table = rotary.rope_table(rotary.rope_frequencies(r), 10)
+    table[0] = float("nan")
+    x = _x(2, l, h, d, dtype=torch.bfloat16)
+    pos = torch.randint(1, 10, (2, l), device="cuda")
+    pos[:, 1], pos[1, 2] = 10, -1
+    unknown = (pos < 0) | (pos > 9)
+    y = rotary.rope(x, table, pos, interleaved=interleaved)
+    assert (y[unknown] == 0).all() and torch.isfinite(y).all() and (y[~unknown] != 0).any()
+    x0 = x.clone()
+    assert torch.equal(rotary.rope(x0, table, pos, interleaved=interleaved, out=x0), y)
+    kp = torch.full((2 * l // 4 + 1, h, 4, d), 3.0, dtype=torch.bfloat16, device="cuda")
+    vp = kp.clone()
+    slots = torch.randperm(2 * l, device="cuda").view(2, l)
+    for w in (torch.full((d,), float("inf"), device="cuda"), torch.full((h, d), float("nan"), device="cuda").bfloat16()):
+        for got in rotary.qk_norm_rope(x, x, w, w, table, pos, interleaved=interleaved):
+            assert (got.transpose(1, 2)[unknown] == 0).all() and not torch.isfinite(got.transpose(1, 2)[~unknown]).any()
+        q, _ = rotary.qk_norm_rope(x, x, w, w, table, pos, interleaved=interleaved, v=x, cache=(kp, vp), slots=slots)
+        s = slots[unknown]
+        assert (q.transpose(1, 2)[unknown] == 0).all() and (kp[s // 4, :, s % 4] == 0).all()
+        s = slots.view(-1)
+        assert torch.equal(vp[s // 4, :, s % 4], x.view(2 * l, h, d))  # values are copied whatever the position
+    with pytest.raises(CastError):
+        _quiet()
+    _quiet()
