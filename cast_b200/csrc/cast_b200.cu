@@ -1242,20 +1242,24 @@ static void launch_rotary_lanes(const castk::RotaryParams &p, cudaStream_t s) {
 
 template <typename InT, typename OutT, bool kNorm, bool kHalf>
 static int launch_rotary(const castk::RotaryParams &p, cudaStream_t s) {
-  if (p.pieces == 2) {
-    if (p.lanes == 4)
-      launch_rotary_lanes<InT, OutT, kNorm, kHalf, 2, 4>(p, s);
-    else if (p.lanes == 8)
-      launch_rotary_lanes<InT, OutT, kNorm, kHalf, 2, 8>(p, s);
-    else
-      launch_rotary_lanes<InT, OutT, kNorm, kHalf, 2, 16>(p, s);
-  } else if (p.lanes == 8) {
-    launch_rotary_lanes<InT, OutT, kNorm, kHalf, 1, 8>(p, s);
-  } else if (p.lanes == 16) {
-    launch_rotary_lanes<InT, OutT, kNorm, kHalf, 1, 16>(p, s);
-  } else {
-    launch_rotary_lanes<InT, OutT, kNorm, kHalf, 1, 32>(p, s);
+  if constexpr (kNorm) {  // (two pieces come with the norm alone)
+    if (p.pieces == 2) {
+      if (p.lanes == 4)
+        launch_rotary_lanes<InT, OutT, kNorm, kHalf, 2, 4>(p, s);
+      else if (p.lanes == 8)
+        launch_rotary_lanes<InT, OutT, kNorm, kHalf, 2, 8>(p, s);
+      else
+        launch_rotary_lanes<InT, OutT, kNorm, kHalf, 2, 16>(p, s);
+      CAST_CUDA_TRY(cudaGetLastError());
+      return CAST_OK;
+    }
   }
+  if (p.lanes == 8)
+    launch_rotary_lanes<InT, OutT, kNorm, kHalf, 1, 8>(p, s);
+  else if (p.lanes == 16)
+    launch_rotary_lanes<InT, OutT, kNorm, kHalf, 1, 16>(p, s);
+  else
+    launch_rotary_lanes<InT, OutT, kNorm, kHalf, 1, 32>(p, s);
   CAST_CUDA_TRY(cudaGetLastError());
   return CAST_OK;
 }
