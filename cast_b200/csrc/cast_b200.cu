@@ -1160,7 +1160,7 @@ struct RotaryPositions {
 
 // Checks shared by both entry points and the parameters they share.
 static int rotary_params(castk::RotaryParams &p, const RotaryPositions &at, int B, int L, int heads,
-                         int D, int R, int flags, bool norm, bool even) {
+                         int D, int R, int flags) {
   if (B <= 0 || L <= 0 || heads <= 0) return fail(CAST_ERR_INVALID_ARGUMENT, "non-positive size");
   if (L > (1 << 30) || B > (1 << 30)) return fail(CAST_ERR_UNSUPPORTED, "%d x %d tokens in one call", B, L);
   if (D <= 0 || D % 8 || D > 256)
@@ -1202,6 +1202,12 @@ static int rotary_params(castk::RotaryParams &p, const RotaryPositions &at, int 
   p.R = R;
   p.inv_d = 1.0f / (float)D;
   p.inverse = (flags >> 1) & 1;
+  return CAST_OK;
+}
+
+// How lanes are laid over the heads of a checked call.
+static void rotary_layout(castk::RotaryParams &p, int heads, bool norm, bool half, bool even, int n_sms) {
+  const int B = p.B, L = p.L, D = p.D, R = p.R;
   // A lane of one piece of eight columns or of two, and how many heads of a
   // token it takes.  With the norm, two pieces halve what a head costs beside
   // its values (reduction, root, addresses), and a lane takes eight heads or
@@ -1222,15 +1228,14 @@ static int rotary_params(castk::RotaryParams &p, const RotaryPositions &at, int 
   while (p.slots_per_token < groups && p.slots_per_token < heads) p.slots_per_token *= 2, ++p.slots_log2;
   auto ctas = [&](int slots, int run) { return (long long)B * ceil_div(L, groups / slots * run); };
   while (!(norm && even) && p.slots_per_token > 1 && heads / p.slots_per_token < 8 &&
-         ctas(p.slots_per_token / 2, 1) >= 148 * 7)
+         ctas(p.slots_per_token / 2, 1) >= n_sms * 7)
     p.slots_per_token /= 2, --p.slots_log2;
   // A CTA takes the tokens its lanes have room for, and up to kRotaryRun times
   // as many one after the other while the grid still fills the device.
   const int at_once = groups >> p.slots_log2;
   int run = 1;
-  while (run < castk::kRotaryRun && ctas(p.slots_per_token, 2 * run) >= 148 * 16) run *= 2;
+  while (run < castk::kRotaryRun && ctas(p.slots_per_token, 2 * run) >= n_sms * 16) run *= 2;
   p.tokens_per_cta = at_once * run;
-  return CAST_OK;
 }
 
 template <typename InT, typename OutT, bool kNorm, bool kHalf, int kC, int kLanes>
@@ -1298,11 +1303,13 @@ extern "C" int cast_rope(const void *x, int dtype, const float *table, int table
   if (!dtype_ok(dtype)) return fail(CAST_ERR_INVALID_ARGUMENT, "dtype %d (0 = bf16, 1 = fp32, 2 = fp16)", dtype);
   castk::RotaryParams p;
   int st = rotary_params(p, {table, table_rows, positions, positions_64, pos_batch_stride, first_position, axes},
-                         B, L, H, D, R, flags, false, false);
+                         B, L, H, D, R, flags);
   if (st) return st;
   if (!aligned16(x) || !aligned16(out) || !strides_ok(strides, 6, dtype))
     return fail(CAST_ERR_ALIGNMENT, "x and out must start, and their strides step, on 16-byte boundaries");
-  if ((st = current_device_sm100(nullptr))) return st;
+  int n_sms = 0;
+  if ((st = current_device_sm100(&n_sms))) return st;
+  rotary_layout(p, H, false, !(flags & 1), false, n_sms);
   rotary_tensor(p.t[0], x, out, nullptr, H, strides, strides + 3);
   return launch_rotary(p, dtype, dtype, false, !(flags & 1), reinterpret_cast<cudaStream_t>(stream));
 }
@@ -1327,18 +1334,20 @@ extern "C" int cast_qk_norm_rope(const void *q, const void *k, const void *v, in
     return fail(CAST_ERR_INVALID_ARGUMENT, "%d query and %d key heads", Hq, Hk);
   if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(CAST_ERR_INVALID_ARGUMENT, "eps must be finite, 0 or more");
   if (slots && (n_pages <= 0 || page <= 0)) return fail(CAST_ERR_INVALID_ARGUMENT, "non-positive cache size");
-  // three heads of one piece a lane, in one batch (see rotary_params)
-  const int wide = 3 * castk::kRotaryThreads / (D <= 64 ? 8 : (D <= 128 ? 16 : 32));
-  const bool filled = Hq == wide && Hk == wide && !v && (flags & 1);
   castk::RotaryParams p;
   int st = rotary_params(p, {table, table_rows, positions, positions_64, pos_batch_stride, first_position, axes},
-                         B, L, Hq + (v ? 2 : 1) * Hk, D, R, flags, q_weight || k_weight, filled);
+                         B, L, Hq + (v ? 2 : 1) * Hk, D, R, flags);
   if (st) return st;
   if (!aligned16(q) || !aligned16(k) || (v && !aligned16(v)) || !aligned16(q_out) || !aligned16(k_out) ||
       (v_out && !aligned16(v_out)) || (q_weight && !aligned16(q_weight)) || (k_weight && !aligned16(k_weight)) ||
       !strides_ok(strides, v ? 9 : 6, dtype) || !strides_ok(strides + 9, 6, out_dtype))
     return fail(CAST_ERR_ALIGNMENT, "tensors must start, and their strides step, on 16-byte boundaries");
-  if ((st = current_device_sm100(nullptr))) return st;
+  int n_sms = 0;
+  if ((st = current_device_sm100(&n_sms))) return st;
+  // three heads of one piece a lane, in one batch (see rotary_layout)
+  const int wide = 3 * castk::kRotaryThreads / (D <= 64 ? 8 : (D <= 128 ? 16 : 32));
+  const bool filled = Hq == wide && Hk == wide && !v && (flags & 1);
+  rotary_layout(p, Hq + (v ? 2 : 1) * Hk, q_weight || k_weight, !(flags & 1), filled, n_sms);
   rotary_tensor(p.t[0], q, q_out, q_weight, Hq, strides, strides + 9);
   rotary_tensor(p.t[1], k, k_out, k_weight, Hk, strides + 3, slots ? nullptr : strides + 12);
   if (v) rotary_tensor(p.t[2], v, v_out, nullptr, Hk, strides + 6, nullptr);
