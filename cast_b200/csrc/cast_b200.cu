@@ -1205,21 +1205,30 @@ static int rotary_params(castk::RotaryParams &p, const RotaryPositions &at, int 
   return CAST_OK;
 }
 
-// How lanes are laid over the heads of a checked call.
-static void rotary_layout(castk::RotaryParams &p, int heads, bool norm, bool half, bool even, int n_sms) {
-  const int B = p.B, L = p.L, D = p.D, R = p.R;
-  // A lane of one piece of eight columns or of two, and how many heads of a
-  // token it takes.  With the norm, two pieces halve what a head costs beside
-  // its values (reduction, root, addresses), and a lane takes eight heads or
-  // more, so that position and table row are paid once for them: 16 + 16 heads
-  // of 128 in 53.1 us (12500 tokens) against 59.4 with one piece, 32 + 8 with
-  // pages in 69.6 against 91.6.  Where one batch of three one-piece heads a
-  // lane is all of q, and all of k, and pairs lie side by side, one piece over
-  // as many lanes as there are is better: 24 + 24 heads of 128 in 48.7 us against
-  // 56.2, float32 76.8 against 99.3, 12 + 12 of 256 94.3 against 99.3 (half
-  // layout: 63.4 against 55.5, two batches: level).  Without the norm one piece
-  // is (66 against 74 us for 31680 tokens of 24 heads), and it has to be where
-  // the half layout's pairs are not half a head apart.
+// How lanes are laid over the heads of a checked call (Hq of q, Hk of k and, with
+// `copies`, of v).
+static void rotary_layout(castk::RotaryParams &p, int Hq, int Hk, bool copies, bool norm, bool half, bool fp32,
+                          int n_sms) {
+  const int B = p.B, L = p.L, D = p.D, R = p.R, heads = Hq + (copies ? 2 : 1) * Hk;
+  // A lane has one piece of eight columns of a head or two, and takes some of
+  // the heads of its token, three of one piece at a time.  Without the norm it
+  // has one piece (31680 tokens of 24 heads of 128: 66 us against 74), as it must
+  // where the half layout's pairs are not half a head apart.  With the norm,
+  // two pieces halve what a head costs beside its values (reduction, root,
+  // addresses), and a lane takes eight heads or more where the tokens fill the
+  // device so, which pays for position and table row once: 12500 tokens of
+  // 16 + 16 heads of 128 take 51 us against 68 in one piece.  But where three
+  // heads a lane are just all of q, and of k (more than two thirds of such a
+  // batch in use), and tokens are few, one piece over as many lanes as there
+  // are is better, side by side: 3520 tokens of 18 + 18 heads 22.0 us against
+  // 24.5, 22 + 22 23.1 against 26.3, 24 + 24 24.1 against 27.0, but 16 + 16 21.4
+  // against 17.9 and 25 + 25 33.8 against 27.6; 6000 tokens of 22 + 22 heads 37.6
+  // against 38.5, 8000 48.3 against 45.3.  float32, whose two pieces do not fit
+  // the registers, has it at any number of tokens (12500 of 18 + 18 heads 95 us
+  // against 121, 24 + 24 115 against 139).
+  const int batch = 3 * castk::kRotaryThreads / (D <= 64 ? 8 : (D <= 128 ? 16 : 32));
+  const bool even = norm && !half && !copies && std::max(Hq, Hk) <= batch && 3 * std::min(Hq, Hk) > 2 * batch &&
+                    (fp32 || (long long)B * L < 40ll * n_sms);
   p.pieces = norm && D % 16 == 0 && (!half || R == D || R == 0) && !even ? 2 : 1;
   p.lanes = p.pieces == 2 ? 4 : 8;
   while (p.lanes * p.pieces * 8 < D) p.lanes *= 2;
@@ -1227,7 +1236,7 @@ static void rotary_layout(castk::RotaryParams &p, int heads, bool norm, bool hal
   p.slots_per_token = 1, p.slots_log2 = 0;
   while (p.slots_per_token < groups && p.slots_per_token < heads) p.slots_per_token *= 2, ++p.slots_log2;
   auto ctas = [&](int slots, int run) { return (long long)B * ceil_div(L, groups / slots * run); };
-  while (!(norm && even) && p.slots_per_token > 1 && heads / p.slots_per_token < 8 &&
+  while (!even && p.slots_per_token > 1 && heads / p.slots_per_token < 8 &&
          ctas(p.slots_per_token / 2, 1) >= n_sms * 7)
     p.slots_per_token /= 2, --p.slots_log2;
   // A CTA takes the tokens its lanes have room for, and up to kRotaryRun times
@@ -1309,7 +1318,7 @@ extern "C" int cast_rope(const void *x, int dtype, const float *table, int table
     return fail(CAST_ERR_ALIGNMENT, "x and out must start, and their strides step, on 16-byte boundaries");
   int n_sms = 0;
   if ((st = current_device_sm100(&n_sms))) return st;
-  rotary_layout(p, H, false, !(flags & 1), false, n_sms);
+  rotary_layout(p, H, 0, false, false, !(flags & 1), dtype == kFp32, n_sms);
   rotary_tensor(p.t[0], x, out, nullptr, H, strides, strides + 3);
   return launch_rotary(p, dtype, dtype, false, !(flags & 1), reinterpret_cast<cudaStream_t>(stream));
 }
@@ -1344,10 +1353,7 @@ extern "C" int cast_qk_norm_rope(const void *q, const void *k, const void *v, in
     return fail(CAST_ERR_ALIGNMENT, "tensors must start, and their strides step, on 16-byte boundaries");
   int n_sms = 0;
   if ((st = current_device_sm100(&n_sms))) return st;
-  // three heads of one piece a lane, in one batch (see rotary_layout)
-  const int wide = 3 * castk::kRotaryThreads / (D <= 64 ? 8 : (D <= 128 ? 16 : 32));
-  const bool filled = Hq == wide && Hk == wide && !v && (flags & 1);
-  rotary_layout(p, Hq + (v ? 2 : 1) * Hk, q_weight || k_weight, !(flags & 1), filled, n_sms);
+  rotary_layout(p, Hq, Hk, v != nullptr, q_weight || k_weight, !(flags & 1), dtype == kFp32, n_sms);
   rotary_tensor(p.t[0], q, q_out, q_weight, Hq, strides, strides + 9);
   rotary_tensor(p.t[1], k, k_out, k_weight, Hk, strides + 3, slots ? nullptr : strides + 12);
   if (v) rotary_tensor(p.t[2], v, v_out, nullptr, Hk, strides + 6, nullptr);

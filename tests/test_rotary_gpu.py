@@ -373,3 +373,20 @@ def test_unknown_positions_are_zeros_whatever_weights_and_table_hold(cuda, inter
     with pytest.raises(CastError):
         _quiet()
     _quiet()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("b,l,hq,hk,d", [(1, 9, 17, 24, 128), (1, 9, 16, 24, 128), (2, 130, 18, 18, 128), (1, 77, 25, 23, 128),
+                                         (1, 3001, 22, 20, 128), (1, 5921, 18, 17, 128), (3, 21, 10, 12, 256),
+                                         (1, 40, 33, 48, 64), (1, 40, 23, 23, 72), (5, 1200, 17, 17, 128)])
+def test_head_counts_around_a_batch_of_three_a_lane(cuda, dtype, b, l, hq, hk, d):
+    f = rotary.rope_frequencies(d)
+    table = rotary.rope_table(f, l)
+    x = _x(b, l, hq + hk, d, dtype=dtype)
+    q, k = x[:, :, :hq], x[:, :, hq:]
+    qw, kw = (1 + _x(d, dtype=torch.float32, seed=s) / 8 for s in (2, 3))
+    theta = ora.angles(torch.arange(l, device="cuda").expand(b, l), f)
+    for y, x, w in zip(rotary.qk_norm_rope(q, k, qw, kw, table), (q, k), (qw, kw)):
+        z = ora.norm(x, w, 1e-6)
+        _close(y.transpose(1, 2), ora.turn(z, theta, True), ora.pair_size(z, d, True), 20)
+    _quiet()
