@@ -67,16 +67,6 @@ def _strides(t: torch.Tensor, order) -> list[int]:
     return [stride[d] if shape[d] > 1 else 0 for d in order]
 
 
-def _dense_strides(shape) -> list[int]:
-    """:func:`_strides` of all dimensions but the last of a contiguous tensor
-    (which the call allocates: a plan needs only its strides)."""
-    out, step = [], 1
-    for n in reversed(shape):
-        out.append(step if n > 1 else 0)
-        step *= max(n, 1)
-    return out[:0:-1]
-
-
 # Checked calls, by all that their checks look at (types, shapes, strides,
 # devices, options; no tensor, address or value): a call like an earlier one
 # is launched without checking it again.  Options enter as the numbers they
@@ -242,9 +232,11 @@ def _rope_plan(x, table, positions, interleaved, axes, inverse, start, out):
     b, l, h, d = x.shape
     dev = x.device
     (rows, p64, batch, first, ax), r, flags = _turns(table, positions, axes, b, l, d, interleaved, inverse, start, dev)
-    if out is not None:
+    if out is None:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    else:
         _check_out("out", out, x.shape, x.dtype, dev)
-    strides = _Six(*_strides(x, (0, 1, 2)), *(_dense_strides(x.shape) if out is None else _strides(out, (0, 1, 2))))
+    strides = _Six(*_strides(x, (0, 1, 2)), *_strides(out, (0, 1, 2)))
     return (x.numel() == 0, dev.index, DTYPES[x.dtype], rows, (p64, batch, first, ax, b, l, h, d, r, flags, strides))
 
 

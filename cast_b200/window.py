@@ -27,7 +27,7 @@ import math
 import torch
 
 from . import _lib
-from .rotary import DTYPES, _check, _check_out, _dense_strides, _keep, _launch, _refuse_gradients, _sig, _strides
+from .rotary import DTYPES, _check, _check_out, _keep, _launch, _refuse_gradients, _sig, _strides
 
 _TYPES = (torch.bfloat16, torch.float16)
 _Twelve = ctypes.c_longlong * 12
@@ -83,15 +83,16 @@ def _window_plan(q, k, v, window, sinks, frame_tokens, kv_lens, out):
     if kv_lens is not None:
         _lens(kv_lens, b, dev)
     rule = _rule(window, sinks, frame_tokens)
-    if out is not None:
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
         _check_out("out", out, q.shape, q.dtype, dev)
     if q.numel() == 0 or lk == 0:
         return q.numel() == 0, lk == 0, dev.index, 0, 0.0, (), ()
     shape = (b, hq, hk, lq, lk, d)
     n = _workspace_bytes("cast_window_attention_workspace_bytes", dev, *shape, *rule)
     order = (0, 1, 2)
-    strides = _Twelve(*_strides(q, order), *_strides(k, order), *_strides(v, order),
-                      *(_dense_strides(q.shape) if out is None else _strides(out, order)))
+    strides = _Twelve(*_strides(q, order), *_strides(k, order), *_strides(v, order), *_strides(out, order))
     return False, False, dev.index, n, 1.0 / math.sqrt(d), DTYPES[q.dtype], (*shape, strides, *rule)
 
 
@@ -151,15 +152,16 @@ def _paged_plan(q, k_pages, v_pages, block_table, kv_lens, window, sinks, frame_
         raise ValueError(f"block_table must be a contiguous int32 [{b}, max_pages], got {tuple(block_table.shape)}")
     _lens(kv_lens, b, dev)
     rule = _rule(window, sinks, frame_tokens)
-    if out is not None:
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
         _check_out("out", out, q.shape, q.dtype, dev)
     max_pages = block_table.shape[1]
     if q.numel() == 0 or max_pages * pages * page == 0:
         return q.numel() == 0, max_pages * pages * page == 0, dev.index, 0, 0.0, (), (), ()
     n = _workspace_bytes("cast_paged_window_attention_workspace_bytes", dev, b, hq, hk, lq, d, page, max_pages, *rule)
     order = (0, 1, 2)
-    strides = _Twelve(*_strides(q, order), *_strides(k_pages, order), *_strides(v_pages, order),
-                      *(_dense_strides(q.shape) if out is None else _strides(out, order)))
+    strides = _Twelve(*_strides(q, order), *_strides(k_pages, order), *_strides(v_pages, order), *_strides(out, order))
     return (False, False, dev.index, n, 1.0 / math.sqrt(d), DTYPES[q.dtype], (max_pages, pages, page),
             (b, hq, hk, lq, d, strides, *rule))
 

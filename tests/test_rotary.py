@@ -231,8 +231,3 @@ def test_gradients_of_both_modes_refused():
             rotary._refuse_gradients(x, None)
             with pytest.raises(ValueError, match="tangent"):  # no_grad does not end forward mode
                 rotary._refuse_gradients(None, forward_ad.make_dual(x, torch.ones(3)))
-
-
-@pytest.mark.parametrize("shape", [(2, 3, 4, 8), (1, 3, 4, 8), (2, 1, 1, 16), (1, 1, 1, 8), (3, 5, 1, 64)])
-def test_strides_of_an_output_that_is_not_there_yet(shape):
-    assert rotary._dense_strides(torch.Size(shape)) == rotary._strides(torch.empty(shape), (0, 1, 2))

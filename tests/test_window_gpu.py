@@ -468,22 +468,3 @@ def test_scores_that_are_nan_in_items_cut_into_parts(cuda, d, dtype, hq, hk, lq,
         got = window.window_attention(q, k, v, window=win, kv_lens=n, sinks=1)
         _check(got, q, k, v, lens, window=win, sinks=1, heads=some)
     _quiet()
-
-
-@pytest.mark.parametrize("lk", [2049, 2050])
-def test_a_call_of_a_new_shape_allocates_one_output(cuda, lk):
-    """A history that grows by a token is a new shape at every step."""
-    table = rotary.rope_table(rotary.rope_frequencies(128), lk)
-    q, k, v = _data(4, 16, 4, 128, lk, lk, BF16)
-    kp, vp, blocks = _pages(k, v, 64)
-    n = torch.full((4,), lk, dtype=torch.int32, device="cuda")
-    one = q.numel() * 2
-    for call in (lambda: rotary.rope(q.transpose(1, 2), table), lambda: window.window_attention(q, k, v, window=100),
-                 lambda: window.paged_window_attention(q, kp, vp, blocks, n, window=100)):
-        torch.cuda.synchronize()
-        torch.cuda.reset_peak_memory_stats()
-        before = torch.cuda.memory_allocated()
-        out = call()
-        assert torch.cuda.max_memory_allocated() - before < 1.5 * one
-        del out
-    _quiet()
