@@ -1403,7 +1403,7 @@ static RowsPlan rows_plan(long long B, int Hk, int group, int Lq, int capacity, 
   r.row_tiles = (int)((rows + tile - 1) / tile);
   const long long items = B * Hk * r.row_tiles;
   const long long tokens = std::min<long long>(Lq, tile / group + 2);
-  const double span = std::min<double>(capacity, (double)(window + sinks + 1) * frame + (double)tokens);
+  const double span = std::min<double>(capacity, ((double)window + (double)sinks + 1) * frame + (double)tokens);
   const long long most = std::max<long long>(1, (long long)(span / 128));
   const long long want = std::max<long long>(1, 2ll * n_sms / items);
   long long n = std::min(most, want);
@@ -1547,7 +1547,7 @@ static TilesPlan tiles_plan(int B, int Hq, int Hk, int Lq, int Lk, long long win
   t.q_tiles = (int)((rows + 127) / 128);
   t.n_items = B * t.head_groups * t.q_tiles;
   const double tokens = std::min<double>(Lq, 128.0 / t.pack);
-  const double keys = std::min<double>(Lk, (double)(window + sinks) * frame + tokens + (frame > 1 ? frame : 0));
+  const double keys = std::min<double>(Lk, ((double)window + (double)sinks) * frame + tokens + (frame > 1 ? frame : 0));
   const double c = std::max(1.0, keys / 128);
   const int waves = t.n_items / slots, rem = t.n_items % slots;
   t.n_whole = t.n_items;

@@ -468,3 +468,16 @@ def test_scores_that_are_nan_in_items_cut_into_parts(cuda, d, dtype, hq, hk, lq,
         got = window.window_attention(q, k, v, window=win, kv_lens=n, sinks=1)
         _check(got, q, k, v, lens, window=win, sinks=1, heads=some)
     _quiet()
+
+
+@pytest.mark.parametrize("lq", [2, 88])
+def test_plans_of_windows_of_any_size(cuda, lq):
+    """From C, window and sinks may be the largest numbers there are (their sum is not one)."""
+    lib, most = _lib.load(), (1 << 63) - 1
+
+    def need(win, sinks):
+        return lib.cast_window_attention_workspace_bytes(1, 2, 1, lq, 20000, 128, win, sinks, 1)
+
+    assert need(20000, 0) > 0
+    for win, sinks in ((most, most), (most, 1), (1, most), (most, 0)):
+        assert need(win, sinks) == need(20000, 0), (win, sinks)
