@@ -146,8 +146,10 @@ struct RotaryLane {
   static constexpr int kPairs = kHalf ? 8 : 4 * kC;  // table entries of a lane's columns
   float cs[kPairs], sn[kPairs];
   bool live, turns[kC];
+  bool blank;  // (without the norm) this token's position is unknown: it is read as zeros
   int c, h0, step, partner, second;  // second: columns from the first piece to the second
 
+  template <bool kBlank>
   __device__ __forceinline__ void load(const RotaryParams &p, const RotaryTensor &t, const InT *row, int hb,
                                        Eight<InT> (&raw)[kBatch][kC]) const {
     const InT *src = row + (long long)(hb + h0) * t.ss[2];
@@ -159,6 +161,13 @@ struct RotaryLane {
       }
       src += step * t.ss[2];
     }
+    if (kBlank && blank) clear(raw);
+  }
+  __device__ __forceinline__ void clear(Eight<InT> (&raw)[kBatch][kC]) const {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+      for (int j = 0; j < kC; ++j) raw[u][j] = Eight<InT>{};
   }
   // Zeros in place of a tensor's heads.
   __device__ __forceinline__ void zeros(const RotaryTensor &t, OutT *at, long long at_step) const {
@@ -197,7 +206,7 @@ struct RotaryLane {
     const bool normed = kNorm && kTurn && t.weight != nullptr;
     if (normed && live && !p.weight_per_head) weight(0);
     for (int hb = 0; hb < t.heads; hb += step * kBatch) {  // same trip count in the whole CTA
-      if (hb > 0) load(p, t, row, hb, raw);
+      if (hb > 0) load<kTurn && !kNorm>(p, t, row, hb, raw);
       OutT *dst = at + (long long)(hb + h0) * at_step;
 #pragma unroll
       for (int u = 0; u < kBatch; ++u, dst += step * at_step) {
@@ -306,7 +315,8 @@ __global__ void __launch_bounds__(kRotaryThreads, rotary_ctas(kC)) rotary_kernel
     }
 
     // on its way while the position and then its table row are fetched
-    f.load(p, p.t[0], src[0] + l * p.t[0].ss[1], 0, raw);
+    f.blank = false;
+    f.template load<false>(p, p.t[0], src[0] + l * p.t[0].ss[1], 0, raw);
 
     // ---- this lane's (cos, sin): none where its columns are not rotated
     if (p.R > 0) {
@@ -333,12 +343,22 @@ __global__ void __launch_bounds__(kRotaryThreads, rotary_ctas(kC)) rotary_kernel
         }
       }
       if (__any_sync(0xffffffffu, !known)) {
-        if (!known) {  // zeros, and said so; what this token's q and k come to is left unwritten
+        // Zeros, and said so.  Under a norm, whose weight may be an infinity or NaN,
+        // what this token's q and k come to is left unwritten; else they are zeros
+        // that are not turned.
+        if (!known) {
           pos[0] = pos[1] = pos[2] = 0;
           if (c == 0 && f.h0 == 0) atomicExch(err, (int)CAST_ERR_INVALID_ARGUMENT);
-          f.zeros(p.t[0], dst[0] + l * p.t[0].ds[1], p.t[0].ds[2]);
-          if (!p.slots) f.zeros(p.t[1], dst[1] + l * p.t[1].ds[1], p.t[1].ds[2]);
-          f.live = false;
+          if constexpr (kNorm) {
+            f.zeros(p.t[0], dst[0] + l * p.t[0].ds[1], p.t[0].ds[2]);
+            if (!p.slots) f.zeros(p.t[1], dst[1] + l * p.t[1].ds[1], p.t[1].ds[2]);
+            f.live = false;
+          } else {
+            f.blank = true;
+            f.clear(raw);
+#pragma unroll
+            for (int j = 0; j < kC; ++j) f.turns[j] = false;
+          }
         }
       }
       if (any_turns) {
@@ -375,7 +395,7 @@ __global__ void __launch_bounds__(kRotaryThreads, rotary_ctas(kC)) rotary_kernel
     f.template run<true>(p, p.t[0], src[0] + l * p.t[0].ss[1], dst[0] + l * p.t[0].ds[1], p.t[0].ds[2], raw);
     if (p.t[1].heads == 0) continue;  // uniform
 
-    f.load(p, p.t[1], src[1] + l * p.t[1].ss[1], 0, raw);
+    f.template load<!kNorm>(p, p.t[1], src[1] + l * p.t[1].ss[1], 0, raw);
     if (!p.slots) {
       f.template run<true>(p, p.t[1], src[1] + l * p.t[1].ss[1], dst[1] + l * p.t[1].ds[1], p.t[1].ds[2], raw);
       continue;
@@ -393,14 +413,14 @@ __global__ void __launch_bounds__(kRotaryThreads, rotary_ctas(kC)) rotary_kernel
     }
     const long long head = (long long)p.page * p.D;
     const bool column = live_token && 8 * kC * c < p.D;
-    if (column && !f.live) {
+    if (kNorm && column && !f.live) {
       f.live = true;
       if (place >= 0) f.zeros(p.t[1], dst[1] + place, head);
       f.live = false;
     }
     f.template run<true>(p, p.t[1], src[1] + l * p.t[1].ss[1], place < 0 ? nullptr : dst[1] + place, head, raw);
-    f.live = column;  // (the value is copied whatever the position)
-    f.load(p, p.t[2], src[2] + l * p.t[2].ss[1], 0, raw);
+    if (kNorm) f.live = column;  // (the value is copied whatever the position)
+    f.template load<false>(p, p.t[2], src[2] + l * p.t[2].ss[1], 0, raw);
     f.template run<false>(p, p.t[2], src[2] + l * p.t[2].ss[1], place < 0 ? nullptr : dst[2] + place, head, raw);
   }
 }

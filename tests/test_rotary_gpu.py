@@ -390,3 +390,30 @@ def test_head_counts_around_a_batch_of_three_a_lane(cuda, dtype, b, l, hq, hk, d
         z = ora.norm(x, w, 1e-6)
         _close(y.transpose(1, 2), ora.turn(z, theta, True), ora.pair_size(z, d, True), 20)
     _quiet()
+
+
+@pytest.mark.parametrize("normed", [False, True])
+@pytest.mark.parametrize("hq,hk,l", [(2, 40, 3), (24, 24, 3), (24, 24, 2500), (3, 1, 4)])
+def test_values_of_unknown_positions_are_copied(cuda, normed, hq, hk, l):
+    """However many heads a lane takes one after the other; keys and queries are zeros."""
+    d = 128
+    table = rotary.rope_table(rotary.rope_frequencies(d), 10)
+    x = _x(1, l, hq + 2 * hk, d, dtype=torch.bfloat16)
+    q, k, v = x[:, :, :hq], x[:, :, hq:hq + hk], x[:, :, hq + hk:]
+    pos = torch.randint(0, 10, (l,), device="cuda")
+    pos[1], pos[2] = 10, -7
+    w = torch.full((d,), float("inf"), device="cuda") if normed else None
+    kp = torch.full((l // 4 + 1, hk, 4, d), 3.0, dtype=torch.bfloat16, device="cuda")
+    vp = kp.clone()
+    slots = torch.randperm(l, device="cuda")[None]
+    got, _ = rotary.qk_norm_rope(q, k, w, w, table, pos, v=v, cache=(kp, vp), slots=slots)
+    s = slots[0]
+    assert torch.equal(vp[s // 4, :, s % 4], v[0])
+    assert (got[0, :, 1:3] == 0).all() and (kp[s[1:3] // 4, :, s[1:3] % 4] == 0).all()
+    if not normed:
+        plain = rotary.qk_norm_rope(q, k, None, None, table, pos)
+        assert torch.equal(got, plain[0]) and torch.equal(kp[s // 4, :, s % 4], plain[1][0].transpose(0, 1))
+        assert torch.isfinite(got).all() and (got[0, :, 0] != 0).any()
+    with pytest.raises(CastError):
+        _quiet()
+    _quiet()
