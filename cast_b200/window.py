@@ -106,8 +106,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     ``window=None``: every earlier key.  ``kv_lens``: int32 ``[B]``, the keys
     of each session (default Lk; the queries are its last Lq positions, and
     rows of k and v behind them are never used, whatever they hold).
-    ``sm_scale`` defaults to ``1/sqrt(D)``.  Returns ``[B,Hq,Lq,D]``; a query
-    that sees nothing gives zeros.  A length outside ``[0, Lk]`` is clipped
+    ``sm_scale`` defaults to ``1/sqrt(D)``.  Returns ``[B,Hq,Lq,D]`` (``out``
+    may be ``q``; it must not overlap k or v); a query that sees nothing gives
+    zeros, one that sees a NaN score NaN.  A length outside ``[0, Lk]`` is clipped
     and sets the device error word.
     """
     window, sinks, frame_tokens = _options(window, sinks, frame_tokens)

@@ -481,3 +481,53 @@ def test_plans_of_windows_of_any_size(cuda, lq):
     assert need(20000, 0) > 0
     for win, sinks in ((most, most), (most, 1), (1, most), (most, 0)):
         assert need(win, sinks) == need(20000, 0), (win, sinks)
+
+
+FORMS = [(1, 8, 2, 128, 1, 200), (1, 2, 1, 64, 3, 3000), (1, 2, 1, 128, 4, 30000), (1, 4, 1, 64, 7, 4000),
+         (2, 4, 2, 128, 150, 700), (1, 2, 1, 64, 90, 20000), (1, 4, 2, 128, 600, 600)]
+
+
+@pytest.mark.parametrize("b,hq,hk,d,lq,lk", FORMS)
+def test_scores_that_are_not_finite(cuda, b, hq, hk, d, lq, lk):
+    """NaN and +infinity in queries and keys make the rows that see them NaN, in
+    every way a call is cut; -infinity hides a key."""
+    q, k, v = _data(b, hq, hk, d, lq, lk, BF16, seed=lk)
+    q[0, 0, 0, 1] = float("nan")
+    k[0, 0, lk - 1] = float("nan")                       # the last row's
+    k[b - 1, hk - 1, lk // 2] = float("-inf")
+    q[b - 1, hq - 1, lq - 1].abs_()                      # q.k = -infinity
+    for win in (None, lk // 3 + lq):
+        got = window.window_attention(q, k, v, window=win)
+        _check(got, q, k, v, None, window=win)
+    q[0, 0, 0, 1] = float("inf")
+    k[0, 0, lk - 1] = 1.0
+    k[b - 1, hk - 1, lk // 2] = 1.0
+    got = window.window_attention(q, k, v, window=None)
+    _check(got, q, k, v, None, window=None)
+    kp, vp, table = _pages(k, v, 64)
+    n = torch.full((b,), lk, dtype=torch.int32, device="cuda")
+    _check(window.paged_window_attention(q, kp, vp, table, n, window=None), q, k, v, None, window=None)
+    _quiet()
+
+
+@pytest.mark.parametrize("b,hq,hk,d,lq,lk", FORMS)
+def test_out_may_be_q(cuda, b, hq, hk, d, lq, lk):
+    q, k, v = _data(b, hq, hk, d, lq, lk, BF16, seed=lk)
+    want = window.window_attention(q, k, v, window=None)
+    kp, vp, table = _pages(k, v, 64)
+    n = torch.full((b,), lk, dtype=torch.int32, device="cuda")
+    paged = window.paged_window_attention(q, kp, vp, table, n, window=None)
+    for _ in range(3):
+        x, y = q.clone(), q.transpose(1, 2).clone().transpose(1, 2)
+        assert torch.equal(window.window_attention(x, k, v, window=None, out=x), want)
+        assert torch.equal(window.window_attention(y, k, v, window=None, out=y), want)
+        y.copy_(q)
+        assert torch.equal(window.paged_window_attention(y, kp, vp, table, n, window=None, out=y), paged)
+
+
+def test_an_option_that_changes_in_place(cuda):
+    q, k, v = _data(1, 2, 1, 64, 5, 90, BF16)
+    win, sinks = torch.tensor(9), torch.tensor(0)
+    for w, s in ((9, 0), (30, 0), (30, 4)):
+        win.fill_(w), sinks.fill_(s)
+        _check(window.window_attention(q, k, v, window=win, sinks=sinks), q, k, v, None, window=w, sinks=s)
