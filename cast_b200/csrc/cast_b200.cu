@@ -1388,12 +1388,14 @@ struct RowsPlan {
   size_t ws_bytes = 0;
 };
 
-// How the few-row kernel cuts a call.  Two of its CTAs fit on an SM, so the
-// keys of a tile of rows are split until there are two CTAs for each SM, or
-// until a part has 128 keys (little more than one step of its warps).  More
-// and smaller parts lose: 16 sessions x 8 key heads take 80.6 us in 2 parts
-// each, 85.4 in 4; 64 x 8 take 160 in 1, 173 in 2.  Up to eight parts are
-// joined in a cluster; more go through the workspace.
+// How the few-row kernel cuts a call.  The keys of a tile of rows are split
+// until there are two CTAs for each SM, or until a part has 128 keys (little
+// more than one step of its warps).  More and smaller parts lose: 16 sessions
+// x 8 key heads take 80.6 us in 2 parts each, 85.4 in 4; 64 x 8 take 160 in 1,
+// 173 in 2.  Two CTAs do fit on an SM for up to 16 rows, and for heads of 64;
+// of 17 to 32 rows of heads of 128 one does, which the count does not follow:
+// such calls run in two waves.  Up to eight parts are joined in a cluster; more
+// go through the workspace.
 static RowsPlan rows_plan(long long B, int Hk, int group, int Lq, int capacity, long long window,
                           long long sinks, int frame, int D, int n_sms) {
   RowsPlan r;
@@ -1533,10 +1535,11 @@ struct TilesPlan {
 // How the many-row kernel cuts a call: an item is a query tile of one head
 // group, and two CTAs run on an SM.  The items of the last, incomplete wave
 // (or of the last two) are cut along their keys into equal parts where that
-// ends sooner, counted in steps of 128 keys (1.5 us with two CTAs on the SM):
-// an item costs its keys and about 4 steps to start and end, a part one more
-// to leave its result, and the second launch that joins them 3 and a little
-// for each part's 64 KB.
+// ends sooner, counted in 128 keys, two steps of the kernel (1.5 us with two
+// CTAs on the SM): an item costs its keys and about 4 such to start and end, a
+// part one more to leave its result, and the second launch that joins them 3
+// and a little for each part's 64 KB.  The costs are those of heads of 128; heads
+// of 64 (four CTAs on the SM) are counted alike.
 static TilesPlan tiles_plan(int B, int Hq, int Hk, int Lq, int Lk, long long window, long long sinks, int frame,
                             int D, int n_sms) {
   TilesPlan t;
@@ -1571,8 +1574,14 @@ static TilesPlan tiles_plan(int B, int Hq, int Hk, int Lq, int Lk, long long win
   return t;
 }
 
-// Rows that a tile of the many-row kernel would hold mostly empty go to the
-// few-row kernel.
+// More than 32 rows of a key head go to the many-row kernel, whatever part of
+// its tiles they fill (a tile has the rows of `pack` heads, a power of two, and
+// a key head whose group is not one is read once for each pack).  Measured, many
+// rows against few, us: heads of 128, 24 / 8 heads, 16 queries over 4096 keys 15.7
+// against 28.1; 28 / 4, 8 queries over 4096 16.8 against 23.4, over 4 x 1000 17.2
+// against 15.1; 66 / 2, 1 query over 30000 114 against 34, 16 queries 114 against
+// 238; heads of 64, 24 / 8, 16 queries over 4096 19.7 against 15.3, 64 queries
+// 19.7 against 26.4; 28 / 4, 8 queries over 30000 52 against 25.
 static bool tiles_wanted(long long rows) { return rows > 32; }
 
 // A tiled map of 16-bit elements (strides in elements; the first dimension

@@ -22,10 +22,15 @@
 // are loaded before the first is worked on.
 //
 // Measured (B200, graph over rotating inputs): rotation alone, 31680 tokens of
-// 24 heads of 128 bf16, 65.9 us = 5.9 TB/s, 0.90 of the measured copy; with
-// the norm, 3520 tokens of 24 + 24 heads, 22.7 us = 3.8 TB/s: about 200
-// instructions a head and 16 lanes, where the rotation alone takes 150 (half of
-// it position and table row).
+// 24 heads of 128 bf16, 66 us = 5.9 TB/s, 0.90 of the measured copy; 12500 in
+// float32 55 us = 5.6 TB/s, 0.85; with the norm, 3520 tokens of 24 + 24 heads,
+// 24.1 us = 3.6 TB/s, 0.55: about 200 instructions a head and 16 lanes (58 % of
+// the issue slots), where the rotation alone takes 150 (half of it position
+// and table row).  The norm's kernels spill: a head's values, the weight in
+// pairs, (cos, sin) and 64-bit pointers are more than the 64 or 72 registers
+// below.  Bytes stored / loaded a thread: one piece, pairs side by side,
+// 16-bit 190 / 190 and float32 380 / 280; half layout 330 / 220 and 540 / 550;
+// two pieces 1000 / 500 and 1400 to 1700 / 1000 to 1400.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -44,9 +49,11 @@ __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
 
 constexpr int kRotaryThreads = 128;
 constexpr int kRotaryRun = 4;  // tokens a lane takes one after the other
-// Heads in flight per lane of one piece or two, and CTAs on an SM: registers
-// for more of either cost more than they give (one piece: 4 heads and 6 CTAs
-// are level; two pieces: 3 heads and 6 CTAs take 94 us where 2 and 7 take 69).
+// Heads in flight per lane of one piece or two, and CTAs on an SM.  Under the
+// norm both counts spill (see above), and these are the best of the counts
+// tried, not the best there could be without spills (one piece: 4 heads and
+// 6 CTAs are level; two pieces: 3 heads and 6 CTAs take 94 us where 2 and 7
+// take 69).
 constexpr int rotary_batch(int pieces) { return pieces == 2 ? 2 : 3; }
 constexpr int rotary_ctas(int pieces) { return pieces == 2 ? 7 : 8; }
 

@@ -200,9 +200,10 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // --------------------------------------------------------------- few rows
 // Warps of a CTA and stages of each warp's ring.  A warp's step is a chain of
 // latencies (products, shuffles, exponentials), so warps count for more than
-// copies far ahead: six warps of two stages, two CTAs an SM (96 KB each), take
-// 80.6 us for 16 sessions x 8 key heads x 8208 keys of 128 (the copy rate);
-// four of three 81.5, four of two (three CTAs) 87.2, eight of two 87.6.
+// copies far ahead.  16 sessions x 8 key heads x 8208 keys of 128, in one series
+// of runs: six warps of two stages, two CTAs an SM (102 KB each), 80.6 us; four
+// of three 81.5; four of two (three CTAs) 87.2; eight of two 87.6.  17 to 32 rows
+// of heads of 128 (254 registers a thread, 116 KB) leave room for one CTA alone.
 constexpr int kRowsWarps = 6;
 constexpr int kRowsStages = 2;
 constexpr int kRowsMaxCluster = 8;
@@ -236,8 +237,10 @@ struct RowsParams {
 // window_rows_join_kernel.  The order of every sum is fixed.
 //
 // Bound: HBM, each key and value once, where there are keys enough: 16 sessions
-// of 8 key heads, 8208 keys of 128 in pages of 64, 81.5 us = 6.5 TB/s (0.99 of
-// the measured copy); small calls by latency: 24 heads, 1088 keys, 7.4 us.
+// of 8 key heads, 8208 keys of 128 in pages of 64, 83.5 us = 6.3 TB/s (0.97 of
+// the measured copy); small calls by latency: 24 heads, 1088 keys, 8.2 us; 17 to
+// 32 rows of heads of 128 by the one CTA an SM: 28 query and 4 key heads,
+// 8 queries over 30000 keys, 50 us = 1.2 TB/s.
 // mma.sync serves here: with 16 rows or fewer the products are a tenth of the
 // time, and their operands go through registers with no descriptor or TMEM
 // traffic.

@@ -27,11 +27,15 @@
 // that only some see, infinities and NaN become zeros and are given back to
 // the rows that see them when these are written.
 //
-// Bound: the softmax warps' steps.  Measured (bf16, heads of 128): 24 heads of
-// 3520 queries over 9 frames of 880, 312 us = 1.10 PFLOP/s of visible pairs
-// (0.68 of the measured bf16 peak; exponentials 0.57 of their pipe, tensor pipe
-// 0.55); 32 / 8 heads, 8192 queries, window 1024, 4 sinks: 157 us; heads of 64,
-// fp16, 3 x 1001 queries over 777 keys: 28 us.
+// Bound: the softmax warps' steps.  Measured (bf16, heads of 128, in a graph;
+// in brackets calls one after the other): 24 heads of 3520 queries over 9
+// frames of 880, 311 to 337 us (365: the power cap) = 1.10 PFLOP/s of visible
+// pairs, 0.68 of the measured bf16 peak (exponentials 0.57 of their pipe, tensor
+// pipe 0.55); 32 / 8 heads, 8192 queries, window 1024, 4 sinks: 155 us (174), of
+// which about a quarter is the start and end of items of 18 steps.  Heads of 64
+// are bound by one S buffer a CTA, whose step is one chain: fp16, 16 / 4 heads,
+// 3 x 1001 queries over 777 keys, 29 us (30), 384 items on 592 places in one wave
+// (exponentials 0.38 of their pipe, tensor pipe 0.15).
 #pragma once
 
 #include "window.cuh"
@@ -116,8 +120,9 @@ struct TilesType<__nv_bfloat16> {
 };
 template <>
 struct TilesType<__half> {
-  // P = 2^(s - m + 8): a step's P sum to 2^15 at most before the maximum
-  // moves, and weights down to 2^-32 of the largest count
+  // P = 2^(s - m + 8): none is above 2^12 without a move of the maximum (a chunk
+  // of P that sums to more than 2^15 is looked at again), and weights down to
+  // 2^-32 of the largest count
   static constexpr uint32_t fmt = 0;
   static constexpr float kShift = 8.0f, kSlack = 4.0f, kSumLimit = 32768.0f;
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return Half2<__half>::pack(a, b); }

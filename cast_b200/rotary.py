@@ -130,7 +130,9 @@ def rope_frequencies(rotary_dim: int, *, base: float = 10000.0, axes=None, scali
     * ``("yarn", f, length)`` or ``("yarn", f, length, fast, slow)``: a pair
       that turns more than ``fast`` (32) times over the ``length`` learned
       positions keeps its step, one that turns less than ``slow`` (1) times is
-      divided by ``f``, the pairs between blend linearly in their index.
+      divided by ``f``, the pairs between blend linearly in their index (from
+      the last whole index that is kept to the first that is divided, which may
+      lie past the last pair, at the axis' last value at most).
     """
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError("rotary_dim must be even and positive")

@@ -1,6 +1,6 @@
 """Rotary positions and the norm of query / key heads in 64 bits.
 
-TEST INFRASTRUCTURE ONLY: the checker for ``cast_rope`` and
+TEST INFRASTRUCTURE ONLY: the oracle of ``cast_rope`` and
 ``cast_qk_norm_rope``; nothing in the product imports it.  Written from the
 formulas, with complex products for the turned pairs.
 """

@@ -1,6 +1,6 @@
 """Sliding-window attention with sinks in 64 bits.
 
-TEST INFRASTRUCTURE ONLY: the checker for ``cast_window_attention`` and
+TEST INFRASTRUCTURE ONLY: the oracle of ``cast_window_attention`` and
 ``cast_paged_window_attention``; nothing in the product imports it.
 """
 
